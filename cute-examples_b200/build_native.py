@@ -17,6 +17,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -24,11 +25,12 @@ REPO = HERE.parent
 PKG = HERE / "gemm_kernels"
 CSRC = HERE / "csrc"
 LIB = PKG / "libgemm_sm100.so"
+OBJ = HERE / "build"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17", "--restrict",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -76,14 +78,20 @@ def ext_path() -> Path:
 
 
 def build_kernel_library(force: bool = False, verbose: bool = False) -> Path:
-    sources = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [REPO / "include" / "gemm_sm100.h"]
-    if not force and _newer(LIB, sources):
+    """One object per .cu file, compiled side by side and only when the file or a header is newer."""
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO / "include" / "gemm_sm100.h"]
+    sources = sorted(CSRC.glob("*.cu"))
+    OBJ.mkdir(exist_ok=True)
+    objects = [OBJ / (s.stem + ".o") for s in sources]
+    stale = [(s, o) for s, o in zip(sources, objects) if force or not _newer(o, [s, *headers])]
+    if not stale and _newer(LIB, objects):
         return LIB
-    cmd = [_nvcc(), *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", str(LIB)] + [str(s) for s in sorted(CSRC.glob("*.cu"))]
-    _run(cmd, verbose)
+    flags = NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else [])
+    with ThreadPoolExecutor(max_workers=max(1, len(stale))) as pool:
+        jobs = [pool.submit(_run, [_nvcc(), *flags, "-c", str(s), "-o", str(o)], verbose) for s, o in stale]
+        for job in jobs:
+            job.result()
+    _run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(LIB), *(str(o) for o in objects)], verbose)
     return LIB
 
 

@@ -180,6 +180,158 @@ void gemm_tn_fanout(const torch::Tensor A, const torch::Tensor B, const std::vec
   raise_for(rc, cuda_error, "gemm_tn_fanout");
 }
 
+// ---------------------------------------------------------------- low-rank adapters
+// Fills `buffer` (torch memory of gemm_sm100_lora_plan_bytes) with what the adapter products need to
+// know about the rows of a batch; see gemm_sm100_lora_plan.
+void lora_plan(const torch::Tensor ids, int64_t adapters, torch::Tensor buffer) {
+  TORCH_CHECK(ids.dim() == 1, "ids must be a 1D tensor with one adapter index per row");
+  TORCH_CHECK(ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64, "ids must be int32 or int64");
+  TORCH_CHECK(ids.is_contiguous(), "ids must be contiguous");
+  TORCH_CHECK(ids.is_cuda() && buffer.is_cuda() && ids.device() == buffer.device(),
+              "ids must be a CUDA tensor on the plan's device");
+  c10::cuda::CUDAGuard guard(ids.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(ids.device().index()).stream();
+  int cuda_error = 0;
+  const int rc = gemm_sm100_lora_plan(ids.const_data_ptr(), ids.scalar_type() == torch::kInt64 ? 1 : 0,
+                                      static_cast<int>(ids.size(0)), static_cast<int>(adapters),
+                                      buffer.mutable_data_ptr(), static_cast<size_t>(buffer.numel()),
+                                      static_cast<void*>(stream), &cuda_error);
+  raise_for(rc, cuda_error, "lora_plan");
+}
+
+namespace {
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+// Row pitch of the last two dimensions (the stride of a single row is not meaningful).
+long pitch(const torch::Tensor& t) {
+  return t.size(-2) > 1 ? static_cast<long>(t.stride(-2)) : static_cast<long>(t.size(-1));
+}
+long matrix_stride(const torch::Tensor& t) {
+  return t.size(0) > 1 ? static_cast<long>(t.stride(0)) : static_cast<long>(t.size(1) * t.size(2));
+}
+void check_like(const torch::Tensor& t, const char* name, const torch::Tensor& like, std::vector<int64_t> shape,
+                bool contiguous = false) {
+  TORCH_CHECK(t.sizes() == c10::IntArrayRef(shape), name, " must be of shape ", c10::IntArrayRef(shape), ", got ", t.sizes());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the same dtype as the other tensors");
+  TORCH_CHECK(t.size(-1) <= 1 || t.numel() == 0 || t.stride(-1) == 1, name, " must have unit stride along its last dimension");
+  TORCH_CHECK(!contiguous || t.is_contiguous(), name, " must be contiguous");
+}
+void check_placed(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), "All tensors must be CUDA tensors (", name, ")");
+  TORCH_CHECK(t.device() == like.device(), "All tensors must be on the same device (", name, ")");
+}
+
+// Shapes and types of what both passes share; fills everything but the plan's contents.
+gemm_sm100_lora_args lora_args(const torch::Tensor& A, const torch::Tensor& B, const torch::Tensor& down,
+                               const torch::Tensor& up, const torch::Tensor& plan, int64_t plan_rows,
+                               int64_t plan_adapters, const OptTensor& scales, double scale) {
+  TORCH_CHECK(A.dim() == 2 && B.dim() == 2, "A and B must be 2D (matrix) tensors");
+  TORCH_CHECK(down.dim() == 3 && up.dim() == 3, "down and up must be 3D tensors: [adapters, R, K] and [adapters, N, R]");
+  const int64_t M = A.size(0), K = A.size(1), N = B.size(0), G = down.size(0), R = down.size(1);
+  TORCH_CHECK(B.size(1) == K, "Inner dimensions of A and B must match (A: ", K, ", B: ", B.size(1), ")");
+  gemm_sm100_lora_args a = {};
+  a.dtype = dtype_code(A);
+  check_like(A, "A", A, {M, K});
+  check_like(B, "B", A, {N, K});
+  check_like(down, "down", A, {G, R, K});
+  check_like(up, "up", A, {G, N, R});
+  TORCH_CHECK(plan_rows == M, "the plan is for ", plan_rows, " rows, A has ", M);
+  TORCH_CHECK(plan_adapters == G, "the plan is for ", plan_adapters, " adapters, down and up hold ", G);
+  TORCH_CHECK(R >= 8 && R % 8 == 0 && R <= GEMM_SM100_LORA_MAX_RANK, "the rank must be a multiple of 8 up to ",
+              GEMM_SM100_LORA_MAX_RANK, ", got ", R);
+  TORCH_CHECK(K > 0 && N > 0 && K % 8 == 0, "K must be a positive multiple of 8 and N positive (K: ", K, ", N: ", N, ")");
+  TORCH_CHECK(M <= INT32_MAX && N <= INT32_MAX && K <= INT32_MAX, "extents must fit in 32 bits");
+  if (scales.has_value()) {
+    TORCH_CHECK(scales->dim() == 1 && scales->size(0) == G && scales->scalar_type() == torch::kFloat32 && scales->is_contiguous(),
+                "scale must be a number or a contiguous float32 tensor with one value per adapter");
+    a.scales = static_cast<const float*>(scales->const_data_ptr());
+  }
+  for (const auto& t : {std::make_pair(&A, "A"), std::make_pair(&B, "B"), std::make_pair(&down, "down"),
+                        std::make_pair(&up, "up"), std::make_pair(&plan, "plan")})
+    check_placed(*t.first, t.second, A);
+  if (scales.has_value()) check_placed(*scales, "scale", A);
+  a.M = static_cast<int>(M), a.N = static_cast<int>(N), a.K = static_cast<int>(K);
+  a.R = static_cast<int>(R), a.adapters = static_cast<int>(G);
+  a.A = A.const_data_ptr(), a.B = B.const_data_ptr(), a.down = down.const_data_ptr(), a.up = up.const_data_ptr();
+  a.lda = pitch(A), a.ldb = pitch(B), a.ld_down = pitch(down), a.ld_up = pitch(up);
+  a.stride_down = matrix_stride(down), a.stride_up = matrix_stride(up);
+  a.scale = static_cast<float>(scale);
+  a.plan = plan.const_data_ptr();
+  return a;
+}
+
+}  // namespace
+
+torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torch::Tensor down, const torch::Tensor up,
+                        const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters, const OptTensor scales,
+                        double scale, torch::Tensor C, torch::Tensor low) {
+  const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
+  check_like(C, "out", A, {a.M, a.N});
+  check_like(low, "low", A, {a.M, a.R});
+  check_placed(C, "out", A);
+  check_placed(low, "low", A);
+  if (a.M == 0) return C;
+  c10::cuda::CUDAGuard guard(A.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(A.device().index()).stream();
+  int cuda_error = 0;
+  int rc;
+  {
+    pybind11::gil_scoped_release release;
+    rc = gemm_sm100_lora(&a, C.mutable_data_ptr(), pitch(C), low.mutable_data_ptr(), pitch(low), static_cast<void*>(stream),
+                         &cuda_error);
+  }
+  raise_for(rc, cuda_error, "gemm_lora");
+  return C;
+}
+
+// `low` undefined: the low-rank rows are computed again.  dA, d_down, d_up undefined: not wanted.
+void gemm_lora_backward(const torch::Tensor dC, const torch::Tensor A, const torch::Tensor B, const torch::Tensor down,
+                        const torch::Tensor up, const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters,
+                        const OptTensor scales, double scale, const OptTensor low, const OptTensor dA,
+                        const OptTensor d_down, const OptTensor d_up) {
+  const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
+  TORCH_CHECK(dC.dim() == 2, "dC must be a 2D (matrix) tensor");
+  check_like(dC, "dC", A, {a.M, a.N});
+  check_placed(dC, "dC", A);
+  TORCH_CHECK(a.N % 8 == 0, "N must be a multiple of 8 (it is the inner dimension of dC * B), got ", a.N);
+  if (low.has_value()) {
+    check_like(*low, "low", A, {a.M, a.R});
+    check_placed(*low, "low", A);
+  }
+  if (dA.has_value()) check_like(*dA, "dA", A, {a.M, a.K}), check_placed(*dA, "dA", A);
+  if (d_down.has_value()) check_like(*d_down, "d_down", A, {a.adapters, a.R, a.K}, true), check_placed(*d_down, "d_down", A);
+  if (d_up.has_value()) check_like(*d_up, "d_up", A, {a.adapters, a.N, a.R}, true), check_placed(*d_up, "d_up", A);
+  c10::cuda::CUDAGuard guard(A.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(A.device().index()).stream();
+  // scratch from the caching allocator: safe in stream order, and part of the graph's own memory under capture
+  const auto options = torch::TensorOptions().dtype(A.scalar_type()).device(A.device());
+  torch::Tensor d_low, low_rows;
+  if (dA.has_value() || d_down.has_value()) d_low = torch::empty({a.M, a.R}, options);
+  int cuda_error = 0;
+  int rc = GEMM_SM100_OK;
+  const char* what = "gemm_lora_backward";
+  if (low.has_value()) {
+    low_rows = *low;
+  } else if (d_up.has_value()) {
+    low_rows = torch::empty({a.M, a.R}, options);
+  }
+  {
+    pybind11::gil_scoped_release release;
+    if (!low.has_value() && d_up.has_value())
+      rc = gemm_sm100_lora_low(&a, low_rows.mutable_data_ptr(), a.R, static_cast<void*>(stream), &cuda_error);
+    if (rc == GEMM_SM100_OK)
+      rc = gemm_sm100_lora_backward(&a, dC.const_data_ptr(), pitch(dC), low_rows.defined() ? low_rows.const_data_ptr() : nullptr,
+                                    low_rows.defined() ? pitch(low_rows) : a.R,
+                                    d_low.defined() ? d_low.mutable_data_ptr() : nullptr, a.R,
+                                    dA.has_value() ? dA->mutable_data_ptr() : nullptr, dA.has_value() ? pitch(*dA) : a.K,
+                                    d_down.has_value() ? d_down->mutable_data_ptr() : nullptr,
+                                    d_up.has_value() ? d_up->mutable_data_ptr() : nullptr, static_cast<void*>(stream),
+                                    &cuda_error);
+  }
+  raise_for(rc, cuda_error, what);
+}
+
 // Waits for the current device and raises if a kernel reported a timed-out wait.
 unsigned int device_status() {
   unsigned int word = 0;
@@ -242,6 +394,17 @@ PYBIND11_MODULE(_C, m) {
         pybind11::arg("C"));
   m.def("gemm_tn_fanout", &gemm_tn_fanout, "A * B^T stored into several outputs given as device addresses",
         pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("output_ptrs"), pybind11::arg("ldc"));
+  m.def("lora_plan", &lora_plan, "Prepares which adapter each row of a batch uses", pybind11::arg("ids"),
+        pybind11::arg("adapters"), pybind11::arg("buffer"));
+  m.def("lora_plan_bytes", &gemm_sm100_lora_plan_bytes, pybind11::arg("M"), pybind11::arg("adapters"));
+  m.def("gemm_lora", &gemm_lora, "C = A * B^T + low * up^T, low = scale * A * down^T with the adapter of each row",
+        pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("down"), pybind11::arg("up"), pybind11::arg("plan"),
+        pybind11::arg("plan_rows"), pybind11::arg("plan_adapters"), pybind11::arg("scales"), pybind11::arg("scale"),
+        pybind11::arg("C"), pybind11::arg("low"));
+  m.def("gemm_lora_backward", &gemm_lora_backward, "Gradients of gemm_lora", pybind11::arg("dC"), pybind11::arg("A"),
+        pybind11::arg("B"), pybind11::arg("down"), pybind11::arg("up"), pybind11::arg("plan"), pybind11::arg("plan_rows"),
+        pybind11::arg("plan_adapters"), pybind11::arg("scales"), pybind11::arg("scale"), pybind11::arg("low"),
+        pybind11::arg("dA"), pybind11::arg("d_down"), pybind11::arg("d_up"));
   m.def("device_status", &device_status,
         "Synchronise the current device and raise if a GEMM kernel reported a failed wait");
   m.def("init", &init, "One-time set-up of the current device; call before capturing a CUDA graph");

@@ -156,9 +156,10 @@ class HostGemm:
         return C_host
 
 
+from .lora import LoraPlan, gemm_lora, gemm_lora_backward  # noqa: E402
 from .nsplit import FusedNSplit, NSplitPlan, fanout_pointers, gemm_tn_nsplit, shard_rows  # noqa: E402
 
 __all__ = [
-    "gemm_tn_test", "gemm_tn", "gemm_nn", "gemm", "HostGemm", "gemm_tn_fanout", "gemm_tn_nsplit", "FusedNSplit", "NSplitPlan", "shard_rows", "device_status",
+    "gemm_tn_test", "gemm_tn", "gemm_nn", "gemm", "LoraPlan", "gemm_lora", "gemm_lora_backward", "HostGemm", "gemm_tn_fanout", "gemm_tn_nsplit", "FusedNSplit", "NSplitPlan", "shard_rows", "device_status",
     "init", "set_option", "set_trace_buffer", "trace_launch", "describe_config", "describe_plan", "select_config", "workspace_bytes", "num_sms", "LIBRARY_PATH",
 ]

@@ -270,6 +270,70 @@ int gemm_sm100_set_trace_buffer(void* device_buffer, size_t bytes);
  * GPU.) */
 int gemm_sm100_selftest_wait_timeout(void* cuda_stream, int* cuda_error_out);
 
+/* ------------------------------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one shared projection.  Row m of the batch uses adapter
+ * g = id(m), or none; with s_g = scale * scales[g]
+ *     low[m] = s_g * A[m] * down_g^T                      (R values, rounded once to the 16-bit type)
+ *     C[m]   = A[m] * B^T + low[m] * up_g^T               (one fp32 accumulator, rounded once)
+ * and for training, with the shared weight B frozen,
+ *     d_low[m] = s_g * dC[m] * up_g                       (R values, rounded once to the 16-bit type)
+ *     dA[m]    = dC[m] * B + d_low[m] * down_g
+ *     d_down_g = sum over the rows m of adapter g of d_low[m]^T * A[m]
+ *     d_up_g   = sum over the rows m of adapter g of dC[m]^T * low[m]
+ * No reference counterpart (the reference has one plain product).
+ *
+ * A row only ever meets its own adapter: infinities or NaN in one adapter, or in the rows that use
+ * it, do not reach another adapter's rows or gradients.  Results do not depend on timing: nothing is
+ * summed by atomics.  Adapters without rows get gradients of zero. */
+
+/* Largest rank R; ranks are multiples of 8.  (Adapters of a lower rank: pad with zeros.) */
+#define GEMM_SM100_LORA_MAX_RANK 128
+/* Largest number of adapters of one call. */
+#define GEMM_SM100_LORA_MAX_ADAPTERS 4096
+
+/* Bytes of device memory that gemm_sm100_lora_plan fills for M rows (0 for bad arguments). */
+size_t gemm_sm100_lora_plan_bytes(int M, int adapters);
+
+/* Prepares on `cuda_stream` which adapter each of the M rows uses, once for all projections of a batch.
+ * `ids`: M 32-bit (ids_are_64 = 0) or 64-bit integers on the device; a value outside [0, adapters)
+ * means "no adapter".  `plan`: gemm_sm100_lora_plan_bytes(M, adapters) bytes, 256-byte aligned,
+ * read by the calls below with the same M and adapters; it may be refilled in stream order. */
+int gemm_sm100_lora_plan(const void* ids, int ids_are_64, int M, int adapters, void* plan, size_t plan_bytes,
+                         void* cuda_stream, int* cuda_error_out);
+
+/* What the forward and the backward pass share.  Everything 16-bit is of type `dtype`, its base
+ * pointers are 16-byte aligned and its pitches (in elements) multiples of 8, with unit stride along the
+ * last dimension.  K > 0 and K % 8 == 0, N > 0, R a multiple of 8 up to GEMM_SM100_LORA_MAX_RANK. */
+typedef struct gemm_sm100_lora_args {
+  int M, N, K, R, adapters, dtype;
+  const void* A;             /* [M, K], pitch lda */
+  const void* B;             /* [N, K], pitch ldb */
+  const void* down;          /* [adapters, R, K]: row pitch ld_down, adapter pitch stride_down */
+  const void* up;            /* [adapters, N, R]: row pitch ld_up, adapter pitch stride_up */
+  long lda, ldb, ld_down, stride_down, ld_up, stride_up;
+  const float* scales;       /* [adapters] on the device, or NULL for 1 */
+  float scale;
+  const void* plan;          /* filled by gemm_sm100_lora_plan with the same M and adapters */
+} gemm_sm100_lora_args;
+
+/* low[M, R] (pitch ld_low) from A and down: the low-rank rows alone; rows without an adapter get zeros.
+ * B and up are not read and may be NULL. */
+int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low, void* cuda_stream,
+                        int* cuda_error_out);
+
+/* C[M, N] (pitch ldc); `low` [M, R] (pitch ld_low) is written on the way and stays valid for the
+ * backward pass.  M == 0 is a no-op.  C and low must not overlap the inputs. */
+int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* low, long ld_low, void* cuda_stream,
+                    int* cuda_error_out);
+
+/* Gradients from dC [M, N] (pitch ld_dc); N % 8 == 0.  dA [M, K] (pitch ld_da), d_down [adapters, R, K] and
+ * d_up [adapters, N, R] (both contiguous) may each be NULL: it is then not computed.  `low` is what the
+ * forward pass (or gemm_sm100_lora_low) wrote, needed for d_up only; `d_low` [M, R] (pitch ld_d_low)
+ * is scratch, needed for dA and d_down.  With M == 0 the adapters' gradients are filled with zeros. */
+int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, const void* low, long ld_low,
+                             void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up, void* cuda_stream,
+                             int* cuda_error_out);
+
 /* Static, human-readable name of a return code. */
 const char* gemm_sm100_error_string(int code);
 
