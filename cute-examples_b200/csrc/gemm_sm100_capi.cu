@@ -21,12 +21,12 @@
 #include <vector>
 #include <cstdint>
 
-#include "../../include/gemm_sm100.h"
-#include "gemm_tn_sm100.cuh"
+#include "gemm_host_sm100.cuh"
 
 namespace {
 
 using namespace gemm_sm100;
+using namespace gemm_sm100::host;
 
 // One status word per device (a __device__ variable exists once per device).
 __device__ unsigned int g_status_word;
@@ -36,85 +36,6 @@ __device__ unsigned int g_status_word;
 constexpr size_t kStaticFlagBytes = 1024;
 constexpr size_t kStaticScratchBytes = kStaticFlagBytes + 5u * 1024u * 1024u;
 static __device__ __align__(256) unsigned char g_static_scratch[kStaticScratchBytes];
-
-constexpr int kMaxDevices = 64;
-constexpr int kNumConfigs = 16;
-
-struct ConfigInfo {
-  int cta_group, mma_n, halves, stages, epi_warps;
-  int a_rows = 128;    // rows of A loaded per stage: the configuration only takes problems of at most that many rows
-  int epi_bufs = 0;    // staging buffers per epilogue warp (0: 8 / epi_warps)
-  int k_sub = 1;       // 64-element K blocks per stage (2: one 3-D TMA box per operand tile and stage)
-};
-constexpr ConfigInfo kConfigs[kNumConfigs] = {
-    {2, 256, 1, 6, 4},   // 256 x 256 pair tile, alternating accumulator slots
-    {2, 256, 2, 4, 8},   // 256 x 512 pair tile, both slots, 8 epilogue warps
-    {1, 256, 1, 4, 4},   // 128 x 256 single-CTA tile
-    {1, 128, 1, 4, 4},   // 128 x 128 single-CTA tile
-    {2, 256, 2, 4, 4},
-    {2, 256, 1, 6, 8},
-    {1, 256, 1, 4, 8},
-    // 256 x 128 pair tile: fewest operand bytes per SM among the small tiles.  Five stages: with
-    // operand boxes this small the ring delivers FEWER bytes per clock the more loads it keeps in
-    // flight (trace counters with the MMAs switched off, 8192 x 4096 x 4096: 0.48 of the MMA rate
-    // with 4 stages, 0.47 with 5, 0.44 with 6, 0.35 with 8), and few-tile problems ran 13-20 % faster
-    // with 5 stages than with 8.
-    {2, 128, 1, 5, 4},
-    {2, 192, 1, 6, 4},   // 256 x 192 pair tile: for tile counts that quantise badly with 256 columns
-    // 128 x 256 tiles for problems of at most 16 / 64 rows: only those rows of A are loaded, and the
-    // shared memory saved holds more stages (6 / 5 x 32 KiB of B in flight per SM instead of 4)
-    {1, 256, 1, 6, 4, 16, 1},
-    {1, 256, 1, 5, 4, 64, 1},
-    // 256 x 128 pair tile with two K blocks per stage (K % 64 == 0 only): half as many, twice as
-    // large TMA boxes as configuration 7
-    {2, 128, 1, 4, 4, 128, 0, 2},
-    // 128 x 128 single-CTA tile with two K blocks per stage, for problems of at most 128 rows whose
-    // columns give too few 256-wide tiles: twice the tiles of configuration 2, half-size partial tiles
-    {1, 128, 1, 3, 4, 128, 0, 2},
-    // 128 x 64 tiles for problems of at most 16 / 64 rows and several thousand columns: four K blocks
-    // (512 bytes of every row) per TMA box, short A
-    {1, 64, 1, 5, 4, 16, 1, 4},
-    {1, 64, 1, 3, 4, 64, 1, 4},
-    // configuration 9 with two K blocks per box (K % 64 == 0): 16 x 28672 x 8192 74.5 against 75.6 us
-    {1, 256, 1, 3, 4, 16, 1, 2},
-};
-
-template <int kIndex, bool kIsBf16>
-using ConfigOf = GemmConfig<kConfigs[kIndex].cta_group, kConfigs[kIndex].mma_n, kConfigs[kIndex].halves,
-                            kConfigs[kIndex].stages, kConfigs[kIndex].epi_warps, kIsBf16, kConfigs[kIndex].a_rows,
-                            kConfigs[kIndex].epi_bufs, kConfigs[kIndex].k_sub>;
-
-struct DeviceState {
-  bool ready = false;
-  int device = 0;
-  int sm_count = 0;
-  int cc_major = 0;
-  unsigned int* status_ptr = nullptr;
-  void* static_scratch = nullptr;      // device address of g_static_scratch on this device
-  int max_ctas[kNumConfigs][2] = {};   // persistent grid limit per config and dtype
-  bool attr_set[kNumConfigs][2] = {};
-};
-
-std::mutex g_mutex;
-DeviceState g_dev[kMaxDevices];
-// Process-wide knobs.  Written by gemm_sm100_set_option / gemm_sm100_set_trace_buffer, read by
-// launches on any thread: atomics, so a concurrent change is seen whole or not at all.
-std::atomic<long> g_opt_tile_config{-1};
-std::atomic<long> g_opt_timeout_ms{2000};
-std::atomic<long> g_opt_max_ctas{0};
-std::atomic<long> g_opt_debug_flags{0};
-std::atomic<long> g_opt_group_m{0};
-std::atomic<long> g_opt_k_rotate{-1};   // 0 never, 1 always, -1 (default) when there is a single tile row: 3 % on the few-row shapes, 2 = serpentine
-std::atomic<long> g_opt_sk_cluster{-1};  // cluster K-split (partial sums through distributed shared memory): -1 planner, 0 never, 1 always where an even split of 2 or 4 is made
-std::atomic<long> g_opt_pdl{1};        // 1: launch with programmatic stream serialization (overlap with the previous kernel's tail)
-std::atomic<long> g_opt_early_prefetch{1};   // with pdl: L2 prefetch of the first stages before waiting for the previous kernel
-std::atomic<long> g_opt_tiles_n{0};    // > 0: force this many tiles per tile row (tests), when the configuration allows the widths
-std::atomic<long> g_opt_balance{1};    // 1: the planner may choose a balanced column tiling; 0: uniform tiles only
-std::atomic<long> g_opt_split_k{-1};   // -1 automatic, 0 never, 1 whenever the configuration allows it
-// Clusters of 2, 4 and 8 CTAs (one CTA per SM) the device holds at once, from the occupancy query.
-std::atomic<int> g_held_clusters[3] = {};
-// Bumped by every gemm_sm100_set_option: cached plans of an older generation are stale.
-std::atomic<unsigned> g_opt_generation{1};
 
 // Workspaces registered with gemm_sm100_workspace_register: the library zero-fills the start once
 // and from then on knows how long a prefix the launches queued so far leave zeroed.
@@ -184,56 +105,6 @@ struct EnvOverrides {
 };
 const EnvOverrides g_env_overrides;
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn g_encode = nullptr;
-
-int set_cuda_error(int* out, cudaError_t e) {
-  if (out) *out = static_cast<int>(e);
-  return GEMM_SM100_ERR_CUDA;
-}
-
-// Looks the driver's tensor-map encoder up once (no link-time dependency on libcuda).
-int get_encoder(int* cuda_error_out) {
-  if (g_encode) return GEMM_SM100_OK;
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult qres;
-  cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
-  if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
-  if (qres != cudaDriverEntryPointSuccess || fn == nullptr)
-    return set_cuda_error(cuda_error_out, cudaErrorSymbolNotFound);
-  g_encode = reinterpret_cast<EncodeTiledFn>(fn);
-  return GEMM_SM100_OK;
-}
-
-// Columns of C the TMA stores cover: whole 16-byte pieces only (the kernel writes the last N % 8
-// columns with plain stores); never 0, which is not a valid extent (the map is unused then).
-inline long tma_store_cols(long n) { return n >= 8 ? (n & ~7L) : 8; }
-
-// Tensor map of a row-major 2-D array of 16-bit elements: `rows` x `cols`, pitch `ld`
-// elements, box `box_rows` x 64 columns, 128-byte swizzle (64 x 2 B = one swizzle row).
-// With k_sub > 1 (cols a multiple of 64) the same array is described as 3-D: 64 elements x rows x
-// 64-element K blocks (128 bytes apart), box 64 x box_rows x k_sub, so that one copy brings k_sub K
-// blocks of the rows, each as its own K-major tile.
-int encode_2d(CUtensorMap* map, const void* base, int dtype, long rows, long cols, long ld,
-              int box_rows, int* cuda_error_out, int k_sub = 1) {
-  const bool blocks = k_sub > 1;
-  const cuuint64_t dims[3] = {blocks ? 64u : static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
-                              static_cast<cuuint64_t>(cols / 64)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2u, 128u};
-  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(k_sub)};
-  const cuuint32_t elem_strides[3] = {1u, 1u, 1u};
-  const CUtensorMapDataType dt =
-      dtype == GEMM_SM100_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = g_encode(map, dt, blocks ? 3 : 2, const_cast<void*>(base), dims, strides, box, elem_strides,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_cuda_error(cuda_error_out, cudaErrorInvalidValue);
-  return GEMM_SM100_OK;
-}
-
 // Per-thread cache of encoded tensor maps.  The encoding depends only on the arguments below, so
 // a caller that multiplies the same buffers again (a layer of a model, a benchmark loop) skips the
 // driver's encoder: three calls of roughly a microsecond each per launch, which is most of the host
@@ -273,6 +144,11 @@ int encode_2d_cached(CUtensorMap* map, const void* base, int dtype, long rows, l
   c.used[slot] = true;
   return GEMM_SM100_OK;
 }
+
+}  // namespace
+
+namespace gemm_sm100 {
+namespace host {
 
 int device_state(DeviceState** out, int* cuda_error_out) {
   int dev = 0;
@@ -326,18 +202,10 @@ int device_state(DeviceState** out, int* cuda_error_out) {
   return GEMM_SM100_OK;
 }
 
-struct Problem {
-  const void* A;
-  const void* B;
-  void* C;
-  int M, N, K;
-  long lda, ldb, ldc;
-  int dtype;
-  bool b_is_kn = false;   // B given as [K, N] (pitch ldb >= N) instead of [N, K]
-  bool a_is_km = false;   // A given as [K, M] (pitch lda >= M) instead of [M, K]
-  float alpha = 1.0f;     // C = alpha * op(A) op(B) + beta * C (only the layout kernels apply them)
-  float beta = 0.0f;
-};
+}  // namespace host
+}  // namespace gemm_sm100
+
+namespace {
 
 int validate(const Problem& p) {
   if (p.M < 0 || p.N < 0 || p.K < 0) return GEMM_SM100_ERR_BAD_SHAPE;
@@ -353,8 +221,6 @@ int validate(const Problem& p) {
     return GEMM_SM100_ERR_BAD_ALIGNMENT;
   return GEMM_SM100_OK;
 }
-
-inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 // Cost model used to choose a tile configuration: time ~ longest chain of tiles on one CTA (pair) x
 // (K blocks of a tile + what a tile boundary costs) / (relative rate of the configuration).
@@ -422,26 +288,6 @@ inline long resident_clusters(int sm_count, int cluster_ctas) {
   return n > 0 ? n : 1;
 }
 
-struct Plan {
-  int config = 0;
-  // Column tiling (TileParams::bal_q / bal_rem): tiles_n tiles per tile row; 0 = uniform tiles.
-  int tiles_n = 0, bal_q = 0, bal_rem = 0, bal_start = 0;
-  bool split_k = false;
-  int ctas = 0;              // grid size
-  size_t flag_bytes = 0;     // K-split: arrival counters (one per CTA), padded to 256 bytes
-  size_t partial_bytes = 0;  // K-split: one fp32 partial tile per CTA
-  int partial_rows = 128;    // K-split: rows kept per partial tile
-  int split_factor = 0;      // K-split: > 1 = every tile cut into this many equal K ranges
-  bool cluster = false;      // even split whose contributors form a cluster and exchange partial sums in shared memory
-};
-
-inline int grid_cap(const ConfigInfo& c, int sm_count) {
-  long cap = sm_count - sm_count % c.cta_group;
-  if (g_opt_max_ctas > 0 && g_opt_max_ctas < cap) cap = g_opt_max_ctas - g_opt_max_ctas % c.cta_group;
-  if (cap < c.cta_group) cap = c.cta_group;
-  return static_cast<int>(cap);
-}
-
 // Host mirror of the kernel's tile_coords(): column-tile index of tile `t`.
 inline int n_tile_of(long t, int m_tiles, int n_tiles, int group_m) {
   const long per_group = static_cast<long>(group_m) * n_tiles;
@@ -450,10 +296,6 @@ inline int n_tile_of(long t, int m_tiles, int n_tiles, int group_m) {
   const long first_m = group * group_m;
   const long rows = (m_tiles - first_m) < group_m ? (m_tiles - first_m) : group_m;
   return static_cast<int>(in_group / rows);
-}
-
-inline int default_group_m(int m_tiles) {
-  return g_opt_group_m.load() > 0 ? static_cast<int>(g_opt_group_m.load()) : (m_tiles >= 16 ? 16 : 8);
 }
 
 // What one K block of a tile of `width` columns costs, in columns of a full-rate tile: the MMAs
@@ -494,20 +336,21 @@ double schedule_cost(const ConfigInfo& c, int m_tiles, int tiles_n, int q, int r
 
 // The K-split schedule gives every CTA the same number of K blocks; it pays when whole tiles
 // quantise badly over the SMs (few tiles, as in the memory-bound small-M shapes) and K is long.
-Plan make_plan(int M, int N, int K, int sm_count, bool allow_split = true, int config_limit = kNumConfigs,
-               bool allow_balance = true) {
+Plan make_plan(int M, int N, int K, int sm_count, bool allow_split, unsigned config_mask, bool allow_balance,
+               bool allow_workspace) {
   Plan best;
   double best_cost = 1e300;
   const long k_blocks = ceil_div(K, 64);
   // A forced configuration that cannot take this problem (more rows than its A tile holds) is
   // ignored: the automatic choice runs instead.
   const long forced_index = g_opt_tile_config.load();
-  const bool forced_config = forced_index >= 0 && forced_index < kNumConfigs && forced_index < config_limit &&
+  const bool forced_config = forced_index >= 0 && forced_index < kNumConfigs && ((config_mask >> forced_index) & 1u) != 0 &&
                              (kConfigs[forced_index].a_rows >= 128 || M <= kConfigs[forced_index].a_rows) &&
                              (kConfigs[forced_index].k_sub == 1 || K % 64 == 0);
   const int first = forced_config ? static_cast<int>(forced_index) : 0;
-  const int last = forced_config ? first + 1 : config_limit;   // config_limit: callers whose kernels exist for the first few configurations only
+  const int last = forced_config ? first + 1 : kNumConfigs;
   for (int i = first; i < last; ++i) {
+    if (((config_mask >> i) & 1u) == 0) continue;
     const ConfigInfo& c = kConfigs[i];
     if (c.a_rows < 128 && M > c.a_rows) continue;        // few-row configurations: only what their A tile holds
     if (c.k_sub > 1 && K % 64 != 0) continue;           // whole 64-element K blocks only (nothing bounds K inside a block)
@@ -623,7 +466,7 @@ Plan make_plan(int M, int N, int K, int sm_count, bool allow_split = true, int c
         split_cost *= 1.15;                                  // the fit is good to about 10 %: ties go to whole tiles
       }
     }
-    const bool can_split = allow_split && has_split_k(i) && units >= 2 && c.k_sub == 1;   // contiguous ranges: 64-element K blocks only
+    const bool can_split = allow_split && allow_workspace && has_split_k(i) && units >= 2 && c.k_sub == 1;   // contiguous ranges: 64-element K blocks only
     // Even split: every tile cut into s equal K ranges, the reduction spread over the contributors.
     // Forced with split_k = s (2..16); automatic when it beats whole tiles and the contiguous ranges.
     int even_s = 0;
@@ -649,7 +492,7 @@ Plan make_plan(int M, int N, int K, int sm_count, bool allow_split = true, int c
         // chunks) of one chunk of one half of the rows
         const int chunks = c.mma_n / 64;
         const bool cluster_ok = (f == 2 || f == 4) && (chunks % f == 0 || f == 2 * chunks);
-        if (sk_cluster != 1 || !cluster_ok)
+        if (allow_workspace && (sk_cluster != 1 || !cluster_ok))
           consider(f, false, ceil_div(tiles * f, slots), kEvenSplitFixedKBlocks[i] + kEvenSplitPerRangeKBlocks[i] / f);
         // 2 or 4 contributors per tile: clusters of up to 8 CTAs, and every chunk that leaves a CTA has
         // a staging slot of its own in shared memory; one unit per CTA (pair), as many waves of
@@ -695,13 +538,19 @@ Plan make_plan(int M, int N, int K, int sm_count, bool allow_split = true, int c
   return best;
 }
 
+}  // namespace
+
+namespace gemm_sm100 {
+namespace host {
+
 // Per-thread cache of plans: the binding asks for the workspace size and then launches, and callers
 // repeat shapes, so the cost model runs once per (shape, option state).
-Plan plan_for(int M, int N, int K, int sm_count, bool allow_split = true, int config_limit = kNumConfigs,
-              bool allow_balance = true) {
+Plan plan_for(int M, int N, int K, int sm_count, bool allow_split, unsigned config_mask, bool allow_balance,
+              bool allow_workspace) {
   struct Entry {
-    int M = -1, N = 0, K = 0, sm = 0, limit = 0;
-    bool allow = false, balance = false;
+    int M = -1, N = 0, K = 0, sm = 0;
+    unsigned mask = 0;
+    bool allow = false, balance = false, workspace = false;
     unsigned generation = 0;
     Plan plan;
   };
@@ -711,94 +560,22 @@ Plan plan_for(int M, int N, int K, int sm_count, bool allow_split = true, int co
   const unsigned generation = g_opt_generation.load(std::memory_order_acquire);
   for (int i = 0; i < kEntries; ++i) {
     const Entry& e = cache[i];
-    if (e.M == M && e.N == N && e.K == K && e.sm == sm_count && e.limit == config_limit && e.allow == allow_split &&
-        e.balance == allow_balance && e.generation == generation)
+    if (e.M == M && e.N == N && e.K == K && e.sm == sm_count && e.mask == config_mask && e.allow == allow_split &&
+        e.balance == allow_balance && e.workspace == allow_workspace && e.generation == generation)
       return e.plan;
   }
   Entry& e = cache[next++ % kEntries];
-  e.M = M, e.N = N, e.K = K, e.sm = sm_count, e.limit = config_limit, e.allow = allow_split;
-  e.balance = allow_balance;
+  e.M = M, e.N = N, e.K = K, e.sm = sm_count, e.mask = config_mask, e.allow = allow_split;
+  e.balance = allow_balance, e.workspace = allow_workspace;
   e.generation = generation;
-  e.plan = make_plan(M, N, K, sm_count, allow_split, config_limit, allow_balance);
+  e.plan = make_plan(M, N, K, sm_count, allow_split, config_mask, allow_balance, allow_workspace);
   return e.plan;
 }
 
-// Tile counts, rasterisation and wait limit of one launch (everything that does not depend on
-// the schedule variant).
-template <class Cfg>
-TileParams base_tile_params(const Problem& p, const DeviceState& st) {
-  TileParams tp;
-  tp.M = p.M;
-  tp.N = p.N;
-  tp.K = p.K;
-  tp.m_tiles = static_cast<int>(ceil_div(p.M, 128L * Cfg::kCtaGroup));
-  tp.n_tiles = static_cast<int>(ceil_div(p.N, Cfg::kBlockN));
-  tp.k_blocks = static_cast<int>(ceil_div(p.K, Cfg::kBlockK));
-  // Rasterisation group: 16 tile rows when the problem has that many (measured best from 8192
-  // to 32768 rows: the A panel of a group is reused by more B tiles), else 8.
-  tp.group_m = default_group_m(tp.m_tiles);
-  tp.bal_q = Cfg::kBlockN / 64;
-  tp.bal_rem = 0;
-  tp.bal_start = 0;
-  tp.b_box_rows = Cfg::kBRows;
-  tp.early_prefetch = (g_opt_pdl.load() != 0 && g_opt_early_prefetch.load() != 0) ? 1 : 0;
-  tp.status = st.status_ptr;
-  tp.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
-  tp.trace = nullptr;
-  tp.debug_flags = 0;
-  tp.sk_flags = nullptr;
-  tp.sk_partials = nullptr;
-  tp.sk_rows = 128;
-  tp.sk_factor = 0;
-  tp.sk_cluster = 0;
-  tp.k_rotate = 0;
-  tp.alpha = p.alpha;
-  tp.beta = p.beta;
-  tp.c_ptr = p.C;
-  tp.ldc = p.ldc;
-  return tp;
-}
+}  // namespace host
+}  // namespace gemm_sm100
 
-// Order of a tile's K blocks (TileParams::k_rotate) for this problem under the "k_rotate" option.
-// Automatic (-1): rotation only in the memory-bound few-row regime (at most 128 rows, thousands of
-// columns).  Other problems keep K ascending, so that the same rows give the same bits whether
-// they are computed in one call or in row panels, and in every operand layout.
-int k_order_for(const Problem& p, bool split_k) {
-  const long k_order = g_opt_k_rotate.load();
-  const bool few_rows = p.M <= 128 && p.N >= 2048 && !split_k;
-  return k_order == 2 ? 2 : ((k_order == 1 || (k_order < 0 && few_rows)) ? 1 : 0);
-}
-
-// Cluster launch of `kernel` on `ctas` CTAs of Cfg::kThreads threads.
-template <class Cfg, class Kernel, class... Args>
-cudaError_t launch_kernel(Kernel kernel, long ctas, int cluster_ctas, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(Cfg::kThreads);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attrs[2];
-  unsigned n = 0;
-  if (cluster_ctas > 1) {                              // single-CTA tiles are launched without a cluster
-    attrs[n].id = cudaLaunchAttributeClusterDimension;
-    attrs[n].val.clusterDim.x = static_cast<unsigned>(cluster_ctas);
-    attrs[n].val.clusterDim.y = 1;
-    attrs[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (g_opt_pdl.load() != 0) {
-    // Programmatic dependent launch: this kernel's CTAs may be scheduled while the previous kernel
-    // of the stream drains (if that kernel allows it, as these kernels do at their start); they
-    // set up barriers and tensor memory and then wait for it to complete before touching global
-    // memory.  Back-to-back GEMMs lose a few microseconds less between launches.
-    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attrs;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
+namespace {
 
 // One-time set-up of a tile configuration on a device: the dynamic shared-memory limit of every
 // instantiation that can be launched for it, and how many CTAs of it are co-resident.
@@ -1224,7 +1001,7 @@ int gemm_sm100_gemm_scaled(const void* A, const void* B, void* C, int M, int N, 
     rc = get_encoder(cuda_error_out);
     if (rc != GEMM_SM100_OK) return rc;
   }
-  Plan plan = plan_for(M, N, K, st->sm_count, /*allow_split=*/false, /*config_limit=*/4, /*allow_balance=*/false);
+  Plan plan = plan_for(M, N, K, st->sm_count, /*allow_split=*/false, /*config_mask=*/0xfu, /*allow_balance=*/false);
   if (plan.config > 3) plan = Plan{};       // (a forced configuration without such a variant)
   if (plan.ctas == 0) {
     const long tiles = ceil_div(M, 256L) * ceil_div(N, 256L);

@@ -108,6 +108,24 @@ struct TileParams {
   long long ldc;                   // plain stores in its last N % 8 columns; row pitch in elements
 };
 
+// Low-rank adapters of the rows, appended to the K loop (kernels instantiated with kLora):
+//   C[m] += low[m] W_g^T   for the adapter g of row m, into the accumulator the K loop has filled.
+// A tile's rows use a list of distinct adapters ("slots").  Each slot is one more product of all rows of
+// the tile with that adapter's weights, issued with the tensor core's row mask so that only the
+// slot's rows take the result: no zeros are multiplied in (0 x Inf from a broken adapter would poison
+// other rows), C is neither written twice nor rounded twice, and what the adapters add to the main loop is
+// their share of the operand bytes: R of K + R columns per slot.
+// An "item" is one slot x one chunk of its ranks; a ring stage holds as many items as fit.
+struct LoraParams {
+  CUtensorMap tmap_low;           // low [M, R]: boxes of `chunk` ranks x the A tile's rows
+  CUtensorMap tmap_w;             // W [adapters, N, R]: boxes of chunk ranks x B rows; with kBIsKN
+                                  // W [adapters, R, N]: boxes of 64 columns x chunk ranks
+  const int* slot_count;          // per tile of 256 rows
+  const int* slot_adapter;        // [tiles][256]
+  const unsigned int* slot_mask;  // [tiles][256][8]
+  int chunk, chunks;              // ranks per item (16, 32 or 64: one swizzle row) and items per slot
+};
+
 // Experiment switches (results are garbage with any of them set).
 enum : unsigned int {
   kDebugSkipLoads = 1u,   // no TMA loads, MMA does not wait for operands: pure MMA issue/execute rate
@@ -279,7 +297,7 @@ struct WaitCtx {
 //
 // Cold path of a bounded mbarrier wait: polls until the phase completes, the CTA is flagged,
 // or the time limit passes (then flags this CTA and its pair peer and records `code`).
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, const WaitCtx& ctx, uint32_t code) {
+static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, const WaitCtx& ctx, uint32_t code) {
   bool done = false;
   // try_wait suspends the thread for a hardware-defined while; normal waits end inside this
   // first batch, without a read of the (slow) global timer.
@@ -312,7 +330,7 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, cons
 // Bounded wait (whole warp) until a global arrival counter reaches `want`.  Arrivals are counted in
 // the low 16 bits; the high bits count the warps that are done with the partial tiles (see the even
 // K-split below).
-__device__ __noinline__ bool wait_counter(const unsigned int* counter, unsigned int want, const WaitCtx& ctx,
+static __device__ __noinline__ bool wait_counter(const unsigned int* counter, unsigned int want, const WaitCtx& ctx,
                                           uint32_t code) {
   const volatile unsigned int* c = counter;
   uint64_t t0 = 0;
@@ -369,6 +387,27 @@ __device__ __forceinline__ TileCols tile_columns(int n_tile, const TileParams& p
   return t;
 }
 
+// The adapter stages of one segment: items [item0, item1) in groups of what a ring stage holds.  A tile
+// that is cut along K deals its stages to the contributors like its K blocks.
+struct LoraWork {
+  int item0, item1, per_stage, stages;
+};
+template <class Cfg>
+__device__ __forceinline__ LoraWork lora_work(const LoraParams& lora, int m_tile, int part, int factor) {
+  const int slots = lora.slot_count[Cfg::kCtaGroup == 2 ? m_tile : m_tile >> 1];
+  LoraWork w;
+  w.per_stage = Cfg::kBlockK / lora.chunk;
+  const int items = slots * lora.chunks;
+  const int all = (items + w.per_stage - 1) / w.per_stage;
+  const int first = factor > 1 ? (int)((long long)part * all / factor) : 0;
+  const int last = factor > 1 ? (int)((long long)(part + 1) * all / factor) : all;
+  // (a loaded value: handed back as warp-uniform for the issue loops)
+  w.stages = __reduce_max_sync(0xffffffffu, last - first);
+  w.item0 = __reduce_max_sync(0xffffffffu, first * w.per_stage);
+  w.item1 = __reduce_max_sync(0xffffffffu, items < last * w.per_stage ? items : last * w.per_stage);
+  return w;
+}
+
 template <bool kIsBf16>
 __device__ __forceinline__ uint32_t pack2(uint32_t lo_bits, uint32_t hi_bits) {
   const float lo = __uint_as_float(lo_bits), hi = __uint_as_float(hi_bits);
@@ -395,9 +434,12 @@ __device__ __forceinline__ uint32_t pack2(uint32_t lo_bits, uint32_t hi_bits) {
 // kAIsKM: likewise A given as [K, M] (M contiguous), i.e. the product A^T * B.
 // kScaled: the epilogue applies alpha and beta (the reference has neither: gemm.cuh:368-377 only
 // converts the accumulator).
-template <class Cfg, bool kDebug, bool kSplitK, bool kBIsKN = false, bool kAIsKM = false, bool kScaled = false>
+// kLora: the rows' low-rank adapters are appended to the K loop (LoraParams).
+template <class Cfg, bool kDebug, bool kSplitK, bool kBIsKN = false, bool kAIsKM = false, bool kScaled = false,
+          bool kLora = false>
 __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CUtensorMap& tmap_b,
-                                             const CUtensorMap* tmap_c, const int num_c, const TileParams& p) {
+                                             const CUtensorMap* tmap_c, const int num_c, const TileParams& p,
+                                             const LoraParams* lora = nullptr) {
   constexpr int G = Cfg::kCtaGroup;
   constexpr int kStages = Cfg::kStages;
   static_assert(!kBIsKN || Cfg::kBRows % 64 == 0, "B[K,N] tiles are loaded in blocks of 64 columns");
@@ -457,6 +499,10 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       *abort_flag = 0;
       prefetch_tensormap(&tmap_a);
       prefetch_tensormap(&tmap_b);
+      if constexpr (kLora) {
+        prefetch_tensormap(&lora->tmap_low);
+        prefetch_tensormap(&lora->tmap_w);
+      }
       for (int d = 0; d < num_c; ++d) prefetch_tensormap(tmap_c + d);
       if constexpr (kSplitK) {
         // every epilogue warp of every contributor to this CTA's rows arrives once on each
@@ -582,6 +628,9 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       const int b_box = p.b_box_rows;
       bool seg_start = true, backwards = false;
       bool ok = true;
+      [[maybe_unused]] LoraWork lw = {0, 0, 1, 0};
+      [[maybe_unused]] int slot_base = 0;
+      int seg_end = seg.kb1;                              // the segment's K blocks, then its adapter stages
       long long stall = 0;
       while (have && ok) {
 #pragma unroll
@@ -601,6 +650,20 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             backwards = !kSplitK && p.k_rotate == 2 && (tiles_done & 1);
             ++tiles_done;
             seg_start = false;
+            seg_end = seg.kb1;
+            if constexpr (kLora) {
+              lw = lora_work<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 0);
+              slot_base = (G == 2 ? m_tile : m_tile >> 1) * 256;
+              seg_end += lw.stages;
+            }
+          }
+          [[maybe_unused]] int item = 0, items = 0, item_adapter = 0;
+          if constexpr (kLora) {
+            if (kb >= seg.kb1) {                          // an adapter stage: lane i fetches the adapter of item i
+              item = lw.item0 + (kb - seg.kb1) * lw.per_stage;
+              items = min(lw.per_stage, lw.item1 - item);
+              if ((int)lane < items) item_adapter = lora->slot_adapter[slot_base + (item + (int)lane) / lora->chunks];
+            }
           }
           long long t0 = 0;
           if constexpr (kDebug) t0 = trace ? clock64() : 0;
@@ -610,6 +673,46 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
           }
           if constexpr (kDebug)
             if (trace) stall += clock64() - t0;
+          if constexpr (kLora) {
+            if (kb >= seg.kb1) {
+              const int chunk = lora->chunk, chunks = lora->chunks;
+              const uint32_t low_bytes = (uint32_t)(Cfg::kARows * chunk * 2);
+              const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);     // one item's tile of W per half
+              if (issuer && is_leader)
+                mbar_arrive_expect_tx(bar_base + kFullOff + 8u * s,
+                                      G * ((chunks == 1 ? 1 : items) * low_bytes +
+                                           (uint32_t)(items * (rows_b[0] + rows_b[1]) * chunk * 2)));
+              const uint32_t full = full_leader + 8u * s;
+              for (int i = 0; i < items; ++i) {
+                const int g = __shfl_sync(0xffffffffu, item_adapter, i);
+                const int r = (chunks == 1 ? 0 : (item + i) % chunks) * chunk;
+                if (issuer) {
+                  // slots of one chunk share the tile of low rows
+                  if (i == 0 || chunks > 1)
+                    tma_load_2d<G>(smem_a + s * Cfg::kABytes + (uint32_t)i * low_bytes, &lora->tmap_low, full, r, row_a, pol);
+#pragma unroll
+                  for (int h = 0; h < Cfg::kHalves; ++h) {
+                    const uint32_t dst = smem_b + s * Cfg::kBBytes + h * Cfg::kBHalfBytes + (uint32_t)i * w_bytes;
+                    if constexpr (!kBIsKN) {
+#pragma unroll 1
+                      for (int j = 0; j < rows_b[h]; j += b_box)
+                        tma_load_3d<G>(dst + (uint32_t)(j * chunk * 2), &lora->tmap_w, full, r, row_b[h] + j, g, pol);
+                    } else {
+#pragma unroll
+                      for (int j = 0; j < Cfg::kBRows / 64; ++j)
+                        tma_load_3d<G>(dst + (uint32_t)(j * chunk * 128), &lora->tmap_w, full, row_b[h] + j * 64, r, g, pol);
+                    }
+                  }
+                }
+              }
+              if (++kb == seg_end) {
+                have = work.next(seg);
+                kb = seg.kb0;
+                seg_start = true;
+              }
+              continue;
+            }
+          }
           int kb_phys = kb + rot;                  // which K block this step loads (order is free)
           if (kb_phys >= k_blocks) kb_phys -= k_blocks;
           if (backwards) kb_phys = k_blocks - 1 - kb;
@@ -649,7 +752,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               }
             }
           }
-          if (++kb == seg.kb1) {
+          if (++kb == seg_end) {
             have = work.next(seg);
             kb = seg.kb0;
             seg_start = true;
@@ -690,12 +793,49 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       bool have = work.next(seg);
       int kb = seg.kb0, iter = 0;          // iter counts segments: it selects the accumulator slot
       bool ok = peer_ready;
+      [[maybe_unused]] LoraWork lw = {0, 0, 1, 0};
+      [[maybe_unused]] int slot_base = 0;
+      int seg_end = seg.kb1;
       long long stall_full = 0, stall_acc = 0;
       const bool skip_mma = kDebug && (dbg & kDebugSkipMma);
       while (have && ok) {
 #pragma unroll
         for (int s = 0; s < kStages; ++s) {
           if (!have) break;
+          const bool first_kb = kb == seg.kb0;
+          if (first_kb) {
+            int m_tile, n_tile;
+            tile_coords(seg.tile, p, m_tile, n_tile);
+            const TileCols tc = tile_columns<Cfg>(n_tile, p);
+            idesc_h[0] = idesc_base | ((uint32_t)(tc.w0 >> 3) << 17);
+            idesc_h[1] = idesc_base | ((uint32_t)(tc.w1 >> 3) << 17);
+            seg_end = seg.kb1;
+            if constexpr (kLora) {
+              lw = lora_work<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 0);
+              slot_base = (G == 2 ? m_tile : m_tile >> 1) * 256;
+              seg_end += lw.stages;
+              if constexpr (G == 1) slot_base = slot_base * 2 + (m_tile & 1);   // in half masks of 128 rows
+            }
+          }
+          [[maybe_unused]] int item = 0, items = 0;
+          [[maybe_unused]] uint4 item_rows[G];
+          if constexpr (kLora) {
+            if (kb >= seg.kb1) {
+              // adapter stage: lane i fetches the row mask of item i while the operands are on their way
+              item = lw.item0 + (kb - seg.kb1) * lw.per_stage;
+              items = min(lw.per_stage, lw.item1 - item);
+              if ((int)lane < items) {
+                const int slot = (item + (int)lane) / lora->chunks;
+                const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask);
+                if constexpr (G == 1) {
+                  item_rows[0] = masks[slot_base + 2 * slot];
+                } else {
+                  item_rows[0] = masks[2 * (slot_base + slot)];
+                  item_rows[1] = masks[2 * (slot_base + slot) + 1];
+                }
+              }
+            }
+          }
           long long tf = 0;
           if constexpr (kDebug) tf = trace ? clock64() : 0;
           if (!(kDebug && (dbg & kDebugSkipLoads)) &&
@@ -713,14 +853,57 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               }
             }
           tc_fence_after_sync();
-          const bool first_kb = kb == seg.kb0;
-          const bool last_kb = kb == seg.kb1 - 1;
-          if (first_kb) {
-            int m_tile, n_tile;
-            tile_coords(seg.tile, p, m_tile, n_tile);
-            const TileCols tc = tile_columns<Cfg>(n_tile, p);
-            idesc_h[0] = idesc_base | ((uint32_t)(tc.w0 >> 3) << 17);
-            idesc_h[1] = idesc_base | ((uint32_t)(tc.w1 >> 3) << 17);
+          const bool last_kb = kb == seg_end - 1;
+          if constexpr (kLora) {
+            if (kb >= seg.kb1) {
+              const int chunk = lora->chunk, chunks = lora->chunks;
+              const uint32_t low_bytes = (uint32_t)(Cfg::kARows * chunk * 2);
+              const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);
+              const uint64_t dl0 = make_smem_desc_rows(smem_a + s * Cfg::kABytes, (uint32_t)chunk * 2u);
+              const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(smem_b + s * Cfg::kBBytes, (uint32_t)chunk * 128u)
+                                          : make_smem_desc_rows(smem_b + s * Cfg::kBBytes, (uint32_t)chunk * 2u);
+              constexpr uint32_t kWStepK = kBIsKN ? 128u : 2u;
+#pragma unroll 1
+              for (int i = 0; i < items; ++i) {
+                uint32_t skip[4 * G];
+#pragma unroll
+                for (int v = 0; v < G; ++v) {
+                  skip[4 * v] = ~__shfl_sync(0xffffffffu, item_rows[v].x, i);
+                  skip[4 * v + 1] = ~__shfl_sync(0xffffffffu, item_rows[v].y, i);
+                  skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, item_rows[v].z, i);
+                  skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, item_rows[v].w, i);
+                }
+                const uint64_t dl = dl0 + (uint64_t)((chunks == 1 ? 0u : (uint32_t)i * low_bytes) >> 4);
+                const uint64_t dw = dw0 + (uint64_t)(((uint32_t)i * w_bytes) >> 4);
+                if (issuer) {
+#pragma unroll
+                  for (int h = 0; h < Cfg::kHalves; ++h) {
+                    const int slot = Cfg::kHalves == 1 ? (iter & 1) : h;
+                    for (int k = 0; k < chunk / Cfg::kUmmaK; ++k)
+                      umma_f16_rows<G>(tmem_base + slot * Cfg::kSlotCols, dl + 2u * k,
+                                       dw + (uint64_t)((h * Cfg::kBHalfBytes) >> 4) + kWStepK * k, idesc_h[h], skip);
+                  }
+                }
+              }
+              if (issuer) {
+                if (last_kb) {
+#pragma unroll
+                  for (int h = 0; h < Cfg::kHalves; ++h) {
+                    const int slot = Cfg::kHalves == 1 ? (iter & 1) : h;
+                    umma_commit<G>(bar_base + kTFullOff + 8u * slot);
+                    if constexpr (G == 2) umma_commit<G>(bar_peer + kTFullOff + 8u * slot);
+                  }
+                }
+                umma_commit<G>(bar_base + kEmptyOff + 8u * s);
+                if constexpr (G == 2) umma_commit<G>(bar_peer + kEmptyOff + 8u * s);
+              }
+              if (++kb == seg_end) {
+                have = work.next(seg);
+                kb = seg.kb0;
+                ++iter;
+              }
+              continue;
+            }
           }
 #pragma unroll
           for (int h = 0; h < Cfg::kHalves; ++h) {
@@ -778,7 +961,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               if constexpr (G == 2) umma_commit<G>(bar_peer + kEmptyOff + 8u * s);
             }
           }
-          if (++kb == seg.kb1) {
+          if (++kb == seg_end) {
             have = work.next(seg);
             kb = seg.kb0;
             ++iter;
@@ -1292,10 +1475,19 @@ gemm_layout_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   gemm_tn_body<Cfg, false, false, kBIsKN, kAIsKM, true>(tmap_a, tmap_b, &tmap_c, 1, p);
 }
 
+// The rows' low-rank adapters appended to the K loop; kBIsKN: B and the adapters' weights with the output
+// column contiguous (the gradient of the activations).
+template <class Cfg, bool kSplitK, bool kBIsKN>
+__global__ void __launch_bounds__(Cfg::kThreads, 1)
+gemm_lora_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_c, const TileParams p, const __grid_constant__ LoraParams lora) {
+  gemm_tn_body<Cfg, false, kSplitK, kBIsKN, false, false, true>(tmap_a, tmap_b, &tmap_c, 1, p, &lora);
+}
+
 // Self-test of the bounded wait: one warp waits on a barrier that nothing ever arrives on.  The
 // wait must give up after the time limit, record kStatusSelfTest and let the kernel return.
 constexpr uint32_t kStatusSelfTest = 0x7e57;
-__global__ void __launch_bounds__(32, 1) wait_timeout_selftest_kernel(unsigned int* status, unsigned long long timeout_ns) {
+static __global__ void __launch_bounds__(32, 1) wait_timeout_selftest_kernel(unsigned int* status, unsigned long long timeout_ns) {
   __shared__ __align__(8) uint64_t bar;
   __shared__ uint32_t abort_flag;
   if (threadIdx.x == 0) {

@@ -182,34 +182,6 @@ __global__ void lora_low_simple_kernel(const uint16_t* P, long ldp, const uint16
   if (lane == 0) out[m * ld_out + r] = lora_from_float<kIsBf16>(sum);
 }
 
-// C[m, n] = sum_l A[m, l] B[n, l] + sum_r low[m, r] W_g[n, r] in one fp32 sum, rounded once; the element (n, l) of B at
-// B + n * stride_bn + l * stride_bl.  Blocks of 16 x 16 threads, one element each.
-template <bool kIsBf16>
-__global__ void lora_product_simple_kernel(const uint16_t* A, long lda, const uint16_t* B, long stride_bn, long stride_bl,
-                                           const uint16_t* low, long ld_low, const uint16_t* W, long stride_g,
-                                           long stride_n, long stride_r, uint16_t* C, long ldc, int M, int N, int L, int R,
-                                           void* plan) {
-  const LoraPlanView v = lora_plan_view(plan, M);
-  __shared__ float sa[16][17], sb[16][17];
-  const int x = threadIdx.x, y = threadIdx.y;
-  const long n0 = static_cast<long>(blockIdx.x) * 16, m0 = static_cast<long>(blockIdx.y) * 16;
-  const long m = m0 + y, n = n0 + x;
-  float sum = 0.0f;
-  for (int l0 = 0; l0 < L; l0 += 16) {
-    sa[y][x] = m < M && l0 + x < L ? lora_to_float<kIsBf16>(A[m * lda + l0 + x]) : 0.0f;
-    sb[y][x] = n0 + y < N && l0 + x < L ? lora_to_float<kIsBf16>(B[(n0 + y) * stride_bn + (l0 + x) * stride_bl]) : 0.0f;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) sum += sa[y][i] * sb[x][i];
-    __syncthreads();
-  }
-  if (m >= M || n >= N) return;
-  const int g = v.row_adapter[m];
-  if (g >= 0)
-    for (int r = 0; r < R; ++r)
-      sum += lora_to_float<kIsBf16>(low[m * ld_low + r]) * lora_to_float<kIsBf16>(W[g * stride_g + n * stride_n + r * stride_r]);
-  C[m * ldc + n] = lora_from_float<kIsBf16>(sum);
-}
-
 // out_g[i, r] = sum over the rows m of adapter g of P[m, i] Q[m, r], stored at out + g * D * R + i * stride_i + r * stride_r.
 // One thread per element.
 template <bool kIsBf16>

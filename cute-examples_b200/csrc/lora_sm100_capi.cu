@@ -4,20 +4,15 @@
 
 #include <cstdint>
 
-#include "../../include/gemm_sm100.h"
+#include "gemm_host_sm100.cuh"
 #include "lora_sm100.cuh"
 
 namespace {
 
 using namespace gemm_sm100;
-
-int cuda_failed(int* out, cudaError_t e) {
-  if (out) *out = static_cast<int>(e);
-  return GEMM_SM100_ERR_CUDA;
-}
+using namespace gemm_sm100::host;
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 // What a 16-bit matrix of `cols` columns has to fulfil; `rows` <= 1 leaves the pitch unused but checked all the same.
 int check_matrix(const void* p, long cols, long ld) {
@@ -61,14 +56,168 @@ void launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const vo
       const_cast<void*>(a.plan));
 }
 
+// The ranks one adapter item covers: one swizzle row of 32, 64 or 128 bytes.
+int rank_chunk(int R) { return R <= 16 ? 16 : (R <= 32 ? 32 : 64); }
+
+// Tensor map of a 16-bit array of two or three dimensions, innermost first, whose rows of `box[0]` elements
+// land in shared memory with the swizzle of that width.
+int encode_rows(CUtensorMap* map, const void* base, int dtype, int rank, const long (&dims)[3], const long (&pitches)[2],
+                const int (&box)[3], int* cuda_error_out) {
+  const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]), static_cast<cuuint64_t>(dims[2])};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitches[0]) * 2u, static_cast<cuuint64_t>(pitches[1]) * 2u};
+  const cuuint32_t b[3] = {static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]), static_cast<cuuint32_t>(box[2])};
+  const cuuint32_t ones[3] = {1u, 1u, 1u};
+  const CUtensorMapSwizzle swizzle = box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : (box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  const CUtensorMapDataType type =
+      dtype == GEMM_SM100_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = g_encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, strides, b, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, cudaErrorInvalidValue);
+}
+
+// Tile configurations with an adapter kernel: every one the planner chooses by itself, but the few-tile ones
+// that it only takes through the workspace; the layouts' four for B as [K, N].
+constexpr unsigned kProductConfigs = (1u << 0) | (1u << 1) | (1u << 2) | (1u << 9) | (1u << 10) | (1u << 11) | (1u << 12) |
+                                     (1u << 13) | (1u << 14) | (1u << 15);
+constexpr unsigned kProductConfigsKN = 0xfu;
+// those whose K can be cut inside a cluster
+constexpr bool has_cluster_split(int config) { return config == 0 || config == 2 || config == 11 || config == 12; }
+
+// The product of the rows with the shared weight and, in the same accumulator, with their adapters.
+struct AdapterOperands {
+  const void* low;
+  long ld_low;
+  const void* W;          // [adapters, N, R], or [adapters, R, N] with p.b_is_kn
+  long ld_w, stride_w;
+  int R, adapters;
+  const void* plan;
+};
+
+template <int kCfgIndex, bool kIsBf16, bool kBIsKN>
+int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan& plan, DeviceState& st, cudaStream_t stream,
+                          int* cuda_error_out) {
+  using Cfg = ConfigOf<kCfgIndex, kIsBf16>;
+  auto kernel = gemm_lora_kernel<Cfg, false, kBIsKN>;
+  if constexpr (!kBIsKN && has_cluster_split(kCfgIndex)) {
+    if (plan.split_k) kernel = gemm_lora_kernel<Cfg, true, false>;
+  }
+  // Attributes of this instantiation and the persistent grid's limit, once per device.
+  static int max_ctas[kMaxDevices][2];
+  int limit;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    int& known = max_ctas[st.device][plan.split_k ? 1 : 0];
+    if (known == 0) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+      if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+      int held = 0;
+      if (Cfg::kCtaGroup == 1) {
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, Cfg::kThreads, Cfg::kSmemBytes);
+        held *= st.sm_count;
+      } else {
+        cudaLaunchConfig_t qc = {};
+        qc.gridDim = dim3(static_cast<unsigned>(st.sm_count - st.sm_count % 2));
+        qc.blockDim = dim3(Cfg::kThreads);
+        qc.dynamicSmemBytes = Cfg::kSmemBytes;
+        cudaLaunchAttribute qa[1];
+        qa[0].id = cudaLaunchAttributeClusterDimension;
+        qa[0].val.clusterDim.x = 2;
+        qa[0].val.clusterDim.y = 1;
+        qa[0].val.clusterDim.z = 1;
+        qc.attrs = qa;
+        qc.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&held, kernel, &qc);
+        held *= 2;
+      }
+      if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+      if (held < 1) return set_cuda_error(cuda_error_out, cudaErrorLaunchOutOfResources);
+      known = held < st.sm_count ? held : st.sm_count - st.sm_count % Cfg::kCtaGroup;
+    }
+    limit = known;
+  }
+
+  TileParams tp = base_tile_params<Cfg>(p, st);
+  int b_box = Cfg::kBRows;
+  if (plan.tiles_n > 0) {
+    tp.n_tiles = plan.tiles_n;
+    tp.bal_q = plan.bal_q;
+    tp.bal_rem = plan.bal_rem;
+    tp.bal_start = plan.bal_start;
+    b_box = 64 / Cfg::kCtaGroup;
+    tp.b_box_rows = b_box;
+  }
+  tp.k_rotate = k_order_for(p, plan.split_k);
+  if (plan.split_k) {
+    tp.sk_factor = plan.split_factor;
+    tp.sk_cluster = 1;
+  }
+  CUtensorMap map_a, map_b, map_c;
+  int rc = encode_2d(&map_a, p.A, p.dtype, p.M, p.K, p.lda, Cfg::kARows, cuda_error_out, Cfg::kKSub);
+  if (rc) return rc;
+  rc = kBIsKN ? encode_2d(&map_b, p.B, p.dtype, p.K, p.N, p.ldb, 64, cuda_error_out)
+              : encode_2d(&map_b, p.B, p.dtype, p.N, p.K, p.ldb, b_box, cuda_error_out, Cfg::kKSub);
+  if (rc) return rc;
+  rc = encode_2d(&map_c, p.C, p.dtype, p.M, tma_store_cols(p.N), p.ldc, 32, cuda_error_out);
+  if (rc) return rc;
+  LoraParams lora;
+  std::memset(&lora, 0, sizeof(lora));
+  lora.chunk = rank_chunk(o.R);
+  lora.chunks = static_cast<int>(ceil_div(o.R, lora.chunk));
+  rc = encode_rows(&lora.tmap_low, o.low, p.dtype, 2, {o.R, p.M, 1}, {o.ld_low, 0}, {lora.chunk, Cfg::kARows, 1}, cuda_error_out);
+  if (rc) return rc;
+  rc = kBIsKN ? encode_rows(&lora.tmap_w, o.W, p.dtype, 3, {p.N, o.R, o.adapters}, {o.ld_w, o.stride_w}, {64, lora.chunk, 1},
+                            cuda_error_out)
+              : encode_rows(&lora.tmap_w, o.W, p.dtype, 3, {o.R, p.N, o.adapters}, {o.ld_w, o.stride_w},
+                            {lora.chunk, b_box, 1}, cuda_error_out);
+  if (rc) return rc;
+  const LoraPlanView view = lora_plan_view(const_cast<void*>(o.plan), p.M);
+  lora.slot_count = view.slot_count;
+  lora.slot_adapter = view.slot_adapter;
+  lora.slot_mask = view.slot_mask;
+
+  long ctas = plan.ctas;
+  if (ctas > limit && !plan.split_k) ctas = limit;
+  const cudaError_t e = launch_kernel<Cfg>(kernel, ctas, plan.split_k ? plan.split_factor * Cfg::kCtaGroup : Cfg::kCtaGroup,
+                                           stream, map_a, map_b, map_c, tp, lora);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+}
+
 template <bool kIsBf16>
-void launch_product(const gemm_sm100_lora_args& a, const void* A, long lda, long stride_bn, long stride_bl, const void* low,
-                    long ld_low, const void* W, long stride_g, long stride_n, long stride_r, int N, int L, void* C, long ldc,
-                    cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(N, 16)), static_cast<unsigned>(ceil_div(a.M, 16)));
-  lora_product_simple_kernel<kIsBf16><<<grid, dim3(16, 16), 0, stream>>>(
-      u16(A), lda, u16(a.B), stride_bn, stride_bl, u16(low), ld_low, u16(W), stride_g, stride_n, stride_r, u16(C), ldc, a.M, N,
-      L, a.R, const_cast<void*>(a.plan));
+int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stream, int* cuda_error_out) {
+  DeviceState* st = nullptr;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    int rc = device_state(&st, cuda_error_out);
+    if (rc != GEMM_SM100_OK) return rc;
+    rc = get_encoder(cuda_error_out);
+    if (rc != GEMM_SM100_OK) return rc;
+  }
+  if (p.b_is_kn) {
+    const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/false, kProductConfigsKN, /*allow_balance=*/false);
+    switch (plan.config) {
+      case 0: return launch_product_config<0, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
+      case 1: return launch_product_config<1, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
+      case 2: return launch_product_config<2, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
+      default: return launch_product_config<3, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
+    }
+  }
+  const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigs, /*allow_balance=*/true,
+                             /*allow_workspace=*/false);
+  switch (plan.config) {
+    case 0: return launch_product_config<0, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 1: return launch_product_config<1, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 2: return launch_product_config<2, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 9: return launch_product_config<9, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 10: return launch_product_config<10, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 11: return launch_product_config<11, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 12: return launch_product_config<12, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 13: return launch_product_config<13, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 14: return launch_product_config<14, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 15: return launch_product_config<15, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    default: return GEMM_SM100_ERR_BAD_OPTION;
+  }
 }
 
 template <bool kIsBf16>
@@ -99,7 +248,7 @@ int gemm_sm100_lora_plan(const void* ids, int ids_are_64, int M, int adapters, v
   const unsigned blocks = static_cast<unsigned>(lora_plan_tiles(M) + adapters);
   lora_plan_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(ids, ids_are_64, M, adapters, plan);
   const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : cuda_failed(cuda_error_out, e);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low, void* cuda_stream, int* cuda_error_out) {
@@ -115,7 +264,7 @@ int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low
   auto launch = a.dtype == GEMM_SM100_BF16 ? launch_low<true> : launch_low<false>;
   launch(a, a.A, a.lda, a.down, a.stride_down, a.ld_down, 1, a.K, low, ld_low, stream);
   const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : cuda_failed(cuda_error_out, e);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* low, long ld_low, void* cuda_stream,
@@ -129,11 +278,10 @@ int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* l
   if ((rc = check_matrix(a.B, a.K, a.ldb)) || (rc = check_up(a)) || (rc = check_matrix(C, a.N, ldc))) return rc;
   rc = gemm_sm100_lora_low(args, low, ld_low, cuda_stream, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
-  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  auto launch = a.dtype == GEMM_SM100_BF16 ? launch_product<true> : launch_product<false>;
-  launch(a, a.A, a.lda, a.ldb, 1, low, ld_low, a.up, a.stride_up, a.ld_up, 1, a.N, a.K, C, ldc, stream);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : cuda_failed(cuda_error_out, e);
+  const Problem p{a.A, a.B, C, a.M, a.N, a.K, a.lda, a.ldb, ldc, a.dtype};
+  const AdapterOperands o{low, ld_low, a.up, a.ld_up, a.stride_up, a.R, a.adapters, a.plan};
+  return (a.dtype == GEMM_SM100_BF16 ? launch_product<true> : launch_product<false>)(
+      p, o, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
 }
 
 int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, const void* low, long ld_low,
@@ -153,7 +301,7 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
     const size_t bytes = static_cast<size_t>(a.adapters) * a.R * 2;
     if (d_down) e = cudaMemsetAsync(d_down, 0, bytes * a.K, stream);
     if (e == cudaSuccess && d_up) e = cudaMemsetAsync(d_up, 0, bytes * a.N, stream);
-    return e == cudaSuccess ? GEMM_SM100_OK : cuda_failed(cuda_error_out, e);
+    return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
   }
   if (!a.plan) return GEMM_SM100_ERR_NULL_POINTER;
   if ((rc = check_matrix(dC, a.N, ld_dc))) return rc;
@@ -165,13 +313,16 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
     if ((rc = check_up(a)) || (rc = check_matrix(d_low, a.R, ld_d_low))) return rc;
     (bf16 ? launch_low<true> : launch_low<false>)(a, dC, ld_dc, a.up, a.stride_up, 1, a.ld_up, a.N, d_low, ld_d_low, stream);
   }
-  if (dA)
-    (bf16 ? launch_product<true> : launch_product<false>)(a, dC, ld_dc, 1, a.ldb, d_low, ld_d_low, a.down, a.stride_down, 1,
-                                                          a.ld_down, a.K, a.N, dA, ld_da, stream);
+  if (dA) {
+    const Problem p{dC, a.B, dA, a.M, a.K, a.N, ld_dc, a.ldb, ld_da, a.dtype, /*b_is_kn=*/true};
+    const AdapterOperands o{d_low, ld_d_low, a.down, a.ld_down, a.stride_down, a.R, a.adapters, a.plan};
+    rc = (bf16 ? launch_product<true> : launch_product<false>)(p, o, stream, cuda_error_out);
+    if (rc != GEMM_SM100_OK) return rc;
+  }
   if (d_down) (bf16 ? launch_grad<true> : launch_grad<false>)(a, a.A, a.lda, d_low, ld_d_low, d_down, 1, a.K, a.K, stream);
   if (d_up) (bf16 ? launch_grad<true> : launch_grad<false>)(a, dC, ld_dc, low, ld_low, d_up, a.R, 1, a.N, stream);
   e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : cuda_failed(cuda_error_out, e);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 }  // extern "C"

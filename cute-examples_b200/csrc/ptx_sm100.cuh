@@ -335,6 +335,32 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint6
         : "memory");
 }
 
+// The same accumulating product for some rows of D only: bit i % 32 of `skip[i / 32]` set leaves row i (TMEM
+// lane i; rows 128.. are the pair peer's) as it is.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_f16_rows(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                              const uint32_t (&skip)[4 * kCtaGroup]) {
+  if constexpr (kCtaGroup == 1)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(skip[0]), "r"(skip[1]), "r"(skip[2]), "r"(skip[3])
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(skip[0]), "r"(skip[1]), "r"(skip[2]), "r"(skip[3]), "r"(skip[4]),
+        "r"(skip[5]), "r"(skip[6]), "r"(skip[7])
+        : "memory");
+}
+
 // Arrive on `bar` (shared::cluster address) once every tcgen05 op issued so far by
 // this thread has completed.  Implies tcgen05.fence::before_thread_sync.
 template <int kCtaGroup>
@@ -375,6 +401,18 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(1024 >> 4) << 32;                // stride byte offset [32,46)
   d |= static_cast<uint64_t>(1) << 46;                        // descriptor version (sm_100)
   d |= static_cast<uint64_t>(2) << 61;                        // layout: SWIZZLE_128B
+  return d;
+}
+
+// The same for rows of 32, 64 or 128 bytes with the swizzle of that width: 8-row groups 8 rows apart.
+__device__ __forceinline__ uint64_t make_smem_desc_rows(uint32_t smem_addr, uint32_t row_bytes) {
+  const uint64_t layout = row_bytes == 128u ? 2u : (row_bytes == 64u ? 4u : 6u);   // SWIZZLE_128B, _64B, _32B
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>((8u * row_bytes) >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= layout << 61;
   return d;
 }
 

@@ -147,3 +147,278 @@ def test_forward_and_gradients_against_the_definition(gk, M, N, K, R, G, kind, d
     res, tol = want(t)
     for name, value in got.items():
         check(name, value, res, tol)
+
+
+@pytest.fixture
+def options(gk):
+    changed = []
+
+    def set_option(name, value):
+        changed.append(name)
+        gk.set_option(name, value)
+
+    yield set_option
+    defaults = {"tile_config": -1, "split_k": -1, "sk_cluster": -1, "tiles_n": 0, "max_ctas": 0}
+    for name in changed:
+        gk.set_option(name, defaults[name])
+
+
+def forward_only(gk, t, **kw):
+    plan = gk.LoraPlan(t["ids"], t["down"].shape[0])
+    return gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], **kw)
+
+
+FORCED = [
+    # tile configuration, split_k, M, N, K, R, G
+    (0, 0, 600, 776, 320, 24, 5), (0, 2, 300, 520, 2048, 16, 9), (0, 4, 300, 520, 4096, 96, 3), (1, 0, 700, 1504, 200, 40, 4),
+    (2, 0, 300, 520, 320, 16, 7), (2, 2, 200, 520, 2048, 64, 40), (2, 4, 129, 264, 2112, 128, 6), (9, 0, 16, 1000, 264, 16, 16),
+    (10, 0, 64, 520, 328, 72, 30), (11, 0, 300, 648, 640, 8, 12), (11, 2, 257, 264, 2048, 32, 11), (12, 0, 128, 520, 640, 48, 90),
+    (12, 4, 100, 392, 4096, 16, 100), (12, 2, 100, 392, 2048, 80, 4), (13, 0, 16, 648, 576, 8, 16), (14, 0, 63, 648, 576, 128, 20),
+    (14, 0, 64, 200, 256, 16, 64), (15, 0, 9, 776, 640, 104, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("config,split,M,N,K,R,G", FORCED)
+def test_every_tile_configuration(gk, options, config, split, M, N, K, R, G, dtype):
+    t = make(M, N, K, R, G, dtype, 31 + config, id_pattern("random", M, G, config))
+    options("tile_config", config)
+    options("split_k", split)
+    options("sk_cluster", 1)
+    C = forward_only(gk, t)
+    gk.device_status()
+    res, tol = want(t)
+    check("C", C, res, tol)
+
+
+@pytest.mark.parametrize("config", [0, 1, 2, 3])
+@pytest.mark.parametrize("M,N,K,R,G", [(300, 264, 520, 16, 7), (600, 128, 1032, 72, 3), (100, 520, 264, 128, 50)])
+def test_every_tile_configuration_of_the_gradient(gk, options, config, M, N, K, R, G):
+    t = make(M, N, K, R, G, torch.bfloat16, 57 + config, id_pattern("random", M, G, config))
+    options("tile_config", config)
+    got = run_all(gk, t)
+    gk.device_status()
+    res, tol = want(t)
+    check("dA", got["dA"], res, tol)
+
+
+@pytest.mark.parametrize("config,tiles_n,N", [(1, 5, 2240), (0, 5, 1216), (2, 5, 1216)])
+def test_balanced_column_tiling(gk, options, config, tiles_n, N):
+    t = make(520, N, 256, 24, 4, torch.bfloat16, 71, id_pattern("runs", 520, 4, 3))
+    options("tile_config", config)
+    options("split_k", 0)
+    options("tiles_n", tiles_n)
+    C = forward_only(gk, t)
+    gk.device_status()
+    res, tol = want(t)
+    check("C", C, res, tol)
+
+
+@pytest.mark.parametrize("max_ctas", [2, 6])
+def test_many_tiles_per_cta(gk, options, max_ctas):
+    t = make(1500, 1544, 192, 40, 5, torch.bfloat16, 73, id_pattern("random", 1500, 5, 4))
+    options("max_ctas", max_ctas)
+    got = run_all(gk, t)
+    gk.device_status()
+    res, tol = want(t)
+    check("C", got["C"], res, tol)
+    check("dA", got["dA"], res, tol)
+
+
+@pytest.mark.parametrize("M,G,kind", [(96, 40, "own"), (1000, 4, "runs"), (700, 9, "random")])
+def test_broken_adapters_and_rows_stay_with_their_own(gk, M, G, kind):
+    """Inf and NaN in one adapter's weights and in its rows: every other row, and every other adapter's
+    gradient, keeps its bits."""
+    N, K, R = 520, 328, 16
+    t = make(M, N, K, R, G, torch.bfloat16, 5, id_pattern(kind, M, G, 6))
+    clean = run_all(gk, t)
+    bad = int(t["ids"][M // 2])
+    if not 0 <= bad < G:
+        bad = int(t["ids"][(t["ids"] >= 0) & (t["ids"] < G)][0])
+    theirs = t["ids"] == bad
+    broken = dict(t, A=t["A"].clone(), dC=t["dC"].clone(), down=t["down"].clone(), up=t["up"].clone())
+    broken["down"][bad, 3] = float("nan")
+    broken["up"][bad, :, 1] = float("inf")
+    rows = theirs.nonzero().flatten()
+    broken["A"][rows[0]] = float("nan")
+    broken["dC"][rows[-1]] = float("inf")
+    got = run_all(gk, broken)
+    others = torch.arange(G, device="cuda") != bad
+    for name in ("C", "low", "dA"):
+        assert torch.equal(got[name][~theirs], clean[name][~theirs]), name
+    for name in ("d_down", "d_up"):
+        assert torch.equal(got[name][others], clean[name][others]), name
+    assert not torch.isfinite(got["C"][theirs].float()).all()
+
+
+def test_rows_without_adapter_equal_the_plain_product(gk):
+    t = make(700, 1032, 512, 16, 4, torch.bfloat16, 8, id_pattern("runs", 700, 4, 2))
+    C = forward_only(gk, t)
+    plain = gk.gemm_tn(t["A"], t["B"])
+    none = (t["ids"] < 0) | (t["ids"] >= 4)
+    assert bool(none.any()) and torch.equal(C[none], plain[none])
+    t["ids"].fill_(-1)
+    assert torch.equal(forward_only(gk, t), plain)
+
+
+def test_strided_operands_and_untouched_neighbours(gk):
+    """Row and adapter pitches larger than the rows; nothing outside the outputs is written."""
+    M, N, K, R, G = 333, 397, 264, 24, 5
+    t = make(M, N + 3, K, R, G, torch.float16, 9, id_pattern("random", M, G, 1))
+    wide = {}
+    for name, shape in (("A", (M, K)), ("B", (N, K)), ("down", (G, R, K)), ("up", (G, N, R))):
+        big = torch.full([s + 8 for s in shape], float("nan"), dtype=torch.float16, device="cuda")
+        view = big[tuple(slice(0, s) for s in shape)]
+        view.copy_(t[name][tuple(slice(0, s) for s in shape)])
+        wide[name] = view
+    out = torch.full((M + 2, 416), 7.0, dtype=torch.float16, device="cuda")
+    low = torch.full((M + 1, 40), 5.0, dtype=torch.float16, device="cuda")
+    plan = gk.LoraPlan(t["ids"].long(), G)
+    got = gk.gemm_lora(wide["A"], wide["B"], wide["down"], wide["up"], plan, scale=t["scale"], out=out[:M, :N], low=low[:M, :R])
+    assert got.data_ptr() == out.data_ptr()
+    t["B"], t["up"], t["dC"] = t["B"][:N], t["up"][:, :N], t["dC"][:, :N]
+    res, tol = want(t)
+    check("C", got, res, tol)
+    check("low", low[:M, :R], res, tol)
+    assert bool((out[:, N:] == 7).all()) and bool((out[M:] == 7).all())
+    assert bool((low[:, R:] == 5).all()) and bool((low[M:] == 5).all())
+
+
+def test_same_bits_on_every_call(gk):
+    t = make(900, 520, 1024, 32, 6, torch.bfloat16, 10, id_pattern("random", 900, 6, 1))
+    first = run_all(gk, t)
+    for _ in range(3):
+        again = run_all(gk, t)
+        for name in first:
+            assert torch.equal(first[name], again[name]), name
+
+
+@pytest.mark.parametrize("needs", [(True, False, False), (False, True, False), (False, False, True), (False, False, False)])
+def test_only_the_wanted_gradients(gk, needs):
+    t = make(300, 264, 200, 16, 3, torch.bfloat16, 11, id_pattern("runs", 300, 3, 1))
+    plan = gk.LoraPlan(t["ids"], 3)
+    full = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"])
+    some = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], needs=needs)
+    for want_it, a, b in zip(needs, full, some):
+        assert torch.equal(a, b) if want_it else b is None
+
+
+def test_number_as_scale_and_kept_low_rows(gk):
+    t = make(200, 264, 200, 16, 3, torch.bfloat16, 12, id_pattern("random", 200, 3, 1))
+    t["scale"] = torch.full((3,), 0.75, device="cuda")
+    plan = gk.LoraPlan(t["ids"], 3)
+    low = torch.empty(200, 16, dtype=torch.bfloat16, device="cuda")
+    a = gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=0.75, low=low)
+    assert torch.equal(a, forward_only(gk, t))
+    kept = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=0.75, low=low)
+    again = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=0.75)
+    for x, y in zip(kept, again):
+        assert torch.equal(x, y)
+
+
+def test_empty_batch(gk):
+    t = make(0, 264, 200, 16, 3, torch.bfloat16, 13, torch.empty(0))
+    got = run_all(gk, t)
+    assert got["C"].shape == (0, 264) and got["dA"].shape == (0, 200)
+    assert bool((got["d_down"] == 0).all()) and bool((got["d_up"] == 0).all())
+
+
+def test_captured_step_follows_the_plan(gk):
+    """Forward and backward captured with the plan's update; replays with other ids and inputs give what the
+    eager calls give, also with two captured graphs that run side by side."""
+    M, N, K, R, G = 500, 520, 512, 16, 6
+    batches = [make(M, N, K, R, G, torch.bfloat16, 20 + i, id_pattern(kind, M, G, i))
+               for i, kind in enumerate(("runs", "random", "own"))]
+    eager = [run_all(gk, t) for t in batches]
+    graphs = []
+    for _ in range(2):
+        s = {k: v.clone() for k, v in batches[0].items()}
+        plan = gk.LoraPlan(s["ids"], G)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.update(s["ids"])
+            low = torch.empty(M, R, dtype=torch.bfloat16, device="cuda")
+            C = gk.gemm_lora(s["A"], s["B"], s["down"], s["up"], plan, scale=s["scale"], low=low)
+            grads = gk.gemm_lora_backward(s["dC"], s["A"], s["B"], s["down"], s["up"], plan, scale=s["scale"])
+        graphs.append((s, graph, dict(zip(("C", "low", "dA", "d_down", "d_up"), (C, low) + grads))))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for first, second in ((0, 1), (1, 2), (2, 0)):
+        torch.cuda.synchronize()
+        for (s, _, _), i in zip(graphs, (first, second)):
+            for k, v in batches[i].items():
+                s[k].copy_(v)
+        torch.cuda.synchronize()
+        for (_, graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, out), i in zip(graphs, (first, second)):
+            for name, value in out.items():
+                assert torch.equal(value, eager[i][name]), (name, i)
+    gk.device_status()
+
+
+def test_two_streams_at_once(gk):
+    t = [make(400, 776, 1024, 32, 5, torch.bfloat16, 30 + i, id_pattern("random", 400, 5, i)) for i in range(2)]
+    alone = [run_all(gk, x) for x in t]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    results = []
+    for _ in range(5):
+        for s, x in zip(streams, t):
+            with torch.cuda.stream(s):
+                results.append(run_all(gk, x))
+    torch.cuda.synchronize()
+    for i, got in enumerate(results):
+        for name in got:
+            assert torch.equal(got[name], alone[i % 2][name]), name
+
+
+def test_a_plan_outlives_its_last_reference(gk):
+    """A plan made on one stream and used on another may be dropped while the kernels that read it are queued."""
+    t = make(300, 520, 1024, 16, 4, torch.bfloat16, 40, id_pattern("random", 300, 4, 1))
+    alone = forward_only(gk, t)
+    side = torch.cuda.Stream()
+    plan = gk.LoraPlan(t["ids"], 4)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(20):
+            big = big @ big * 1e-4
+        got = gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"])
+    size = plan.buffer.numel()
+    del plan
+    torch.full((size,), 255, dtype=torch.uint8, device="cuda")     # would take the freed block
+    torch.cuda.synchronize()
+    assert torch.equal(got, alone)
+
+
+def test_gradients_against_differences(gk):
+    """Central differences of the plain 64-bit forward pass along random directions."""
+    M, N, K, R, G = 40, 64, 48, 8, 3
+    t = make(M, N, K, R, G, torch.float16, 50, id_pattern("random", M, G, 2))
+    got = run_all(gk, t)
+    ids, valid = t["ids"].long(), (t["ids"] >= 0) & (t["ids"] < G)
+    x = {k: t[k].double() for k in ("A", "B", "down", "up", "dC", "scale")}
+
+    def loss(A, down, up):
+        total = (A @ x["B"].T * x["dC"]).sum()
+        for m in valid.nonzero().flatten().tolist():
+            g = int(ids[m])
+            total = total + (x["scale"][g] * (up[g] @ (down[g] @ A[m])) * x["dC"][m]).sum()
+        return total
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for i, name in enumerate(("A", "down", "up")):
+        direction = torch.randn(x[name].shape, generator=gen, device="cuda", dtype=torch.float64)
+        args = [x["A"], x["down"], x["up"]]
+        step = 1e-3
+        up_args, down_args = list(args), list(args)
+        up_args[i], down_args[i] = args[i] + step * direction, args[i] - step * direction
+        slope = float((loss(*up_args) - loss(*down_args)) / (2 * step))
+        grad = got["dA" if name == "A" else "d_" + name].double()
+        # the loss is linear in each argument, so the difference is exact but for 64-bit rounding; each
+        # element of the gradient carries its own tolerance
+        _, tol = want(t)
+        bound = float((tol["dA" if name == "A" else "d_" + name] * direction.abs()).sum()) + 1e-6
+        assert abs(float((grad * direction).sum()) - slope) <= bound
