@@ -10,6 +10,8 @@
 
 #include <cstdint>
 
+#include "gemm_tn_sm100.cuh"
+
 namespace gemm_sm100 {
 
 constexpr int kLoraTileRows = 256;   // rows of one slot list: the rows of a pair tile of the GEMM
@@ -22,7 +24,7 @@ struct LoraPlanView {
   int* slot_count;       // [tiles]
   int* slot_adapter;     // [tiles][256]
   uint32_t* slot_mask;   // [tiles][256][8]: bit r % 32 of word r / 32 is row r of the tile
-  int* row_adapter;      // [M]: -1 for rows without an adapter
+  int* row_slot;         // [M]: the row's slot in its tile, -1 for rows without an adapter
   int* order;            // [M]
   int* offsets;          // [adapters + 1]
 };
@@ -41,8 +43,8 @@ __host__ __device__ inline LoraPlanView lora_plan_view(void* plan, long M) {
   v.slot_count = static_cast<int*>(plan);
   v.slot_adapter = v.slot_count + lora_plan_round(tiles);
   v.slot_mask = reinterpret_cast<uint32_t*>(v.slot_adapter + tiles * kLoraTileRows);
-  v.row_adapter = reinterpret_cast<int*>(v.slot_mask + tiles * kLoraTileRows * 8);
-  v.order = v.row_adapter + lora_plan_round(M);
+  v.row_slot = reinterpret_cast<int*>(v.slot_mask + tiles * kLoraTileRows * 8);
+  v.order = v.row_slot + lora_plan_round(M);
   v.offsets = v.order + lora_plan_round(M);
   return v;
 }
@@ -69,7 +71,6 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids
     const int tile = blockIdx.x;
     const long row = static_cast<long>(tile) * kLoraTileRows + t;
     const int id = row < M ? lora_read_id(ids, ids_are_64, row, adapters) : -1;
-    if (row < M) v.row_adapter[row] = id;
     s_id[t] = id;
     for (int w = 0; w < 8; ++w) s_mask[t][w] = 0;
     __syncthreads();
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids
     if (opens) s_slot[t] = slot;
     __syncthreads();
     if (id >= 0) atomicOr(&s_mask[s_slot[first]][warp], 1u << lane);   // the same mask in whatever order
+    if (row < M) v.row_slot[row] = id >= 0 ? s_slot[first] : -1;
     if (opens) v.slot_adapter[tile * kLoraTileRows + slot] = id;
     if (t == 0) v.slot_count[tile] = count;
     __syncthreads();
@@ -139,6 +141,232 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids
   }
 }
 
+// ------------------------------------------------------------------------------ low-rank rows
+// low[m] = s_g P[m] W_g^T over the long axis L: P = A and W = down [R, L], or (kRankInner) P = dC and W = up
+// [L, R].  A tile of 128 rows is one MMA operand; the adapters of the tile's rows lie side by side along
+// the MMA's N, in groups of up to 128 columns, so that P is read once however many adapters a group
+// holds, and every row takes its own adapter's columns out of the accumulator.  The work is a read of
+// P and of the adapters in use: bytes, not products, bound it.  L is cut over the CTAs of a cluster, which
+// add their partial rows through distributed shared memory in rank order.
+struct LowParams {
+  CUtensorMap tmap_p;    // [M, L]: boxes of 64 x p_rows
+  CUtensorMap tmap_w;    // [adapters, R, L]: boxes of 64 x R, or [adapters, L, R]: boxes of 64 ranks x 64
+  const void* plan;
+  const float* scales;
+  float scale;
+  void* out;             // [M, R], pitch ld_out
+  long ld_out;
+  int M, R, L;
+  int p_rows;            // rows per box of P: 128, or fewer when M is
+  int group_slots;       // adapters per group
+  int groups;            // CTA clusters per tile: groups are dealt to them round-robin
+  unsigned int* status;
+  unsigned long long timeout_ns;
+};
+
+struct LowConfig {
+  static constexpr int kThreads = 192;                 // producer, MMA issuer, four epilogue warps
+  static constexpr int kStages = 3;
+  static constexpr int kPBytes = 128 * 64 * 2, kWBytes = 128 * 64 * 2;
+  static constexpr int kStageBytes = kPBytes + kWBytes;
+  static constexpr int kTmemCols = 128;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 128;   // two CTAs per SM
+};
+
+template <bool kIsBf16, bool kRankInner>
+__global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const __grid_constant__ LowParams p) {
+  using Cfg = LowConfig;
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t smem_p = base, smem_w = base + kStages * Cfg::kPBytes;
+  uint8_t* bar_mem = smem_raw + (base - smem_u32(smem_raw)) + kStages * Cfg::kStageBytes;
+  const uint32_t full = smem_u32(bar_mem), empty = full + 8u * kStages, done = empty + 8u * kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 8 * (2 * kStages + 1));
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  uint32_t splits_reg;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits_reg));
+  const int splits = static_cast<int>(splits_reg);
+  const int unit = static_cast<int>(blockIdx.x) / splits;
+  const int tile = unit / p.groups, group0 = unit % p.groups;
+  WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    prefetch_tensormap(&p.tmap_p);
+    prefetch_tensormap(&p.tmap_w);
+    for (int b = 0; b < 2 * kStages + 1; ++b) mbar_init(full + 8u * b, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(tmem_slot), Cfg::kTmemCols);
+    tmem_relinquish<1>();
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const LoraPlanView v = lora_plan_view(const_cast<void*>(p.plan), p.M);
+  const int tile256 = tile >> 1;
+  const int slots = v.slot_count[tile256];
+  const int* adapters = v.slot_adapter + tile256 * kLoraTileRows;
+  const int k_blocks = (p.L + 63) / 64;
+  const int kb0 = static_cast<int>(static_cast<long>(k_blocks) * rank / splits);
+  const int kb1 = static_cast<int>(static_cast<long>(k_blocks) * (rank + 1) / splits);
+  const int R = p.R;
+  // columns of the accumulator per adapter: the ranks, or whole 64-element blocks of them
+  const int slot_cols = kRankInner ? (R > 64 ? 128 : 64) : R;
+  const int groups = slots == 0 ? 1 : (slots + p.group_slots - 1) / p.group_slots;   // (no slot: zeros are written)
+  const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
+  uint32_t step = 0;                                   // ring position, running on over the groups
+  uint32_t parity = 0;
+#pragma unroll 1
+  for (int group = group0; group < groups; group += p.groups, parity ^= 1u) {
+    const int slot0 = group * p.group_slots;
+    const int n_slots = min(p.group_slots, slots - slot0);
+    const bool ok = *abort_flag == 0;
+    if (n_slots > 0 && ok) {
+      if (warp == 0) {
+        const uint64_t pol = policy_evict_normal();
+        const bool issuer = elect_one();
+        const uint32_t w_bytes = kRankInner ? static_cast<uint32_t>(slot_cols) * 128u : static_cast<uint32_t>(R) * 128u;
+        const uint32_t bytes = static_cast<uint32_t>(p.p_rows) * 128u + n_slots * w_bytes;
+        uint32_t at = step;
+        for (int kb = kb0; kb < kb1; ++kb, ++at) {
+          const uint32_t s = at % kStages;
+          if (!wait_bounded(empty + 8u * s, ((at / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) break;
+          if (issuer) {
+            mbar_arrive_expect_tx(full + 8u * s, bytes);
+            tma_load_2d<1>(smem_p + s * Cfg::kPBytes, &p.tmap_p, full + 8u * s, kb * 64, tile * 128, pol);
+            for (int j = 0; j < n_slots; ++j) {
+              const int g = adapters[slot0 + j];
+              const uint32_t dst = smem_w + s * Cfg::kWBytes + j * w_bytes;
+              if constexpr (!kRankInner) {
+                tma_load_3d<1>(dst, &p.tmap_w, full + 8u * s, kb * 64, 0, g, pol);
+              } else {
+                for (int b = 0; b * 64 < R; ++b) tma_load_3d<1>(dst + b * 8192, &p.tmap_w, full + 8u * s, b * 64, kb * 64, g, pol);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      } else if (warp == 1) {
+        const bool issuer = elect_one();
+        const int n = kRankInner ? (R + 15) / 16 * 16 : (n_slots * R + 15) / 16 * 16;
+        const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>(n), kRankInner ? 1u : 0u, 0);
+        uint32_t at = step;
+        bool all = true;
+        for (int kb = kb0; kb < kb1; ++kb, ++at) {
+          const uint32_t s = at % kStages;
+          if (!wait_bounded(full + 8u * s, (at / kStages) & 1u, ctx, kStatusTimeoutMma)) {
+            all = false;
+            break;
+          }
+          tc_fence_after_sync();
+          if (issuer) {
+            const uint64_t dp = make_smem_desc_sw128(smem_p + s * Cfg::kPBytes);
+            if constexpr (!kRankInner) {
+              const uint64_t dw = make_smem_desc_sw128(smem_w + s * Cfg::kWBytes);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * k, idesc, kb > kb0 || k > 0);
+            } else {
+              for (int j = 0; j < n_slots; ++j) {
+                const uint64_t dw = make_smem_desc_sw128_mn(smem_w + s * Cfg::kWBytes + j * slot_cols * 128, 8192);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_f16<1>(tmem + j * slot_cols, dp + 2u * k, dw + 128u * k, idesc, kb > kb0 || k > 0);
+              }
+            }
+            umma_commit<1>(empty + 8u * s);
+            if (kb == kb1 - 1) umma_commit<1>(done);
+          }
+          __syncwarp();
+        }
+        (void)all;
+      } else {
+        // Every row's own columns, into the partial rows (the idle ring: all its loads have been consumed).
+        const int q = warp & 3;
+        const int row = q * 32 + static_cast<int>(lane);
+        const long m = static_cast<long>(tile) * 128 + row;
+        const int mine = m < p.M ? v.row_slot[m] - slot0 : -1;
+        if (wait_bounded(done, parity, ctx, kStatusTimeoutEpilogue)) {
+          tc_fence_after_sync();
+          const uint32_t dst = base + static_cast<uint32_t>(row * pitch) * 4u;
+#pragma unroll 1
+          for (int j = 0; j < n_slots; ++j) {
+            if (!__any_sync(0xffffffffu, mine == j)) continue;
+            for (int r = 0; r < R; r += 8) {
+              uint32_t x[8];
+              tmem_ld_32x8(tmem + (static_cast<uint32_t>(q * 32) << 16) + j * slot_cols + r, x);
+              tmem_ld_wait();
+              if (mine == j) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * 4u), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                             "r"(x[3])
+                             : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * 4u + 16u), "r"(x[4]), "r"(x[5]),
+                             "r"(x[6]), "r"(x[7])
+                             : "memory");
+              }
+            }
+          }
+          tc_fence_before_sync();
+        }
+      }
+      step += static_cast<uint32_t>(kb1 - kb0);
+    }
+    // every CTA's partial rows are written
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    // This CTA's share of the rows, summed over the cluster in rank order.
+    const int share = 128 / splits, quads = R / 4;
+    for (int i = threadIdx.x; i < share * quads; i += Cfg::kThreads) {
+      const int row = rank * share + i / quads, r = i % quads * 4;
+      const long m = static_cast<long>(tile) * 128 + row;
+      if (m >= p.M) break;
+      const int slot = v.row_slot[m];
+      uint16_t* out = static_cast<uint16_t*>(p.out) + m * p.ld_out + r;
+      if (slot < 0) {
+        if (group == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
+        continue;
+      }
+      if (slot < slot0 || slot >= slot0 + n_slots || !ok) continue;
+      const uint32_t src = base + static_cast<uint32_t>(row * pitch + r) * 4u;
+      float4 sum = ld_cluster_v4(map_to_cta(src, 0));
+      for (int c = 1; c < splits; ++c) {
+        const float4 x = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+      }
+      const float f = p.scales ? p.scale * p.scales[adapters[slot]] : p.scale;
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x * f), __float_as_uint(sum.y * f)),
+                     pack2<kIsBf16>(__float_as_uint(sum.z * f), __float_as_uint(sum.w * f)));
+    }
+    // the partial rows may go (to the next group's loads, or with the CTA); the plain reads and writes of the
+    // ring come before the next group's asynchronous ones
+    fence_proxy_async_smem();
+    cluster_arrive();
+    cluster_wait();
+  }
+
+  if (*abort_flag != 0) {
+#pragma unroll 1
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);   // a wait gave up: loads in flight land before the memory goes
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, Cfg::kTmemCols);
+  }
+}
+
 // ------------------------------------------------------------------------------ simple kernels
 template <bool kIsBf16>
 __device__ __forceinline__ float lora_to_float(uint16_t bits) {
@@ -158,28 +386,6 @@ __device__ __forceinline__ uint16_t lora_from_float(float x) {
     memcpy(&bits, &h, 2);
   }
   return bits;
-}
-
-// out[m, r] = s_g sum_l P[m, l] W_g[r, l], the element (r, l) of W_g at W + g * stride_g + r * stride_r + l * stride_l.
-// One warp per (row, r).
-template <bool kIsBf16>
-__global__ void lora_low_simple_kernel(const uint16_t* P, long ldp, const uint16_t* W, long stride_g, long stride_r,
-                                       long stride_l, const float* scales, float scale, uint16_t* out, long ld_out, int M,
-                                       int R, int L, void* plan) {
-  const LoraPlanView v = lora_plan_view(plan, M);
-  const long item = (static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (item >= static_cast<long>(M) * R) return;
-  const long m = item / R;
-  const int r = static_cast<int>(item % R), lane = threadIdx.x & 31;
-  const int g = v.row_adapter[m];
-  float sum = 0.0f;
-  if (g >= 0) {
-    const uint16_t* w = W + g * stride_g + r * stride_r;
-    for (int l = lane; l < L; l += 32) sum += lora_to_float<kIsBf16>(P[m * ldp + l]) * lora_to_float<kIsBf16>(w[l * stride_l]);
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    sum *= scales ? scale * scales[g] : scale;
-  }
-  if (lane == 0) out[m * ld_out + r] = lora_from_float<kIsBf16>(sum);
 }
 
 // out_g[i, r] = sum over the rows m of adapter g of P[m, i] Q[m, r], stored at out + g * D * R + i * stride_i + r * stride_r.

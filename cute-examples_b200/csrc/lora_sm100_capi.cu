@@ -47,13 +47,11 @@ int check_up(const gemm_sm100_lora_args& a) {
 const uint16_t* u16(const void* p) { return static_cast<const uint16_t*>(p); }
 uint16_t* u16(void* p) { return static_cast<uint16_t*>(p); }
 
-template <bool kIsBf16>
-void launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long stride_g, long stride_r,
-                long stride_l, int L, void* out, long ld_out, cudaStream_t stream) {
-  const long warps = static_cast<long>(a.M) * a.R;
-  lora_low_simple_kernel<kIsBf16><<<static_cast<unsigned>(ceil_div(warps, 8)), 256, 0, stream>>>(
-      u16(P), ldp, u16(W), stride_g, stride_r, stride_l, a.scales, a.scale, u16(out), ld_out, a.M, a.R, L,
-      const_cast<void*>(a.plan));
+// Device state and tensor map encoder.
+int ready(DeviceState** st, int* cuda_error_out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  const int rc = device_state(st, cuda_error_out);
+  return rc != GEMM_SM100_OK ? rc : get_encoder(cuda_error_out);
 }
 
 // The ranks one adapter item covers: one swizzle row of 32, 64 or 128 bytes.
@@ -187,13 +185,8 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
 template <bool kIsBf16>
 int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
-  {
-    std::lock_guard<std::mutex> lock(g_mutex);
-    int rc = device_state(&st, cuda_error_out);
-    if (rc != GEMM_SM100_OK) return rc;
-    rc = get_encoder(cuda_error_out);
-    if (rc != GEMM_SM100_OK) return rc;
-  }
+  const int rc = ready(&st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
   if (p.b_is_kn) {
     const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/false, kProductConfigsKN, /*allow_balance=*/false);
     switch (plan.config) {
@@ -218,6 +211,83 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
     case 15: return launch_product_config<15, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     default: return GEMM_SM100_ERR_BAD_OPTION;
   }
+}
+
+// Launch in clusters of `cluster` CTAs; a programmatic dependent of the kernel before it like the GEMM's kernels.
+template <class Kernel, class Params>
+cudaError_t launch_cluster(Kernel kernel, long ctas, int cluster, int threads, int smem_bytes, cudaStream_t stream,
+                           const Params& params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = g_opt_pdl.load() != 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
+// The dynamic shared-memory limit of a kernel, set once per device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices], int device) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (done[device]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[device] = true;
+  return e;
+}
+
+// low rows of P [M, L] through W: down [adapters, R, L], or (kRankInner) up [adapters, L, R].
+template <bool kIsBf16, bool kRankInner>
+int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
+               long ld_out, cudaStream_t stream, int* cuda_error_out) {
+  DeviceState* st = nullptr;
+  int rc = ready(&st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  auto kernel = lora_low_kernel<kIsBf16, kRankInner>;
+  static bool allowed[kMaxDevices];
+  cudaError_t e = allow_smem(kernel, LowConfig::kSmemBytes, allowed, st->device);
+  if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+
+  LowParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.p_rows = a.M >= 128 ? 128 : static_cast<int>(ceil_div(a.M, 8) * 8);
+  rc = encode_rows(&p.tmap_p, P, a.dtype, 2, {L, a.M, 1}, {ldp, 0}, {64, p.p_rows, 1}, cuda_error_out);
+  if (rc) return rc;
+  rc = kRankInner ? encode_rows(&p.tmap_w, W, a.dtype, 3, {a.R, L, a.adapters}, {ld_w, stride_w}, {64, 64, 1}, cuda_error_out)
+                  : encode_rows(&p.tmap_w, W, a.dtype, 3, {L, a.R, a.adapters}, {ld_w, stride_w}, {64, a.R, 1}, cuda_error_out);
+  if (rc) return rc;
+  p.plan = a.plan;
+  p.scales = a.scales;
+  p.scale = a.scale;
+  p.out = out;
+  p.ld_out = ld_out;
+  p.M = a.M, p.R = a.R, p.L = L;
+  p.group_slots = kRankInner ? (a.R > 64 ? 1 : 2) : 128 / a.R;
+  p.status = st->status_ptr;
+  p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
+
+  // Two CTAs fit on an SM.  L is cut over as many CTAs of a cluster as leave them all at work at once;
+  // what is free beyond that takes groups of adapters of the same tile (how many a tile really has is
+  // known on the device only: a CTA without a group has nothing to do).
+  const long tiles = ceil_div(a.M, 128), room = 2L * st->sm_count, k_blocks = ceil_div(L, 64);
+  int splits = 8;
+  while (splits > 1 && (tiles * splits > room || splits > k_blocks)) splits /= 2;
+  const long most_slots = a.adapters < (a.M < kLoraTileRows ? a.M : kLoraTileRows) ? a.adapters
+                                                                                 : (a.M < kLoraTileRows ? a.M : kLoraTileRows);
+  const long most_groups = ceil_div(most_slots, p.group_slots);
+  long groups = room / (tiles * splits);
+  groups = groups < 1 ? 1 : (groups > most_groups ? most_groups : groups);
+  p.groups = static_cast<int>(groups);
+  e = launch_cluster(kernel, tiles * groups * splits, splits, LowConfig::kThreads, LowConfig::kSmemBytes, stream, p);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 template <bool kIsBf16>
@@ -260,11 +330,9 @@ int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low
   if (a.M == 0) return GEMM_SM100_OK;
   if (!a.plan) return GEMM_SM100_ERR_NULL_POINTER;
   if ((rc = check_matrix(a.A, a.K, a.lda)) || (rc = check_down(a)) || (rc = check_matrix(low, a.R, ld_low))) return rc;
-  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  auto launch = a.dtype == GEMM_SM100_BF16 ? launch_low<true> : launch_low<false>;
-  launch(a, a.A, a.lda, a.down, a.stride_down, a.ld_down, 1, a.K, low, ld_low, stream);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+  auto launch = a.dtype == GEMM_SM100_BF16 ? launch_low<true, false> : launch_low<false, false>;
+  return launch(a, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low, ld_low, static_cast<cudaStream_t>(cuda_stream),
+                cuda_error_out);
 }
 
 int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* low, long ld_low, void* cuda_stream,
@@ -311,7 +379,9 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
   const bool bf16 = a.dtype == GEMM_SM100_BF16;
   if (dA || d_down) {
     if ((rc = check_up(a)) || (rc = check_matrix(d_low, a.R, ld_d_low))) return rc;
-    (bf16 ? launch_low<true> : launch_low<false>)(a, dC, ld_dc, a.up, a.stride_up, 1, a.ld_up, a.N, d_low, ld_d_low, stream);
+    rc = (bf16 ? launch_low<true, true> : launch_low<false, true>)(a, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low,
+                                                                   ld_d_low, stream, cuda_error_out);
+    if (rc != GEMM_SM100_OK) return rc;
   }
   if (dA) {
     const Problem p{dC, a.B, dA, a.M, a.K, a.N, ld_dc, a.ldb, ld_da, a.dtype, /*b_is_kn=*/true};
