@@ -367,44 +367,226 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
   }
 }
 
-// ------------------------------------------------------------------------------ simple kernels
-template <bool kIsBf16>
-__device__ __forceinline__ float lora_to_float(uint16_t bits) {
-  if constexpr (kIsBf16) return __uint_as_float(static_cast<uint32_t>(bits) << 16);
-  __half h;
-  memcpy(&h, &bits, 2);
-  return __half2float(h);
-}
-template <bool kIsBf16>
-__device__ __forceinline__ uint16_t lora_from_float(float x) {
-  uint16_t bits;
-  if constexpr (kIsBf16) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(x);
-    memcpy(&bits, &h, 2);
-  } else {
-    const __half h = __float2half_rn(x);
-    memcpy(&bits, &h, 2);
-  }
-  return bits;
-}
+// ------------------------------------------------------------------------------ adapters' gradients
+// out_g[i, r] = sum over the rows m of adapter g of P[m, i] Q[m, r]: d_down (P = A, Q = d_low, stored as [R, D])
+// and d_up (P = dC, Q = low, stored as [D, R]).  128 columns i of P are the MMA's M, the ranks its N, and the
+// rows are contracted: P and Q go to the tensor core as they lie in memory, as MN-major operands.  The rows of
+// an adapter may be anywhere in the batch, so threads gather them (plan order) with 16-byte asynchronous
+// copies into the swizzled tiles; places behind the last row are filled with zeros in both operands and read
+// nothing.  One read of P bounds it.  The rows are cut over the CTAs of a cluster, which add their
+// partial sums through distributed shared memory in rank order.
+struct GradSide {
+  const uint16_t* P;
+  const uint16_t* Q;
+  uint16_t* out;
+  long ldp, ldq;
+  int D;                 // columns of P; 0: this gradient is not wanted
+  int rank_outer;        // 1: out is [R, D], 0: [D, R]
+};
+struct GradParams {
+  GradSide side[2];
+  const void* plan;
+  int M, R, adapters;
+  int tiles0;            // column tiles of side 0
+  unsigned int* status;
+  unsigned long long timeout_ns;
+};
 
-// out_g[i, r] = sum over the rows m of adapter g of P[m, i] Q[m, r], stored at out + g * D * R + i * stride_i + r * stride_r.
-// One thread per element.
-template <bool kIsBf16>
-__global__ void lora_grad_simple_kernel(const uint16_t* P, long ldp, const uint16_t* Q, long ldq, uint16_t* out, long stride_i,
-                                        long stride_r, int M, int D, int R, void* plan) {
-  const LoraPlanView v = lora_plan_view(plan, M);
-  const long item = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (item >= static_cast<long>(D) * R) return;
-  const int g = blockIdx.y;
-  const long i = item % D, r = item / D;
-  float sum = 0.0f;
-  const int end = v.offsets[g + 1];
-  for (int at = v.offsets[g]; at < end; ++at) {
-    const long m = v.order[at];
-    sum += lora_to_float<kIsBf16>(P[m * ldp + i]) * lora_to_float<kIsBf16>(Q[m * ldq + r]);
+template <int kRankBlocks>   // 64-element blocks of ranks: 1 or 2
+struct GradConfig {
+  static constexpr int kThreads = 160;                 // four warps gather and store, one issues
+  static constexpr int kStages = 3;
+  static constexpr int kPBytes = 2 * 64 * 128, kQBytes = kRankBlocks * 64 * 128;
+  static constexpr int kStageBytes = kPBytes + kQBytes;
+  static constexpr int kTmemCols = kRankBlocks * 64;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 128;
+  static constexpr int kCtasPerSm = kRankBlocks == 1 ? 3 : 2;
+};
+
+template <bool kIsBf16, int kRankBlocks>
+__global__ void __launch_bounds__(160, GradConfig<kRankBlocks>::kCtasPerSm)
+lora_grad_kernel(const __grid_constant__ GradParams p) {
+  using Cfg = GradConfig<kRankBlocks>;
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t smem_p = base, smem_q = base + kStages * Cfg::kPBytes;
+  uint8_t* bar_mem = smem_raw + (base - smem_u32(smem_raw)) + kStages * Cfg::kStageBytes;
+  const uint32_t full = smem_u32(bar_mem), empty = full + 8u * kStages, done = empty + 8u * kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 8 * (2 * kStages + 1));
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  uint32_t splits_reg;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits_reg));
+  const int splits = static_cast<int>(splits_reg);
+  const int unit = static_cast<int>(blockIdx.x) / splits;
+  // units: the column tiles of side 0 of every adapter, then those of side 1
+  const int units0 = p.tiles0 * p.adapters;
+  const GradSide& side = p.side[unit < units0 ? 0 : 1];
+  const int tiles = (side.D + 127) / 128;
+  const int local = unit < units0 ? unit : unit - units0;
+  const int g = local / tiles, col0 = (local - g * tiles) * 128;
+  WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int b = 0; b < kStages; ++b) {
+      mbar_init(full + 8u * b, 4);
+      mbar_init(empty + 8u * b, 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
   }
-  out[static_cast<long>(g) * D * R + i * stride_i + r * stride_r] = lora_from_float<kIsBf16>(sum);
+  if (warp == 4) {
+    tmem_alloc<1>(smem_u32(tmem_slot), Cfg::kTmemCols);
+    tmem_relinquish<1>();
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const LoraPlanView v = lora_plan_view(const_cast<void*>(p.plan), p.M);
+  const int first = v.offsets[g], last = v.offsets[g + 1];
+  const int blocks = (last - first + 63) / 64;           // of 64 rows
+  auto block_of = [&](int c) { return static_cast<int>(static_cast<long>(blocks) * c / splits); };
+  const int b0 = block_of(rank), b1 = block_of(rank + 1);
+  const int R = p.R;
+  const int pitch = side.rank_outer ? 128 + 4 : R + 4;   // floats per row of the partial sums: [r][i] or [i][r]
+  if (b1 > b0) {
+    if (warp < 4) {
+      // Thread: 16-byte piece `piece` of the rows tid / 16 + 8 k of every block, and the same piece of Q
+      // where Q has it; two 64-column blocks of P, 128-byte swizzle.
+      const int tid = threadIdx.x, piece = tid & 15, r0 = tid >> 4;
+      const bool col_ok = col0 + piece * 8 < side.D, q_ok = piece * 8 < R;
+      const uint16_t* src_p = side.P + (col_ok ? col0 + piece * 8 : 0);
+      const uint16_t* src_q = side.Q + (q_ok ? piece * 8 : 0);
+      // row t of a block sits at t * 128, its piece c at c ^ (t % 8); t % 8 == r0 for all of this thread's rows
+      const uint32_t place = static_cast<uint32_t>((piece >> 3) * 8192 + r0 * 128 + (((piece & 7) ^ r0) << 4));
+      int row[8];
+      auto fetch_rows = [&](int b) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = first + b * 64 + r0 + 8 * k;
+          row[k] = b < b1 && at < last ? v.order[at] : -1;
+        }
+      };
+      fetch_rows(b0);
+      bool good = true;
+      int n = 0;
+      for (int b = b0; b < b1; ++b, ++n) {
+        const uint32_t s = static_cast<uint32_t>(n) % kStages;
+        if (!wait_bounded(empty + 8u * s, ((static_cast<uint32_t>(n) / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) {
+          good = false;
+          break;
+        }
+        const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool live = row[k] >= 0;
+          const long m = live ? row[k] : 0;
+          cp_async_16(dst_p + k * 1024u, src_p + m * side.ldp, live && col_ok);
+          if (q_ok) cp_async_16(dst_q + k * 1024u, src_q + m * side.ldq, live);
+        }
+        cp_async_commit();
+        fetch_rows(b + 1);
+        if (n >= kStages - 1) {
+          // the oldest stage in flight has landed: hand it to the tensor core
+          cp_async_wait<kStages - 1>();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + 8u * ((static_cast<uint32_t>(n) + 1u) % kStages));
+        }
+      }
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (good && lane == 0)
+        for (int t = n >= kStages - 1 ? n - (kStages - 1) : 0; t < n; ++t) mbar_arrive(full + 8u * (static_cast<uint32_t>(t) % kStages));
+    } else {
+      const bool issuer = elect_one();
+      const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>((R + 15) / 16 * 16), 1u, 1u);
+      for (int b = b0, n = 0; b < b1; ++b, ++n) {
+        const uint32_t s = static_cast<uint32_t>(n) % kStages;
+        if (!wait_bounded(full + 8u * s, (static_cast<uint32_t>(n) / kStages) & 1u, ctx, kStatusTimeoutMma)) break;
+        tc_fence_after_sync();
+        if (issuer) {
+          const uint64_t dp = make_smem_desc_sw128_mn(smem_p + s * Cfg::kPBytes, 8192);
+          const uint64_t dq = make_smem_desc_sw128_mn(smem_q + s * Cfg::kQBytes, 8192);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 128u * k, dq + 128u * k, idesc, n > 0 || k > 0);
+          umma_commit<1>(empty + 8u * s);
+          if (b == b1 - 1) umma_commit<1>(done);
+        }
+        __syncwarp();
+      }
+    }
+    if (warp < 4) {
+      if (wait_bounded(done, 0, ctx, kStatusTimeoutEpilogue)) {
+        // the partial sums, into the idle ring
+        tc_fence_after_sync();
+        const int i = warp * 32 + static_cast<int>(lane);
+        for (int r = 0; r < R; r += 8) {
+          uint32_t x[8];
+          tmem_ld_32x8(tmem + (static_cast<uint32_t>(warp * 32) << 16) + r, x);
+          tmem_ld_wait();
+          if (side.rank_outer) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + static_cast<uint32_t>((r + e) * pitch + i) * 4u), "r"(x[e])
+                           : "memory");
+          } else {
+            const uint32_t dst = base + static_cast<uint32_t>(i * pitch + r) * 4u;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                         : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 16u), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                         : "memory");
+          }
+        }
+        tc_fence_before_sync();
+      }
+    }
+  }
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  // This CTA's share of the sums, four neighbours at a time, added over the cluster in rank order.
+  {
+    const int per_row = (side.rank_outer ? 128 : R) / 4, quads = 32 * R;
+    const int q0 = quads * rank / splits, q1 = quads * (rank + 1) / splits;
+    uint16_t* out = side.out + static_cast<long>(g) * side.D * R;
+    for (int q = q0 + static_cast<int>(threadIdx.x); q < q1; q += Cfg::kThreads) {
+      const int y = q / per_row, x = q % per_row * 4;
+      const int i = col0 + (side.rank_outer ? x : y);
+      if (i >= side.D) continue;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const uint32_t src = base + static_cast<uint32_t>(y * pitch + x) * 4u;
+      for (int c = 0; c < splits; ++c) {
+        if (block_of(c) == block_of(c + 1)) continue;     // a CTA without rows
+        const float4 t = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
+        sum.x += t.x, sum.y += t.y, sum.z += t.z, sum.w += t.w;
+      }
+      const long at = side.rank_outer ? static_cast<long>(y) * side.D + i : static_cast<long>(i) * R + x;
+      *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x), __float_as_uint(sum.y)),
+                                                       pack2<kIsBf16>(__float_as_uint(sum.z), __float_as_uint(sum.w)));
+    }
+  }
+  cluster_arrive();
+  cluster_wait();
+  if (*abort_flag != 0) {
+#pragma unroll 1
+    for (int t = 0; t < 200; ++t) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, Cfg::kTmemCols);
+  }
 }
 
 }  // namespace gemm_sm100

@@ -290,12 +290,34 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
-template <bool kIsBf16>
-void launch_grad(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* Q, long ldq, void* out, long stride_i,
-                 long stride_r, int D, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<long>(D) * a.R, 256)), static_cast<unsigned>(a.adapters));
-  lora_grad_simple_kernel<kIsBf16><<<grid, 256, 0, stream>>>(u16(P), ldp, u16(Q), ldq, u16(out), stride_i, stride_r, a.M, D,
-                                                             a.R, const_cast<void*>(a.plan));
+// Both adapters' gradients in one launch.
+template <bool kIsBf16, int kRankBlocks>
+int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradSide& up, cudaStream_t stream,
+                int* cuda_error_out) {
+  using Cfg = GradConfig<kRankBlocks>;
+  DeviceState* st = nullptr;
+  const int rc = ready(&st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  auto kernel = lora_grad_kernel<kIsBf16, kRankBlocks>;
+  static bool allowed[kMaxDevices];
+  cudaError_t e = allow_smem(kernel, Cfg::kSmemBytes, allowed, st->device);
+  if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+  GradParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.side[0] = down;
+  p.side[1] = up;
+  p.plan = a.plan;
+  p.M = a.M, p.R = a.R, p.adapters = a.adapters;
+  p.tiles0 = static_cast<int>(ceil_div(down.D, 128));
+  p.status = st->status_ptr;
+  p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
+  // The rows may all belong to one adapter: a CTA gets at most 1024 of them where a cluster can do that.
+  int splits = 8;
+  while (splits > 1 && a.M <= 512L * splits) splits /= 2;
+  const long units = (ceil_div(down.D, 128) + ceil_div(up.D, 128)) * a.adapters;
+  if (units * splits > 0x7fffffffL) return GEMM_SM100_ERR_BAD_SHAPE;
+  e = launch_cluster(kernel, units * splits, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 }  // namespace
@@ -389,10 +411,11 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
     rc = (bf16 ? launch_product<true> : launch_product<false>)(p, o, stream, cuda_error_out);
     if (rc != GEMM_SM100_OK) return rc;
   }
-  if (d_down) (bf16 ? launch_grad<true> : launch_grad<false>)(a, a.A, a.lda, d_low, ld_d_low, d_down, 1, a.K, a.K, stream);
-  if (d_up) (bf16 ? launch_grad<true> : launch_grad<false>)(a, dC, ld_dc, low, ld_low, d_up, a.R, 1, a.N, stream);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+  if (!d_down && !d_up) return GEMM_SM100_OK;
+  const GradSide down{u16(a.A), u16(d_low), u16(d_down), a.lda, ld_d_low, d_down ? a.K : 0, 1};
+  const GradSide up{u16(dC), u16(low), u16(d_up), ld_dc, ld_low, d_up ? a.N : 0, 0};
+  if (a.R <= 64) return (bf16 ? launch_grad<true, 1> : launch_grad<false, 1>)(a, down, up, stream, cuda_error_out);
+  return (bf16 ? launch_grad<true, 2> : launch_grad<false, 2>)(a, down, up, stream, cuda_error_out);
 }
 
 }  // extern "C"
