@@ -209,6 +209,7 @@ TileParams base_tile_params(const Problem& p, const DeviceState& st) {
   tp.bal_rem = 0;
   tp.bal_start = 0;
   tp.b_box_rows = Cfg::kBRows;
+  tp.a_box_rows = Cfg::kARows;
   tp.early_prefetch = (g_opt_pdl.load() != 0 && g_opt_early_prefetch.load() != 0) ? 1 : 0;
   tp.status = st.status_ptr;
   tp.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;

@@ -76,6 +76,10 @@ struct TileParams {
   // for double-width configurations, more than kMmaN (both halves non-empty).
   int bal_q, bal_rem, bal_start;
   int b_box_rows;  // rows per TMA box of B: kBRows for uniform tiles, 64 / kCtaGroup for balanced ones
+  // Rows per TMA box of A; fewer than kARows only in the adapter kernels and when M is smaller: a box that is
+  // mostly rows that do not exist loads slowly (1 x 4096 x 4096, 128 x 128 tiles: 25.2 us against 15.4 us for 16 rows),
+  // and what the MMA then reads behind the loaded rows only reaches accumulator rows >= M.
+  int a_box_rows;
   // > 0: before waiting for the previous kernel of the stream (programmatic dependent launch), the
   // producer asks L2 for the operand boxes of its first two stages.  A prefetch is only a hint
   // and L2 is where this GPU's writes become visible, so it is safe whatever that kernel still
@@ -212,6 +216,13 @@ struct GemmConfig {
   static_assert(kEpiBufs == 1 || kEpiBufs == 2, "staging buffers per epilogue warp");
   // the MMA reads 128 rows from every A stage: the last stage's read must stay inside the ring
   static_assert(kStages * kABytes + kBlockM * kBlockK * 2 - kABytes <= kStages * kStageBytes, "A over-read leaves the ring");
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// Where the adapter kernels keep a segment's plan entries, behind the barriers.
+template <class Cfg>
+struct LoraConfig : Cfg {
+  static constexpr int kSmemBytes = Cfg::kSmemBytes + 256 + 32 * 32;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
@@ -387,25 +398,44 @@ __device__ __forceinline__ TileCols tile_columns(int n_tile, const TileParams& p
   return t;
 }
 
-// The adapter stages of one segment: items [item0, item1) in groups of what a ring stage holds.  A tile
-// that is cut along K deals its stages to the contributors like its K blocks.
+// The adapter stages of one segment.  The tile's items, `per_stage` to a ring stage, are dealt stage by stage to
+// the contributors of a tile that is cut along K.  Which adapters and rows they are is read from the plan: an
+// issuing warp that waited for such a load in the middle of its loop left the tensor core idle for one to two
+// microseconds per load (8192 x 4096 x 4096, rank 16: 90 us more than without adapters), so the first 32 entries of
+// a segment are copied to shared memory while its K blocks run and picked up behind them.
 struct LoraWork {
-  int item0, item1, per_stage, stages;
+  int stages, items, per_stage, part, factor;
+  int base;                                // the tile's first slot in the plan
+  __device__ __forceinline__ int slot_of(int entry, int chunks) const {   // entry: this segment's items in order
+    const int stage = entry / per_stage;
+    return ((part + stage * factor) * per_stage + entry - stage * per_stage) / chunks;
+  }
 };
+constexpr int kLoraEntries = 32;
+
 template <class Cfg>
-__device__ __forceinline__ LoraWork lora_work(const LoraParams& lora, int m_tile, int part, int factor) {
-  const int slots = lora.slot_count[Cfg::kCtaGroup == 2 ? m_tile : m_tile >> 1];
+__device__ __forceinline__ LoraWork lora_begin(const LoraParams& lora, int m_tile, int part, int factor, uint32_t count_dst) {
   LoraWork w;
+  w.part = part;
+  w.factor = factor > 1 ? factor : 1;
   w.per_stage = Cfg::kBlockK / lora.chunk;
-  const int items = slots * lora.chunks;
-  const int all = (items + w.per_stage - 1) / w.per_stage;
-  const int first = factor > 1 ? (int)((long long)part * all / factor) : 0;
-  const int last = factor > 1 ? (int)((long long)(part + 1) * all / factor) : all;
-  // (a loaded value: handed back as warp-uniform for the issue loops)
-  w.stages = __reduce_max_sync(0xffffffffu, last - first);
-  w.item0 = __reduce_max_sync(0xffffffffu, first * w.per_stage);
-  w.item1 = __reduce_max_sync(0xffffffffu, items < last * w.per_stage ? items : last * w.per_stage);
+  w.stages = w.items = 0;
+  const int tile = Cfg::kCtaGroup == 2 ? m_tile : m_tile >> 1;
+  w.base = tile * 256;
+  if (lane_id() == 0) cp_async_4(count_dst, lora.slot_count + tile);
   return w;
+}
+// The entries have arrived: how many stages they make.
+__device__ __forceinline__ void lora_resolve(LoraWork& w, const LoraParams& lora, uint32_t count_src) {
+  cp_async_wait<0>();
+  __syncwarp();
+  int count;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(count) : "r"(count_src) : "memory");
+  w.items = count * lora.chunks;
+  const int all = (w.items + w.per_stage - 1) / w.per_stage;
+  const int stages = all > w.part ? (all - w.part + w.factor - 1) / w.factor : 0;
+  // (a loaded value: handed back as warp-uniform for the issue loops)
+  w.stages = __reduce_max_sync(0xffffffffu, stages);
 }
 
 template <bool kIsBf16>
@@ -475,6 +505,8 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
   constexpr uint32_t kRxReadyOff = Cfg::kBarrierBytes - 16, kRxDoneOff = Cfg::kBarrierBytes - 8;
   static_assert(8 * (2 * kStages + 5) + 8 <= Cfg::kBarrierBytes - 16, "barrier block too small");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 8 * (2 * kStages + 5));
+  // adapter kernels: where the plan's entries land (producer: count, adapters; MMA issuer: count, row masks)
+  [[maybe_unused]] const uint32_t lora_smem = bar_base + Cfg::kBarrierBytes;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -605,7 +637,10 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
   // Everything up to here used only this CTA's own resources (and hints to L2).  Global memory
   // (operands that the previous kernel in the stream may have written, C that it may still be
   // writing) comes next.
-  grid_dependency_wait();
+  // The adapter kernels wait later: the kernel in front of them computes the low rows and lets them start
+  // only after its own wait, when everything before it has completed.  So all they need it for are the
+  // low rows, and the K loop runs beside it.
+  if constexpr (!kLora) grid_dependency_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -628,8 +663,10 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       const int b_box = p.b_box_rows;
       bool seg_start = true, backwards = false;
       bool ok = true;
-      [[maybe_unused]] LoraWork lw = {0, 0, 1, 0};
-      [[maybe_unused]] int slot_base = 0;
+      [[maybe_unused]] LoraWork lw = {};
+      [[maybe_unused]] int entry_adapter = 0;             // lane i: adapter of entry i of the current 32
+      [[maybe_unused]] bool low_ready = false;
+      const int a_rows = kLora ? p.a_box_rows : Cfg::kARows;
       int seg_end = seg.kb1;                              // the segment's K blocks, then its adapter stages
       long long stall = 0;
       while (have && ok) {
@@ -645,24 +682,16 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             rows_b[1] = tc.w1 / G;
             row_b[0] = tc.col0 + (int)cta_rank * rows_b[0];
             row_b[1] = tc.col0 + tc.w0 + (int)cta_rank * rows_b[1];
-            tx_bytes = (uint32_t)(Cfg::kABytes + (rows_b[0] + rows_b[1]) * Cfg::kBlockK * 2) * G;
+            tx_bytes = (uint32_t)(a_rows * Cfg::kBlockK * 2 + (rows_b[0] + rows_b[1]) * Cfg::kBlockK * 2) * G;
             rot = p.k_rotate == 1 ? (int)(((long long)seg.tile * k_blocks) / num_tiles) : 0;
             backwards = !kSplitK && p.k_rotate == 2 && (tiles_done & 1);
             ++tiles_done;
             seg_start = false;
             seg_end = seg.kb1;
             if constexpr (kLora) {
-              lw = lora_work<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 0);
-              slot_base = (G == 2 ? m_tile : m_tile >> 1) * 256;
-              seg_end += lw.stages;
-            }
-          }
-          [[maybe_unused]] int item = 0, items = 0, item_adapter = 0;
-          if constexpr (kLora) {
-            if (kb >= seg.kb1) {                          // an adapter stage: lane i fetches the adapter of item i
-              item = lw.item0 + (kb - seg.kb1) * lw.per_stage;
-              items = min(lw.per_stage, lw.item1 - item);
-              if ((int)lane < items) item_adapter = lora->slot_adapter[slot_base + (item + (int)lane) / lora->chunks];
+              lw = lora_begin<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 1, lora_smem);
+              const int slot = lw.slot_of((int)lane, lora->chunks);
+              if (slot < 256) cp_async_4(lora_smem + 16u + lane * 4u, lora->slot_adapter + lw.base + slot);
             }
           }
           long long t0 = 0;
@@ -675,21 +704,32 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             if (trace) stall += clock64() - t0;
           if constexpr (kLora) {
             if (kb >= seg.kb1) {
+              if (!low_ready) {
+                grid_dependency_wait();
+                low_ready = true;
+              }
               const int chunk = lora->chunk, chunks = lora->chunks;
-              const uint32_t low_bytes = (uint32_t)(Cfg::kARows * chunk * 2);
+              const int stage = kb - seg.kb1, first = (lw.part + stage * lw.factor) * lw.per_stage;
+              const int items = min(lw.per_stage, lw.items - first);
+              const int entry = stage * lw.per_stage;
+              if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
+                const int slot = lw.slot_of(entry + (int)lane, chunks);
+                entry_adapter = slot < 256 ? lora->slot_adapter[lw.base + slot] : 0;
+              }
+              const uint32_t low_stride = (uint32_t)(Cfg::kARows * chunk * 2);
               const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);     // one item's tile of W per half
               if (issuer && is_leader)
                 mbar_arrive_expect_tx(bar_base + kFullOff + 8u * s,
-                                      G * ((chunks == 1 ? 1 : items) * low_bytes +
-                                           (uint32_t)(items * (rows_b[0] + rows_b[1]) * chunk * 2)));
+                                      (uint32_t)(G * chunk * 2 *
+                                                 ((chunks == 1 ? 1 : items) * a_rows + items * (rows_b[0] + rows_b[1]))));
               const uint32_t full = full_leader + 8u * s;
               for (int i = 0; i < items; ++i) {
-                const int g = __shfl_sync(0xffffffffu, item_adapter, i);
-                const int r = (chunks == 1 ? 0 : (item + i) % chunks) * chunk;
+                const int g = __shfl_sync(0xffffffffu, entry_adapter, (entry + i) % kLoraEntries);
+                const int r = (chunks == 1 ? 0 : (first + i) % chunks) * chunk;
                 if (issuer) {
                   // slots of one chunk share the tile of low rows
                   if (i == 0 || chunks > 1)
-                    tma_load_2d<G>(smem_a + s * Cfg::kABytes + (uint32_t)i * low_bytes, &lora->tmap_low, full, r, row_a, pol);
+                    tma_load_2d<G>(smem_a + s * Cfg::kABytes + (uint32_t)i * low_stride, &lora->tmap_low, full, r, row_a, pol);
 #pragma unroll
                   for (int h = 0; h < Cfg::kHalves; ++h) {
                     const uint32_t dst = smem_b + s * Cfg::kBBytes + h * Cfg::kBHalfBytes + (uint32_t)i * w_bytes;
@@ -753,6 +793,12 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             }
           }
           if (++kb == seg_end) {
+            if constexpr (kLora) {
+              lora_resolve(lw, *lora, lora_smem);
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(entry_adapter) : "r"(lora_smem + 16u + lane * 4u) : "memory");
+              seg_end += lw.stages;
+              if (lw.stages > 0) continue;
+            }
             have = work.next(seg);
             kb = seg.kb0;
             seg_start = true;
@@ -793,8 +839,11 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       bool have = work.next(seg);
       int kb = seg.kb0, iter = 0;          // iter counts segments: it selects the accumulator slot
       bool ok = peer_ready;
-      [[maybe_unused]] LoraWork lw = {0, 0, 1, 0};
-      [[maybe_unused]] int slot_base = 0;
+      [[maybe_unused]] LoraWork lw = {};
+      [[maybe_unused]] uint4 entry_rows[G];                // lane i: row mask of entry i of the current 32
+      [[maybe_unused]] int half = 0;                       // which 128 rows of the plan's 256-row tile (single-CTA tiles)
+      [[maybe_unused]] const uint32_t count_smem = lora_smem + 160u, mask_smem = lora_smem + 256u;
+      const int a_rows = kLora ? p.a_box_rows : Cfg::kARows;
       int seg_end = seg.kb1;
       long long stall_full = 0, stall_acc = 0;
       const bool skip_mma = kDebug && (dbg & kDebugSkipMma);
@@ -811,28 +860,14 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             idesc_h[1] = idesc_base | ((uint32_t)(tc.w1 >> 3) << 17);
             seg_end = seg.kb1;
             if constexpr (kLora) {
-              lw = lora_work<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 0);
-              slot_base = (G == 2 ? m_tile : m_tile >> 1) * 256;
-              seg_end += lw.stages;
-              if constexpr (G == 1) slot_base = slot_base * 2 + (m_tile & 1);   // in half masks of 128 rows
-            }
-          }
-          [[maybe_unused]] int item = 0, items = 0;
-          [[maybe_unused]] uint4 item_rows[G];
-          if constexpr (kLora) {
-            if (kb >= seg.kb1) {
-              // adapter stage: lane i fetches the row mask of item i while the operands are on their way
-              item = lw.item0 + (kb - seg.kb1) * lw.per_stage;
-              items = min(lw.per_stage, lw.item1 - item);
-              if ((int)lane < items) {
-                const int slot = (item + (int)lane) / lora->chunks;
-                const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask);
-                if constexpr (G == 1) {
-                  item_rows[0] = masks[slot_base + 2 * slot];
-                } else {
-                  item_rows[0] = masks[2 * (slot_base + slot)];
-                  item_rows[1] = masks[2 * (slot_base + slot) + 1];
-                }
+              lw = lora_begin<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 1, count_smem);
+              half = m_tile & 1;
+              const int slot = lw.slot_of((int)lane, lora->chunks);
+              if (slot < 256) {
+                const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask) + 2 * (size_t)(lw.base + slot);
+#pragma unroll
+                for (int v = 0; v < G; ++v)
+                  cp_async_16(mask_smem + (lane * G + v) * 16u, masks + (G == 1 ? half : v), true);
               }
             }
           }
@@ -853,11 +888,34 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               }
             }
           tc_fence_after_sync();
+          if constexpr (kLora) {
+            if (kb == seg.kb1 - 1) {
+              lora_resolve(lw, *lora, count_smem);
+#pragma unroll
+              for (int v = 0; v < G; ++v)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(entry_rows[v].x), "=r"(entry_rows[v].y), "=r"(entry_rows[v].z), "=r"(entry_rows[v].w)
+                             : "r"(mask_smem + (lane * G + v) * 16u)
+                             : "memory");
+              seg_end += lw.stages;
+            }
+          }
           const bool last_kb = kb == seg_end - 1;
           if constexpr (kLora) {
             if (kb >= seg.kb1) {
               const int chunk = lora->chunk, chunks = lora->chunks;
-              const uint32_t low_bytes = (uint32_t)(Cfg::kARows * chunk * 2);
+              const int stage = kb - seg.kb1, first = (lw.part + stage * lw.factor) * lw.per_stage;
+              const int items = min(lw.per_stage, lw.items - first);
+              const int entry = stage * lw.per_stage;
+              if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
+                const int slot = lw.slot_of(entry + (int)lane, chunks);
+                if (slot < 256) {
+                  const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask) + 2 * (size_t)(lw.base + slot);
+#pragma unroll
+                  for (int v = 0; v < G; ++v) entry_rows[v] = masks[G == 1 ? half : v];
+                }
+              }
+              const uint32_t low_stride = (uint32_t)(Cfg::kARows * chunk * 2);
               const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);
               const uint64_t dl0 = make_smem_desc_rows(smem_a + s * Cfg::kABytes, (uint32_t)chunk * 2u);
               const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(smem_b + s * Cfg::kBBytes, (uint32_t)chunk * 128u)
@@ -868,12 +926,12 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
                 uint32_t skip[4 * G];
 #pragma unroll
                 for (int v = 0; v < G; ++v) {
-                  skip[4 * v] = ~__shfl_sync(0xffffffffu, item_rows[v].x, i);
-                  skip[4 * v + 1] = ~__shfl_sync(0xffffffffu, item_rows[v].y, i);
-                  skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, item_rows[v].z, i);
-                  skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, item_rows[v].w, i);
+                  skip[4 * v] = ~__shfl_sync(0xffffffffu, entry_rows[v].x, (entry + i) % kLoraEntries);
+                  skip[4 * v + 1] = ~__shfl_sync(0xffffffffu, entry_rows[v].y, (entry + i) % kLoraEntries);
+                  skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, entry_rows[v].z, (entry + i) % kLoraEntries);
+                  skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, entry_rows[v].w, (entry + i) % kLoraEntries);
                 }
-                const uint64_t dl = dl0 + (uint64_t)((chunks == 1 ? 0u : (uint32_t)i * low_bytes) >> 4);
+                const uint64_t dl = dl0 + (uint64_t)((chunks == 1 ? 0u : (uint32_t)i * low_stride) >> 4);
                 const uint64_t dw = dw0 + (uint64_t)(((uint32_t)i * w_bytes) >> 4);
                 if (issuer) {
 #pragma unroll
@@ -934,7 +992,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
                 for (int k = 1; k < Cfg::kBlockK / Cfg::kUmmaK; ++k) {
                   // four steps inside a 64-element K block, then on to the stage's next K block (its own
                   // K-major tile, right behind the first)
-                  constexpr uint32_t kASub = (uint32_t)(Cfg::kABytes / Cfg::kKSub) >> 4;
+                  const uint32_t kASub = kLora ? (uint32_t)a_rows * 8u : (uint32_t)(Cfg::kABytes / Cfg::kKSub) >> 4;
                   constexpr uint32_t kBSub = (uint32_t)(Cfg::kBHalfBytes / Cfg::kKSub) >> 4;
                   umma_f16<G>(tmem_d, da + kASub * (k >> 2) + kAStepK * (k & 3), db + kBSub * (k >> 2) + kBStepK * (k & 3),
                               idesc_h[h], 1u);
@@ -1431,6 +1489,9 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
         trace[kTraceEpiEnd] = clock64();
       }
   }
+
+  // (this kernel is complete only when the one in front of it is)
+  if constexpr (kLora) grid_dependency_wait();
 
   // ------------------------------------------------------------------ tear-down
   if (*abort_flag != 0) {

@@ -170,7 +170,8 @@ struct LowConfig {
   static constexpr int kPBytes = 128 * 64 * 2, kWBytes = 128 * 64 * 2;
   static constexpr int kStageBytes = kPBytes + kWBytes;
   static constexpr int kTmemCols = 128;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 128;   // two CTAs per SM
+  static constexpr int kBarrierBytes = 128;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + 128 * 8;   // two CTAs per SM
 };
 
 template <bool kIsBf16, bool kRankInner>
@@ -184,6 +185,8 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
   const uint32_t full = smem_u32(bar_mem), empty = full + 8u * kStages, done = empty + 8u * kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 8 * (2 * kStages + 1));
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  int* row_slot = reinterpret_cast<int*>(bar_mem + Cfg::kBarrierBytes);
+  float* row_factor = reinterpret_cast<float*>(row_slot + 128);
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
   const int rank = static_cast<int>(cluster_ctarank());
@@ -209,16 +212,17 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  grid_launch_dependents();
   grid_dependency_wait();
+  // only now: the product kernel behind this one relies on everything before this kernel being complete
+  grid_launch_dependents();
 
   const LoraPlanView v = lora_plan_view(const_cast<void*>(p.plan), p.M);
   const int tile256 = tile >> 1;
   const int slots = v.slot_count[tile256];
   const int* adapters = v.slot_adapter + tile256 * kLoraTileRows;
   const int k_blocks = (p.L + 63) / 64;
-  const int kb0 = static_cast<int>(static_cast<long>(k_blocks) * rank / splits);
-  const int kb1 = static_cast<int>(static_cast<long>(k_blocks) * (rank + 1) / splits);
+  // The CTAs of a cluster take the K blocks in turn: what they read of a row of P at any moment is contiguous.
+  const int steps = (k_blocks - rank + splits - 1) / splits;
   const int R = p.R;
   // columns of the accumulator per adapter: the ranks, or whole 64-element blocks of them
   const int slot_cols = kRankInner ? (R > 64 ? 128 : 64) : R;
@@ -226,6 +230,15 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
   const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
   uint32_t step = 0;                                   // ring position, running on over the groups
   uint32_t parity = 0;
+  if (warp >= 2) {
+    // every row's slot and factor, while the first operands are on their way
+    const int row = (warp & 3) * 32 + static_cast<int>(lane);
+    const long m = static_cast<long>(tile) * 128 + row;
+    const int slot = m < p.M ? v.row_slot[m] : -1;
+    row_slot[row] = slot;
+    row_factor[row] = slot >= 0 && p.scales ? p.scale * p.scales[adapters[slot]] : p.scale;
+    __syncwarp();
+  }
 #pragma unroll 1
   for (int group = group0; group < groups; group += p.groups, parity ^= 1u) {
     const int slot0 = group * p.group_slots;
@@ -237,16 +250,19 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
         const bool issuer = elect_one();
         const uint32_t w_bytes = kRankInner ? static_cast<uint32_t>(slot_cols) * 128u : static_cast<uint32_t>(R) * 128u;
         const uint32_t bytes = static_cast<uint32_t>(p.p_rows) * 128u + n_slots * w_bytes;
+        const int my_adapter = static_cast<int>(lane) < n_slots ? adapters[slot0 + lane] : 0;
         uint32_t at = step;
-        for (int kb = kb0; kb < kb1; ++kb, ++at) {
+        for (int kb = rank; kb < k_blocks; kb += splits, ++at) {
           const uint32_t s = at % kStages;
           if (!wait_bounded(empty + 8u * s, ((at / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) break;
           if (issuer) {
             mbar_arrive_expect_tx(full + 8u * s, bytes);
             tma_load_2d<1>(smem_p + s * Cfg::kPBytes, &p.tmap_p, full + 8u * s, kb * 64, tile * 128, pol);
-            for (int j = 0; j < n_slots; ++j) {
-              const int g = adapters[slot0 + j];
-              const uint32_t dst = smem_w + s * Cfg::kWBytes + j * w_bytes;
+          }
+          for (int j = 0; j < n_slots; ++j) {
+            const int g = __shfl_sync(0xffffffffu, my_adapter, j);
+            const uint32_t dst = smem_w + s * Cfg::kWBytes + j * w_bytes;
+            if (issuer) {
               if constexpr (!kRankInner) {
                 tma_load_3d<1>(dst, &p.tmap_w, full + 8u * s, kb * 64, 0, g, pol);
               } else {
@@ -261,40 +277,34 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
         const int n = kRankInner ? (R + 15) / 16 * 16 : (n_slots * R + 15) / 16 * 16;
         const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>(n), kRankInner ? 1u : 0u, 0);
         uint32_t at = step;
-        bool all = true;
-        for (int kb = kb0; kb < kb1; ++kb, ++at) {
+        for (int i = 0; i < steps; ++i, ++at) {
           const uint32_t s = at % kStages;
-          if (!wait_bounded(full + 8u * s, (at / kStages) & 1u, ctx, kStatusTimeoutMma)) {
-            all = false;
-            break;
-          }
+          if (!wait_bounded(full + 8u * s, (at / kStages) & 1u, ctx, kStatusTimeoutMma)) break;
           tc_fence_after_sync();
           if (issuer) {
             const uint64_t dp = make_smem_desc_sw128(smem_p + s * Cfg::kPBytes);
             if constexpr (!kRankInner) {
               const uint64_t dw = make_smem_desc_sw128(smem_w + s * Cfg::kWBytes);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * k, idesc, kb > kb0 || k > 0);
+              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * k, idesc, i > 0 || k > 0);
             } else {
               for (int j = 0; j < n_slots; ++j) {
                 const uint64_t dw = make_smem_desc_sw128_mn(smem_w + s * Cfg::kWBytes + j * slot_cols * 128, 8192);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  umma_f16<1>(tmem + j * slot_cols, dp + 2u * k, dw + 128u * k, idesc, kb > kb0 || k > 0);
+                  umma_f16<1>(tmem + j * slot_cols, dp + 2u * k, dw + 128u * k, idesc, i > 0 || k > 0);
               }
             }
             umma_commit<1>(empty + 8u * s);
-            if (kb == kb1 - 1) umma_commit<1>(done);
+            if (i == steps - 1) umma_commit<1>(done);
           }
           __syncwarp();
         }
-        (void)all;
       } else {
         // Every row's own columns, into the partial rows (the idle ring: all its loads have been consumed).
         const int q = warp & 3;
         const int row = q * 32 + static_cast<int>(lane);
-        const long m = static_cast<long>(tile) * 128 + row;
-        const int mine = m < p.M ? v.row_slot[m] - slot0 : -1;
+        const int mine = row_slot[row] - slot0;
         if (wait_bounded(done, parity, ctx, kStatusTimeoutEpilogue)) {
           tc_fence_after_sync();
           const uint32_t dst = base + static_cast<uint32_t>(row * pitch) * 4u;
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
           tc_fence_before_sync();
         }
       }
-      step += static_cast<uint32_t>(kb1 - kb0);
+      step += static_cast<uint32_t>(steps);
     }
     // every CTA's partial rows are written
     __syncthreads();
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
       const int row = rank * share + i / quads, r = i % quads * 4;
       const long m = static_cast<long>(tile) * 128 + row;
       if (m >= p.M) break;
-      const int slot = v.row_slot[m];
+      const int slot = row_slot[row];
       uint16_t* out = static_cast<uint16_t*>(p.out) + m * p.ld_out + r;
       if (slot < 0) {
         if (group == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
@@ -338,12 +348,15 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
       }
       if (slot < slot0 || slot >= slot0 + n_slots || !ok) continue;
       const uint32_t src = base + static_cast<uint32_t>(row * pitch + r) * 4u;
-      float4 sum = ld_cluster_v4(map_to_cta(src, 0));
-      for (int c = 1; c < splits; ++c) {
-        const float4 x = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
-        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-      }
-      const float f = p.scales ? p.scale * p.scales[adapters[slot]] : p.scale;
+      float4 x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < splits) x[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
+      float4 sum = x[0];
+#pragma unroll
+      for (int c = 1; c < 8; ++c)
+        if (c < splits) sum.x += x[c].x, sum.y += x[c].y, sum.z += x[c].z, sum.w += x[c].w;
+      const float f = row_factor[row];
       *reinterpret_cast<uint2*>(out) =
           make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x * f), __float_as_uint(sum.y * f)),
                      pack2<kIsBf16>(__float_as_uint(sum.z * f), __float_as_uint(sum.w * f)));
@@ -565,11 +578,15 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
       if (i >= side.D) continue;
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       const uint32_t src = base + static_cast<uint32_t>(y * pitch + x) * 4u;
-      for (int c = 0; c < splits; ++c) {
-        if (block_of(c) == block_of(c + 1)) continue;     // a CTA without rows
-        const float4 t = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
-        sum.x += t.x, sum.y += t.y, sum.z += t.z, sum.w += t.w;
+      float4 t[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        t[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // (a CTA without rows has left nothing)
+        if (c < splits && block_of(c) != block_of(c + 1)) t[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
       }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum.x += t[c].x, sum.y += t[c].y, sum.z += t[c].z, sum.w += t[c].w;
       const long at = side.rank_outer ? static_cast<long>(y) * side.D + i : static_cast<long>(i) * R + x;
       *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x), __float_as_uint(sum.y)),
                                                        pack2<kIsBf16>(__float_as_uint(sum.z), __float_as_uint(sum.w)));

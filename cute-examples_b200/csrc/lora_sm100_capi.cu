@@ -96,7 +96,7 @@ struct AdapterOperands {
 template <int kCfgIndex, bool kIsBf16, bool kBIsKN>
 int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan& plan, DeviceState& st, cudaStream_t stream,
                           int* cuda_error_out) {
-  using Cfg = ConfigOf<kCfgIndex, kIsBf16>;
+  using Cfg = LoraConfig<ConfigOf<kCfgIndex, kIsBf16>>;
   auto kernel = gemm_lora_kernel<Cfg, false, kBIsKN>;
   if constexpr (!kBIsKN && has_cluster_split(kCfgIndex)) {
     if (plan.split_k) kernel = gemm_lora_kernel<Cfg, true, false>;
@@ -146,13 +146,14 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
     b_box = 64 / Cfg::kCtaGroup;
     tp.b_box_rows = b_box;
   }
+  if (p.M < Cfg::kARows) tp.a_box_rows = static_cast<int>(ceil_div(p.M, 8) * 8);
   tp.k_rotate = k_order_for(p, plan.split_k);
   if (plan.split_k) {
     tp.sk_factor = plan.split_factor;
     tp.sk_cluster = 1;
   }
   CUtensorMap map_a, map_b, map_c;
-  int rc = encode_2d(&map_a, p.A, p.dtype, p.M, p.K, p.lda, Cfg::kARows, cuda_error_out, Cfg::kKSub);
+  int rc = encode_2d(&map_a, p.A, p.dtype, p.M, p.K, p.lda, tp.a_box_rows, cuda_error_out, Cfg::kKSub);
   if (rc) return rc;
   rc = kBIsKN ? encode_2d(&map_b, p.B, p.dtype, p.K, p.N, p.ldb, 64, cuda_error_out)
               : encode_2d(&map_b, p.B, p.dtype, p.N, p.K, p.ldb, b_box, cuda_error_out, Cfg::kKSub);
@@ -163,7 +164,7 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
   std::memset(&lora, 0, sizeof(lora));
   lora.chunk = rank_chunk(o.R);
   lora.chunks = static_cast<int>(ceil_div(o.R, lora.chunk));
-  rc = encode_rows(&lora.tmap_low, o.low, p.dtype, 2, {o.R, p.M, 1}, {o.ld_low, 0}, {lora.chunk, Cfg::kARows, 1}, cuda_error_out);
+  rc = encode_rows(&lora.tmap_low, o.low, p.dtype, 2, {o.R, p.M, 1}, {o.ld_low, 0}, {lora.chunk, tp.a_box_rows, 1}, cuda_error_out);
   if (rc) return rc;
   rc = kBIsKN ? encode_rows(&lora.tmap_w, o.W, p.dtype, 3, {p.N, o.R, o.adapters}, {o.ld_w, o.stride_w}, {64, lora.chunk, 1},
                             cuda_error_out)
