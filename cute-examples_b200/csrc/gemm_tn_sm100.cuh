@@ -438,6 +438,250 @@ __device__ __forceinline__ void lora_resolve(LoraWork& w, const LoraParams& lora
   w.stages = __reduce_max_sync(0xffffffffu, stages);
 }
 
+// The producer's and the MMA issuer's loops of the adapter kernels: like the plain kernel's, but with one loop for a
+// segment's K blocks and one for its adapter stages behind them, over a ring position that runs on.  (Carried
+// as a branch inside the plain kernel's flattened loop, the adapter stages made every K block of the 256 x 256
+// pair tile wait for its issue: 8192 x 4096 x 4096 took 300 us with no row using an adapter, 176 us without the branch.)
+struct RingView {
+  uint32_t smem_a, smem_b;       // operand tiles of the stages
+  uint32_t full, empty;          // barriers, one per stage, 8 bytes apart
+  uint32_t entries;              // LoraConfig's memory
+};
+
+template <class Cfg, bool kSplitK, bool kBIsKN>
+__device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CUtensorMap& tmap_b, const TileParams& p,
+                                             const LoraParams& lora, const RingView& ring, const WaitCtx& ctx,
+                                             WorkIter<kSplitK> work, uint32_t pair_base, uint32_t cta_rank) {
+  constexpr int G = Cfg::kCtaGroup;
+  const bool issuer = elect_one(), is_leader = cta_rank == 0;
+  const uint32_t lane = lane_id();
+  const uint64_t pol = policy_evict_normal();
+  const uint32_t full_leader = (G == 2) ? map_to_cta(ring.full, pair_base) : ring.full;
+  const int num_tiles = p.m_tiles * p.n_tiles, k_blocks = p.k_blocks, b_box = p.b_box_rows, a_rows = p.a_box_rows;
+  const int chunk = lora.chunk, chunks = lora.chunks;
+  uint32_t s = 0, phase = 0;
+  int tiles_done = 0;
+  bool low_ready = false;
+  Segment seg;
+  while (work.next(seg)) {
+    int m_tile, n_tile;
+    tile_coords(seg.tile, p, m_tile, n_tile);
+    const int row_a = (m_tile * G + (int)cta_rank) * Cfg::kBlockM;
+    const TileCols tc = tile_columns<Cfg>(n_tile, p);
+    const int rows_b[2] = {tc.w0 / G, tc.w1 / G};
+    const int row_b[2] = {tc.col0 + (int)cta_rank * rows_b[0], tc.col0 + tc.w0 + (int)cta_rank * rows_b[1]};
+    const uint32_t tx_bytes = (uint32_t)((a_rows + rows_b[0] + rows_b[1]) * Cfg::kBlockK * 2) * G;
+    const int rot = p.k_rotate == 1 ? (int)(((long long)seg.tile * k_blocks) / num_tiles) : 0;
+    const bool backwards = !kSplitK && p.k_rotate == 2 && (tiles_done & 1);
+    ++tiles_done;
+    LoraWork lw = lora_begin<Cfg>(lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? p.sk_factor : 1, ring.entries);
+    {
+      const int slot = lw.slot_of((int)lane, chunks);
+      if (slot < 256) cp_async_4(ring.entries + 16u + lane * 4u, lora.slot_adapter + lw.base + slot);
+    }
+#pragma unroll 1
+    for (int kb = seg.kb0; kb < seg.kb1; ++kb) {
+      if (!wait_bounded(ring.empty + 8u * s, phase ^ 1u, ctx, kStatusTimeoutProducer + s)) return;
+      int kb_phys = kb + rot;
+      if (kb_phys >= k_blocks) kb_phys -= k_blocks;
+      if (backwards) kb_phys = k_blocks - 1 - kb;
+      const int x = kb_phys * Cfg::kBlockK;
+      if (issuer) {
+        const uint32_t full = full_leader + 8u * s, dst_a = ring.smem_a + s * Cfg::kABytes, dst_b = ring.smem_b + s * Cfg::kBBytes;
+        if (is_leader) mbar_arrive_expect_tx(ring.full + 8u * s, tx_bytes);
+        if constexpr (Cfg::kKSub > 1) tma_load_3d<G>(dst_a, &tmap_a, full, 0, row_a, kb_phys * Cfg::kKSub, pol);
+        else tma_load_2d<G>(dst_a, &tmap_a, full, x, row_a, pol);
+#pragma unroll
+        for (int h = 0; h < Cfg::kHalves; ++h) {
+          if constexpr (Cfg::kKSub > 1) {
+            tma_load_3d<G>(dst_b + h * Cfg::kBHalfBytes, &tmap_b, full, 0, row_b[h], kb_phys * Cfg::kKSub, pol);
+          } else if constexpr (!kBIsKN) {
+#pragma unroll 1
+            for (int j = 0; j < rows_b[h]; j += b_box)
+              tma_load_2d<G>(dst_b + h * Cfg::kBHalfBytes + j * (Cfg::kBlockK * 2), &tmap_b, full, x, row_b[h] + j, pol);
+          } else {
+#pragma unroll
+            for (int j = 0; j < Cfg::kBRows / 64; ++j)
+              tma_load_2d<G>(dst_b + h * Cfg::kBHalfBytes + j * 8192, &tmap_b, full, row_b[h] + j * 64, x, pol);
+          }
+        }
+      }
+      if (++s == Cfg::kStages) s = 0, phase ^= 1u;
+    }
+    lora_resolve(lw, lora, ring.entries);
+    int entry_adapter;                                   // lane i: adapter of entry i of the current 32
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(entry_adapter) : "r"(ring.entries + 16u + lane * 4u) : "memory");
+    if (lw.stages > 0 && !low_ready) {
+      grid_dependency_wait();
+      low_ready = true;
+    }
+#pragma unroll 1
+    for (int stage = 0; stage < lw.stages; ++stage) {
+      const int first = (lw.part + stage * lw.factor) * lw.per_stage, entry = stage * lw.per_stage;
+      const int items = min(lw.per_stage, lw.items - first);
+      if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
+        const int slot = lw.slot_of(entry + (int)lane, chunks);
+        entry_adapter = slot < 256 ? lora.slot_adapter[lw.base + slot] : 0;
+      }
+      if (!wait_bounded(ring.empty + 8u * s, phase ^ 1u, ctx, kStatusTimeoutProducer + s)) return;
+      const uint32_t full = full_leader + 8u * s, dst_a = ring.smem_a + s * Cfg::kABytes, dst_b = ring.smem_b + s * Cfg::kBBytes;
+      if (issuer && is_leader)
+        mbar_arrive_expect_tx(ring.full + 8u * s, (uint32_t)(G * chunk * 2 * ((chunks == 1 ? 1 : items) * a_rows +
+                                                                             items * (rows_b[0] + rows_b[1]))));
+#pragma unroll 1
+      for (int i = 0; i < items; ++i) {
+        const int g = __shfl_sync(0xffffffffu, entry_adapter, (entry + i) % kLoraEntries);
+        const int r = (chunks == 1 ? 0 : (first + i) % chunks) * chunk;
+        if (issuer) {
+          // slots of one chunk share the tile of low rows
+          if (i == 0 || chunks > 1)
+            tma_load_2d<G>(dst_a + (uint32_t)(i * Cfg::kARows * chunk * 2), &lora.tmap_low, full, r, row_a, pol);
+#pragma unroll
+          for (int h = 0; h < Cfg::kHalves; ++h) {
+            const uint32_t dst = dst_b + h * Cfg::kBHalfBytes + (uint32_t)(i * Cfg::kBRows * chunk * 2);
+            if constexpr (!kBIsKN) {
+#pragma unroll 1
+              for (int j = 0; j < rows_b[h]; j += b_box)
+                tma_load_3d<G>(dst + (uint32_t)(j * chunk * 2), &lora.tmap_w, full, r, row_b[h] + j, g, pol);
+            } else {
+#pragma unroll
+              for (int j = 0; j < Cfg::kBRows / 64; ++j)
+                tma_load_3d<G>(dst + (uint32_t)(j * chunk * 128), &lora.tmap_w, full, row_b[h] + j * 64, r, g, pol);
+            }
+          }
+        }
+      }
+      if (++s == Cfg::kStages) s = 0, phase ^= 1u;
+    }
+  }
+}
+
+template <class Cfg, bool kSplitK, bool kBIsKN>
+__device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams& lora, const RingView& ring, const WaitCtx& ctx,
+                                           WorkIter<kSplitK> work, uint32_t pair_base, uint32_t tfull, uint32_t tempty,
+                                           uint32_t tmem_base) {
+  constexpr int G = Cfg::kCtaGroup;
+  const bool issuer = elect_one();
+  const uint32_t lane = lane_id();
+  constexpr uint32_t idesc_base = make_idesc_f16(Cfg::kIsBf16 ? 1u : 0u, Cfg::kBlockM * G, 0, kBIsKN ? 1u : 0u, 0);
+  const uint64_t da0 = make_smem_desc_sw128(ring.smem_a);
+  const uint64_t db0 = kBIsKN ? make_smem_desc_sw128_mn(ring.smem_b, 8192) : make_smem_desc_sw128(ring.smem_b);
+  constexpr uint32_t kBStepK = kBIsKN ? 128u : 2u;
+  const uint32_t peer = (G == 2) ? pair_base + 1u : 0u;
+  const uint32_t empty_peer = (G == 2) ? map_to_cta(ring.empty, peer) : 0u, tfull_peer = (G == 2) ? map_to_cta(tfull, peer) : 0u;
+  const uint32_t a_sub = (uint32_t)p.a_box_rows * 8u;       // 16-byte units between a stage's K blocks of A
+  constexpr uint32_t kBSub = (uint32_t)(Cfg::kBHalfBytes / Cfg::kKSub) >> 4;
+  const int chunk = lora.chunk, chunks = lora.chunks;
+  const uint64_t dl0 = make_smem_desc_rows(ring.smem_a, (uint32_t)chunk * 2u);
+  const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(ring.smem_b, (uint32_t)chunk * 128u)
+                              : make_smem_desc_rows(ring.smem_b, (uint32_t)chunk * 2u);
+  const uint32_t count_smem = ring.entries + 160u, mask_smem = ring.entries + 256u;
+  uint32_t s = 0, phase = 0;
+  int iter = 0;
+  Segment seg;
+  for (; work.next(seg); ++iter) {
+    int m_tile, n_tile;
+    tile_coords(seg.tile, p, m_tile, n_tile);
+    const TileCols tc = tile_columns<Cfg>(n_tile, p);
+    const uint32_t idesc[2] = {idesc_base | ((uint32_t)(tc.w0 >> 3) << 17), idesc_base | ((uint32_t)(tc.w1 >> 3) << 17)};
+    LoraWork lw = lora_begin<Cfg>(lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? p.sk_factor : 1, count_smem);
+    // row masks: all 256 rows of the plan's tile, or this tile's half of them
+    const uint4* masks = reinterpret_cast<const uint4*>(lora.slot_mask) + 2 * (size_t)lw.base + (G == 1 ? (m_tile & 1) : 0);
+    {
+      const int slot = lw.slot_of((int)lane, chunks);
+      if (slot < 256)
+#pragma unroll
+        for (int v = 0; v < G; ++v) cp_async_16(mask_smem + (lane * G + v) * 16u, masks + 2 * slot + v, true);
+    }
+    // accumulator slots of this tile, and the parity of their hand-over barriers
+    const uint32_t slot0 = Cfg::kHalves == 1 ? (uint32_t)(iter & 1) : 0u;
+    const uint32_t slot_phase = Cfg::kHalves == 1 ? ((iter >> 1) & 1u) : (iter & 1u);
+#pragma unroll 1
+    for (int kb = seg.kb0; kb < seg.kb1; ++kb) {
+      if (!wait_bounded(ring.full + 8u * s, phase, ctx, kStatusTimeoutMma + s)) return;
+      tc_fence_after_sync();
+      const uint32_t first = kb == seg.kb0;
+#pragma unroll
+      for (int h = 0; h < Cfg::kHalves; ++h) {
+        if (first) {
+          if (!wait_bounded(tempty + 8u * (slot0 + h), slot_phase ^ 1u, ctx, kStatusTimeoutMmaAcc + slot0 + h)) return;
+          tc_fence_after_sync();
+        }
+        const uint32_t tmem_d = tmem_base + (slot0 + h) * Cfg::kSlotCols;
+        const uint64_t da = da0 + (uint64_t)((s * Cfg::kABytes) >> 4);
+        const uint64_t db = db0 + (uint64_t)((s * Cfg::kBBytes + h * Cfg::kBHalfBytes) >> 4);
+        if (issuer) {
+          umma_f16<G>(tmem_d, da, db, idesc[h], first ? 0u : 1u);
+#pragma unroll
+          for (int k = 1; k < Cfg::kBlockK / Cfg::kUmmaK; ++k)
+            umma_f16<G>(tmem_d, da + (Cfg::kKSub > 1 ? a_sub * (k >> 2) : 0u) + 2u * (k & 3), db + kBSub * (k >> 2) + kBStepK * (k & 3),
+                        idesc[h], 1u);
+        }
+      }
+      if (issuer) {
+        umma_commit<G>(ring.empty + 8u * s);
+        if constexpr (G == 2) umma_commit<G>(empty_peer + 8u * s);
+      }
+      if (++s == Cfg::kStages) s = 0, phase ^= 1u;
+    }
+    lora_resolve(lw, lora, count_smem);
+    uint4 entry_rows[G];                                 // lane i: row mask of entry i of the current 32
+#pragma unroll
+    for (int v = 0; v < G; ++v)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(entry_rows[v].x), "=r"(entry_rows[v].y), "=r"(entry_rows[v].z), "=r"(entry_rows[v].w)
+                   : "r"(mask_smem + (lane * G + v) * 16u)
+                   : "memory");
+#pragma unroll 1
+    for (int stage = 0; stage < lw.stages; ++stage) {
+      const int first = (lw.part + stage * lw.factor) * lw.per_stage, entry = stage * lw.per_stage;
+      const int items = min(lw.per_stage, lw.items - first);
+      if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
+        const int slot = lw.slot_of(entry + (int)lane, chunks);
+        if (slot < 256)
+#pragma unroll
+          for (int v = 0; v < G; ++v) entry_rows[v] = masks[2 * slot + v];
+      }
+      if (!wait_bounded(ring.full + 8u * s, phase, ctx, kStatusTimeoutMma + s)) return;
+      tc_fence_after_sync();
+      const uint64_t dls = dl0 + (uint64_t)((s * Cfg::kABytes) >> 4), dws = dw0 + (uint64_t)((s * Cfg::kBBytes) >> 4);
+#pragma unroll 1
+      for (int i = 0; i < items; ++i) {
+        uint32_t skip[4 * G];
+#pragma unroll
+        for (int v = 0; v < G; ++v) {
+          skip[4 * v] = ~__shfl_sync(0xffffffffu, entry_rows[v].x, (entry + i) % kLoraEntries);
+          skip[4 * v + 1] = ~__shfl_sync(0xffffffffu, entry_rows[v].y, (entry + i) % kLoraEntries);
+          skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, entry_rows[v].z, (entry + i) % kLoraEntries);
+          skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, entry_rows[v].w, (entry + i) % kLoraEntries);
+        }
+        const uint64_t dl = dls + (uint64_t)((chunks == 1 ? 0u : (uint32_t)(i * Cfg::kARows * chunk * 2)) >> 4);
+        const uint64_t dw = dws + (uint64_t)((uint32_t)(i * Cfg::kBRows * chunk * 2) >> 4);
+        if (issuer) {
+#pragma unroll
+          for (int h = 0; h < Cfg::kHalves; ++h)
+            for (int k = 0; k < chunk / Cfg::kUmmaK; ++k)
+              umma_f16_rows<G>(tmem_base + (slot0 + h) * Cfg::kSlotCols, dl + 2u * k,
+                               dw + (uint64_t)((h * Cfg::kBHalfBytes) >> 4) + kBStepK * k, idesc[h], skip);
+        }
+      }
+      if (issuer) {
+        umma_commit<G>(ring.empty + 8u * s);
+        if constexpr (G == 2) umma_commit<G>(empty_peer + 8u * s);
+      }
+      if (++s == Cfg::kStages) s = 0, phase ^= 1u;
+    }
+    // the tile's accumulator is complete
+    if (issuer) {
+#pragma unroll
+      for (int h = 0; h < Cfg::kHalves; ++h) {
+        umma_commit<G>(tfull + 8u * (slot0 + h));
+        if constexpr (G == 2) umma_commit<G>(tfull_peer + 8u * (slot0 + h));
+      }
+    }
+  }
+}
+
 template <bool kIsBf16>
 __device__ __forceinline__ uint32_t pack2(uint32_t lo_bits, uint32_t hi_bits) {
   const float lo = __uint_as_float(lo_bits), hi = __uint_as_float(hi_bits);
@@ -470,6 +714,7 @@ template <class Cfg, bool kDebug, bool kSplitK, bool kBIsKN = false, bool kAIsKM
 __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CUtensorMap& tmap_b,
                                              const CUtensorMap* tmap_c, const int num_c, const TileParams& p,
                                              const LoraParams* lora = nullptr) {
+
   constexpr int G = Cfg::kCtaGroup;
   constexpr int kStages = Cfg::kStages;
   static_assert(!kBIsKN || Cfg::kBRows % 64 == 0, "B[K,N] tiles are loaded in blocks of 64 columns");
@@ -505,8 +750,6 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
   constexpr uint32_t kRxReadyOff = Cfg::kBarrierBytes - 16, kRxDoneOff = Cfg::kBarrierBytes - 8;
   static_assert(8 * (2 * kStages + 5) + 8 <= Cfg::kBarrierBytes - 16, "barrier block too small");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 8 * (2 * kStages + 5));
-  // adapter kernels: where the plan's entries land (producer: count, adapters; MMA issuer: count, row masks)
-  [[maybe_unused]] const uint32_t lora_smem = bar_base + Cfg::kBarrierBytes;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -642,7 +885,26 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
   // low rows, and the K loop runs beside it.
   if constexpr (!kLora) grid_dependency_wait();
 
-  if (warp == 0) {
+  // adapter kernels: the ring as their loops see it, the plan's entries behind the barriers
+  [[maybe_unused]] const RingView ring = {smem_a, smem_b, bar_base + kFullOff, bar_base + kEmptyOff, bar_base + Cfg::kBarrierBytes};
+
+  if (kLora && warp == 0) {
+    if constexpr (kLora)
+      lora_produce<Cfg, kSplitK, kBIsKN>(tmap_a, tmap_b, p, *lora, ring, ctx,
+                                         WorkIter<kSplitK>(cluster_id, num_clusters, num_tiles, k_blocks, sk_factor), pair_base,
+                                         cta_rank);
+    __syncwarp();
+  } else if (kLora && warp == 1) {
+    if constexpr (kLora) {
+      bool peer_ready = true;
+      if (G == 2 && is_leader) peer_ready = wait_bounded(bar_base + kTmemReadyOff, 0u, ctx, kStatusTimeoutMmaAcc + 0xf);
+      if (is_leader && peer_ready)
+        lora_issue<Cfg, kSplitK, kBIsKN>(p, *lora, ring, ctx,
+                                         WorkIter<kSplitK>(cluster_id, num_clusters, num_tiles, k_blocks, sk_factor), pair_base,
+                                         bar_base + kTFullOff, bar_base + kTEmptyOff, tmem_base);
+    }
+    __syncwarp();
+  } else if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     // The whole warp runs the loop, one elected lane issues.  The loop is flattened over
     // (tile, k-block) and unrolled over the ring so that every barrier and shared-memory
@@ -663,11 +925,6 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       const int b_box = p.b_box_rows;
       bool seg_start = true, backwards = false;
       bool ok = true;
-      [[maybe_unused]] LoraWork lw = {};
-      [[maybe_unused]] int entry_adapter = 0;             // lane i: adapter of entry i of the current 32
-      [[maybe_unused]] bool low_ready = false;
-      const int a_rows = kLora ? p.a_box_rows : Cfg::kARows;
-      int seg_end = seg.kb1;                              // the segment's K blocks, then its adapter stages
       long long stall = 0;
       while (have && ok) {
 #pragma unroll
@@ -682,17 +939,11 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
             rows_b[1] = tc.w1 / G;
             row_b[0] = tc.col0 + (int)cta_rank * rows_b[0];
             row_b[1] = tc.col0 + tc.w0 + (int)cta_rank * rows_b[1];
-            tx_bytes = (uint32_t)(a_rows * Cfg::kBlockK * 2 + (rows_b[0] + rows_b[1]) * Cfg::kBlockK * 2) * G;
+            tx_bytes = (uint32_t)(Cfg::kABytes + (rows_b[0] + rows_b[1]) * Cfg::kBlockK * 2) * G;
             rot = p.k_rotate == 1 ? (int)(((long long)seg.tile * k_blocks) / num_tiles) : 0;
             backwards = !kSplitK && p.k_rotate == 2 && (tiles_done & 1);
             ++tiles_done;
             seg_start = false;
-            seg_end = seg.kb1;
-            if constexpr (kLora) {
-              lw = lora_begin<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 1, lora_smem);
-              const int slot = lw.slot_of((int)lane, lora->chunks);
-              if (slot < 256) cp_async_4(lora_smem + 16u + lane * 4u, lora->slot_adapter + lw.base + slot);
-            }
           }
           long long t0 = 0;
           if constexpr (kDebug) t0 = trace ? clock64() : 0;
@@ -702,57 +953,6 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
           }
           if constexpr (kDebug)
             if (trace) stall += clock64() - t0;
-          if constexpr (kLora) {
-            if (kb >= seg.kb1) {
-              if (!low_ready) {
-                grid_dependency_wait();
-                low_ready = true;
-              }
-              const int chunk = lora->chunk, chunks = lora->chunks;
-              const int stage = kb - seg.kb1, first = (lw.part + stage * lw.factor) * lw.per_stage;
-              const int items = min(lw.per_stage, lw.items - first);
-              const int entry = stage * lw.per_stage;
-              if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
-                const int slot = lw.slot_of(entry + (int)lane, chunks);
-                entry_adapter = slot < 256 ? lora->slot_adapter[lw.base + slot] : 0;
-              }
-              const uint32_t low_stride = (uint32_t)(Cfg::kARows * chunk * 2);
-              const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);     // one item's tile of W per half
-              if (issuer && is_leader)
-                mbar_arrive_expect_tx(bar_base + kFullOff + 8u * s,
-                                      (uint32_t)(G * chunk * 2 *
-                                                 ((chunks == 1 ? 1 : items) * a_rows + items * (rows_b[0] + rows_b[1]))));
-              const uint32_t full = full_leader + 8u * s;
-              for (int i = 0; i < items; ++i) {
-                const int g = __shfl_sync(0xffffffffu, entry_adapter, (entry + i) % kLoraEntries);
-                const int r = (chunks == 1 ? 0 : (first + i) % chunks) * chunk;
-                if (issuer) {
-                  // slots of one chunk share the tile of low rows
-                  if (i == 0 || chunks > 1)
-                    tma_load_2d<G>(smem_a + s * Cfg::kABytes + (uint32_t)i * low_stride, &lora->tmap_low, full, r, row_a, pol);
-#pragma unroll
-                  for (int h = 0; h < Cfg::kHalves; ++h) {
-                    const uint32_t dst = smem_b + s * Cfg::kBBytes + h * Cfg::kBHalfBytes + (uint32_t)i * w_bytes;
-                    if constexpr (!kBIsKN) {
-#pragma unroll 1
-                      for (int j = 0; j < rows_b[h]; j += b_box)
-                        tma_load_3d<G>(dst + (uint32_t)(j * chunk * 2), &lora->tmap_w, full, r, row_b[h] + j, g, pol);
-                    } else {
-#pragma unroll
-                      for (int j = 0; j < Cfg::kBRows / 64; ++j)
-                        tma_load_3d<G>(dst + (uint32_t)(j * chunk * 128), &lora->tmap_w, full, row_b[h] + j * 64, r, g, pol);
-                    }
-                  }
-                }
-              }
-              if (++kb == seg_end) {
-                have = work.next(seg);
-                kb = seg.kb0;
-                seg_start = true;
-              }
-              continue;
-            }
-          }
           int kb_phys = kb + rot;                  // which K block this step loads (order is free)
           if (kb_phys >= k_blocks) kb_phys -= k_blocks;
           if (backwards) kb_phys = k_blocks - 1 - kb;
@@ -792,13 +992,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               }
             }
           }
-          if (++kb == seg_end) {
-            if constexpr (kLora) {
-              lora_resolve(lw, *lora, lora_smem);
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(entry_adapter) : "r"(lora_smem + 16u + lane * 4u) : "memory");
-              seg_end += lw.stages;
-              if (lw.stages > 0) continue;
-            }
+          if (++kb == seg.kb1) {
             have = work.next(seg);
             kb = seg.kb0;
             seg_start = true;
@@ -839,38 +1033,12 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
       bool have = work.next(seg);
       int kb = seg.kb0, iter = 0;          // iter counts segments: it selects the accumulator slot
       bool ok = peer_ready;
-      [[maybe_unused]] LoraWork lw = {};
-      [[maybe_unused]] uint4 entry_rows[G];                // lane i: row mask of entry i of the current 32
-      [[maybe_unused]] int half = 0;                       // which 128 rows of the plan's 256-row tile (single-CTA tiles)
-      [[maybe_unused]] const uint32_t count_smem = lora_smem + 160u, mask_smem = lora_smem + 256u;
-      const int a_rows = kLora ? p.a_box_rows : Cfg::kARows;
-      int seg_end = seg.kb1;
       long long stall_full = 0, stall_acc = 0;
       const bool skip_mma = kDebug && (dbg & kDebugSkipMma);
       while (have && ok) {
 #pragma unroll
         for (int s = 0; s < kStages; ++s) {
           if (!have) break;
-          const bool first_kb = kb == seg.kb0;
-          if (first_kb) {
-            int m_tile, n_tile;
-            tile_coords(seg.tile, p, m_tile, n_tile);
-            const TileCols tc = tile_columns<Cfg>(n_tile, p);
-            idesc_h[0] = idesc_base | ((uint32_t)(tc.w0 >> 3) << 17);
-            idesc_h[1] = idesc_base | ((uint32_t)(tc.w1 >> 3) << 17);
-            seg_end = seg.kb1;
-            if constexpr (kLora) {
-              lw = lora_begin<Cfg>(*lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? sk_factor : 1, count_smem);
-              half = m_tile & 1;
-              const int slot = lw.slot_of((int)lane, lora->chunks);
-              if (slot < 256) {
-                const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask) + 2 * (size_t)(lw.base + slot);
-#pragma unroll
-                for (int v = 0; v < G; ++v)
-                  cp_async_16(mask_smem + (lane * G + v) * 16u, masks + (G == 1 ? half : v), true);
-              }
-            }
-          }
           long long tf = 0;
           if constexpr (kDebug) tf = trace ? clock64() : 0;
           if (!(kDebug && (dbg & kDebugSkipLoads)) &&
@@ -888,80 +1056,14 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               }
             }
           tc_fence_after_sync();
-          if constexpr (kLora) {
-            if (kb == seg.kb1 - 1) {
-              lora_resolve(lw, *lora, count_smem);
-#pragma unroll
-              for (int v = 0; v < G; ++v)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(entry_rows[v].x), "=r"(entry_rows[v].y), "=r"(entry_rows[v].z), "=r"(entry_rows[v].w)
-                             : "r"(mask_smem + (lane * G + v) * 16u)
-                             : "memory");
-              seg_end += lw.stages;
-            }
-          }
-          const bool last_kb = kb == seg_end - 1;
-          if constexpr (kLora) {
-            if (kb >= seg.kb1) {
-              const int chunk = lora->chunk, chunks = lora->chunks;
-              const int stage = kb - seg.kb1, first = (lw.part + stage * lw.factor) * lw.per_stage;
-              const int items = min(lw.per_stage, lw.items - first);
-              const int entry = stage * lw.per_stage;
-              if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
-                const int slot = lw.slot_of(entry + (int)lane, chunks);
-                if (slot < 256) {
-                  const uint4* masks = reinterpret_cast<const uint4*>(lora->slot_mask) + 2 * (size_t)(lw.base + slot);
-#pragma unroll
-                  for (int v = 0; v < G; ++v) entry_rows[v] = masks[G == 1 ? half : v];
-                }
-              }
-              const uint32_t low_stride = (uint32_t)(Cfg::kARows * chunk * 2);
-              const uint32_t w_bytes = (uint32_t)(Cfg::kBRows * chunk * 2);
-              const uint64_t dl0 = make_smem_desc_rows(smem_a + s * Cfg::kABytes, (uint32_t)chunk * 2u);
-              const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(smem_b + s * Cfg::kBBytes, (uint32_t)chunk * 128u)
-                                          : make_smem_desc_rows(smem_b + s * Cfg::kBBytes, (uint32_t)chunk * 2u);
-              constexpr uint32_t kWStepK = kBIsKN ? 128u : 2u;
-#pragma unroll 1
-              for (int i = 0; i < items; ++i) {
-                uint32_t skip[4 * G];
-#pragma unroll
-                for (int v = 0; v < G; ++v) {
-                  skip[4 * v] = ~__shfl_sync(0xffffffffu, entry_rows[v].x, (entry + i) % kLoraEntries);
-                  skip[4 * v + 1] = ~__shfl_sync(0xffffffffu, entry_rows[v].y, (entry + i) % kLoraEntries);
-                  skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, entry_rows[v].z, (entry + i) % kLoraEntries);
-                  skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, entry_rows[v].w, (entry + i) % kLoraEntries);
-                }
-                const uint64_t dl = dl0 + (uint64_t)((chunks == 1 ? 0u : (uint32_t)i * low_stride) >> 4);
-                const uint64_t dw = dw0 + (uint64_t)(((uint32_t)i * w_bytes) >> 4);
-                if (issuer) {
-#pragma unroll
-                  for (int h = 0; h < Cfg::kHalves; ++h) {
-                    const int slot = Cfg::kHalves == 1 ? (iter & 1) : h;
-                    for (int k = 0; k < chunk / Cfg::kUmmaK; ++k)
-                      umma_f16_rows<G>(tmem_base + slot * Cfg::kSlotCols, dl + 2u * k,
-                                       dw + (uint64_t)((h * Cfg::kBHalfBytes) >> 4) + kWStepK * k, idesc_h[h], skip);
-                  }
-                }
-              }
-              if (issuer) {
-                if (last_kb) {
-#pragma unroll
-                  for (int h = 0; h < Cfg::kHalves; ++h) {
-                    const int slot = Cfg::kHalves == 1 ? (iter & 1) : h;
-                    umma_commit<G>(bar_base + kTFullOff + 8u * slot);
-                    if constexpr (G == 2) umma_commit<G>(bar_peer + kTFullOff + 8u * slot);
-                  }
-                }
-                umma_commit<G>(bar_base + kEmptyOff + 8u * s);
-                if constexpr (G == 2) umma_commit<G>(bar_peer + kEmptyOff + 8u * s);
-              }
-              if (++kb == seg_end) {
-                have = work.next(seg);
-                kb = seg.kb0;
-                ++iter;
-              }
-              continue;
-            }
+          const bool first_kb = kb == seg.kb0;
+          const bool last_kb = kb == seg.kb1 - 1;
+          if (first_kb) {
+            int m_tile, n_tile;
+            tile_coords(seg.tile, p, m_tile, n_tile);
+            const TileCols tc = tile_columns<Cfg>(n_tile, p);
+            idesc_h[0] = idesc_base | ((uint32_t)(tc.w0 >> 3) << 17);
+            idesc_h[1] = idesc_base | ((uint32_t)(tc.w1 >> 3) << 17);
           }
 #pragma unroll
           for (int h = 0; h < Cfg::kHalves; ++h) {
@@ -992,7 +1094,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
                 for (int k = 1; k < Cfg::kBlockK / Cfg::kUmmaK; ++k) {
                   // four steps inside a 64-element K block, then on to the stage's next K block (its own
                   // K-major tile, right behind the first)
-                  const uint32_t kASub = kLora ? (uint32_t)a_rows * 8u : (uint32_t)(Cfg::kABytes / Cfg::kKSub) >> 4;
+                  constexpr uint32_t kASub = (uint32_t)(Cfg::kABytes / Cfg::kKSub) >> 4;
                   constexpr uint32_t kBSub = (uint32_t)(Cfg::kBHalfBytes / Cfg::kKSub) >> 4;
                   umma_f16<G>(tmem_d, da + kASub * (k >> 2) + kAStepK * (k & 3), db + kBSub * (k >> 2) + kBStepK * (k & 3),
                               idesc_h[h], 1u);
@@ -1019,7 +1121,7 @@ __device__ __forceinline__ void gemm_tn_body(const CUtensorMap& tmap_a, const CU
               if constexpr (G == 2) umma_commit<G>(bar_peer + kEmptyOff + 8u * s);
             }
           }
-          if (++kb == seg_end) {
+          if (++kb == seg.kb1) {
             have = work.next(seg);
             kb = seg.kb0;
             ++iter;
