@@ -386,8 +386,11 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
 // rows are contracted: P and Q go to the tensor core as they lie in memory, as MN-major operands.  The rows of
 // an adapter may be anywhere in the batch, so threads gather them (plan order) with 16-byte asynchronous
 // copies into the swizzled tiles; places behind the last row are filled with zeros in both operands and read
-// nothing.  One read of P bounds it.  The rows are cut over the CTAs of a cluster, which add their
-// partial sums through distributed shared memory in rank order.
+// nothing.  One read of P bounds it.
+// Work: a column tile of one adapter, whose rows are cut over `splits` CTAs of a cluster of eight (1, 2, 4 or 8: the
+// fewest with at most `split_rows` rows each), which add their partial sums through distributed shared
+// memory in rank order.  The cluster takes 8 / splits neighbouring tiles at once, and a grid that fills the
+// device walks over all adapters' groups of tiles.
 struct GradSide {
   const uint16_t* P;
   const uint16_t* Q;
@@ -400,16 +403,20 @@ struct GradParams {
   GradSide side[2];
   const void* plan;
   int M, R, adapters;
-  int tiles0;            // column tiles of side 0
+  int tiles0, tiles;     // column tiles of side 0, and of both sides
+  int split_rows;
   unsigned int* status;
   unsigned long long timeout_ns;
 };
 
+constexpr int kGradCluster = 8;
 template <int kRankBlocks>   // 64-element blocks of ranks: 1 or 2
 struct GradConfig {
   static constexpr int kThreads = 160;                 // four warps gather and store, one issues
-  static constexpr int kStages = 3;
-  static constexpr int kPBytes = 2 * 64 * 128, kQBytes = kRankBlocks * 64 * 128;
+  static constexpr int kRows = 32;                     // rows per ring stage (the entries a warp fetches ahead assume 32)
+  static constexpr int kStages = 6;
+  static constexpr int kBlockBytes = kRows * 128;      // 64 columns of a stage
+  static constexpr int kPBytes = 2 * kBlockBytes, kQBytes = kRankBlocks * kBlockBytes;
   static constexpr int kStageBytes = kPBytes + kQBytes;
   static constexpr int kTmemCols = kRankBlocks * 64;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 128;
@@ -420,7 +427,7 @@ template <bool kIsBf16, int kRankBlocks>
 __global__ void __launch_bounds__(160, GradConfig<kRankBlocks>::kCtasPerSm)
 lora_grad_kernel(const __grid_constant__ GradParams p) {
   using Cfg = GradConfig<kRankBlocks>;
-  constexpr int kStages = Cfg::kStages;
+  constexpr int kStages = Cfg::kStages, kRows = Cfg::kRows;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t smem_p = base, smem_q = base + kStages * Cfg::kPBytes;
@@ -431,22 +438,13 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
   const int rank = static_cast<int>(cluster_ctarank());
-  uint32_t splits_reg;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits_reg));
-  const int splits = static_cast<int>(splits_reg);
-  const int unit = static_cast<int>(blockIdx.x) / splits;
-  // units: the column tiles of side 0 of every adapter, then those of side 1
-  const int units0 = p.tiles0 * p.adapters;
-  const GradSide& side = p.side[unit < units0 ? 0 : 1];
-  const int tiles = (side.D + 127) / 128;
-  const int local = unit < units0 ? unit : unit - units0;
-  const int g = local / tiles, col0 = (local - g * tiles) * 128;
+  const int cluster = static_cast<int>(blockIdx.x) / kGradCluster, clusters = static_cast<int>(gridDim.x) / kGradCluster;
   WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int b = 0; b < kStages; ++b) {
-      mbar_init(full + 8u * b, 4);
+      mbar_init(full + 8u * b, 128);
       mbar_init(empty + 8u * b, 1);
     }
     mbar_init(done, 1);
@@ -464,136 +462,174 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
   grid_dependency_wait();
 
   const LoraPlanView v = lora_plan_view(const_cast<void*>(p.plan), p.M);
-  const int first = v.offsets[g], last = v.offsets[g + 1];
-  const int blocks = (last - first + 63) / 64;           // of 64 rows
-  auto block_of = [&](int c) { return static_cast<int>(static_cast<long>(blocks) * c / splits); };
-  const int b0 = block_of(rank), b1 = block_of(rank + 1);
   const int R = p.R;
-  const int pitch = side.rank_outer ? 128 + 4 : R + 4;   // floats per row of the partial sums: [r][i] or [i][r]
-  if (b1 > b0) {
-    if (warp < 4) {
-      // Thread: 16-byte piece `piece` of the rows tid / 16 + 8 k of every block, and the same piece of Q
-      // where Q has it; two 64-column blocks of P, 128-byte swizzle.
-      const int tid = threadIdx.x, piece = tid & 15, r0 = tid >> 4;
-      const bool col_ok = col0 + piece * 8 < side.D, q_ok = piece * 8 < R;
-      const uint16_t* src_p = side.P + (col_ok ? col0 + piece * 8 : 0);
-      const uint16_t* src_q = side.Q + (q_ok ? piece * 8 : 0);
-      // row t of a block sits at t * 128, its piece c at c ^ (t % 8); t % 8 == r0 for all of this thread's rows
-      const uint32_t place = static_cast<uint32_t>((piece >> 3) * 8192 + r0 * 128 + (((piece & 7) ^ r0) << 4));
-      int row[8];
-      auto fetch_rows = [&](int b) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int at = first + b * 64 + r0 + 8 * k;
-          row[k] = b < b1 && at < last ? v.order[at] : -1;
-        }
-      };
-      fetch_rows(b0);
-      bool good = true;
-      int n = 0;
-      for (int b = b0; b < b1; ++b, ++n) {
-        const uint32_t s = static_cast<uint32_t>(n) % kStages;
-        if (!wait_bounded(empty + 8u * s, ((static_cast<uint32_t>(n) / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) {
-          good = false;
-          break;
-        }
-        const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const bool live = row[k] >= 0;
-          const long m = live ? row[k] : 0;
-          cp_async_16(dst_p + k * 1024u, src_p + m * side.ldp, live && col_ok);
-          if (q_ok) cp_async_16(dst_q + k * 1024u, src_q + m * side.ldq, live);
-        }
-        cp_async_commit();
-        fetch_rows(b + 1);
-        if (n >= kStages - 1) {
-          // the oldest stage in flight has landed: hand it to the tensor core
-          cp_async_wait<kStages - 1>();
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + 8u * ((static_cast<uint32_t>(n) + 1u) % kStages));
-        }
-      }
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (good && lane == 0)
-        for (int t = n >= kStages - 1 ? n - (kStages - 1) : 0; t < n; ++t) mbar_arrive(full + 8u * (static_cast<uint32_t>(t) % kStages));
-    } else {
-      const bool issuer = elect_one();
-      const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>((R + 15) / 16 * 16), 1u, 1u);
-      for (int b = b0, n = 0; b < b1; ++b, ++n) {
-        const uint32_t s = static_cast<uint32_t>(n) % kStages;
-        if (!wait_bounded(full + 8u * s, (static_cast<uint32_t>(n) / kStages) & 1u, ctx, kStatusTimeoutMma)) break;
-        tc_fence_after_sync();
-        if (issuer) {
-          const uint64_t dp = make_smem_desc_sw128_mn(smem_p + s * Cfg::kPBytes, 8192);
-          const uint64_t dq = make_smem_desc_sw128_mn(smem_q + s * Cfg::kQBytes, 8192);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 128u * k, dq + 128u * k, idesc, n > 0 || k > 0);
-          umma_commit<1>(empty + 8u * s);
-          if (b == b1 - 1) umma_commit<1>(done);
-        }
-        __syncwarp();
-      }
+  uint32_t n = 0;                                        // ring position, running on over the units
+  uint32_t rounds = 0;                                   // uses of the accumulator so far
+  // The adapters' groups of tiles, one adapter after another, are the units of the grid; clusters take them in
+  // turn.  Every warp finds its units by itself, 32 adapters at a time.
+  int u = cluster, batch_start = 0;
+#pragma unroll 1
+  for (int g0 = 0; g0 < p.adapters; g0 += 32) {
+    int my_first = 0, my_last = 0, my_splits = 1, my_end = 0;
+    if (g0 + static_cast<int>(lane) < p.adapters) {
+      my_first = v.offsets[g0 + lane];
+      my_last = v.offsets[g0 + lane + 1];
+      while (my_splits < kGradCluster && my_last - my_first > p.split_rows * my_splits) my_splits *= 2;
+      my_end = (p.tiles * my_splits + kGradCluster - 1) / kGradCluster;
     }
-    if (warp < 4) {
-      if (wait_bounded(done, 0, ctx, kStatusTimeoutEpilogue)) {
-        // the partial sums, into the idle ring
-        tc_fence_after_sync();
-        const int i = warp * 32 + static_cast<int>(lane);
-        for (int r = 0; r < R; r += 8) {
-          uint32_t x[8];
-          tmem_ld_32x8(tmem + (static_cast<uint32_t>(warp * 32) << 16) + r, x);
-          tmem_ld_wait();
-          if (side.rank_outer) {
+    for (int o = 1; o < 32; o *= 2) {
+      const int below = __shfl_up_sync(0xffffffffu, my_end, o);
+      if (static_cast<int>(lane) >= o) my_end += below;
+    }
+    my_end += batch_start;                               // where this lane's adapter ends in the grid's units
+    const int batch_end = __shfl_sync(0xffffffffu, my_end, 31);
+#pragma unroll 1
+    for (; u < batch_end; u += clusters) {
+      const int owner = __popc(__ballot_sync(0xffffffffu, my_end <= u));
+      const int g = g0 + owner;
+      const int first = __shfl_sync(0xffffffffu, my_first, owner), last = __shfl_sync(0xffffffffu, my_last, owner);
+      const int splits = __shfl_sync(0xffffffffu, my_splits, owner), group_tiles = kGradCluster / splits;
+      const int start_of = __shfl_sync(0xffffffffu, my_end, owner > 0 ? owner - 1 : 0);
+      const int start = owner > 0 ? start_of : batch_start;
+      const int tile = (u - start) * group_tiles + rank / splits, part = rank % splits;
+      const bool work = tile < p.tiles && *abort_flag == 0;
+      const GradSide& side = p.side[tile < p.tiles0 ? 0 : 1];
+      const int col0 = (tile < p.tiles0 ? tile : tile - p.tiles0) * 128;
+      const int blocks = (last - first + kRows - 1) / kRows;
+      const int shift = __popc(splits - 1);
+      auto block_of = [&](int c) { return static_cast<int>((static_cast<long>(blocks) * c) >> shift); };
+      const int b0 = block_of(part), b1 = block_of(part + 1);
+      const int pitch = side.rank_outer ? 128 + 4 : R + 4;   // floats per row of the partial sums: [r][i] or [i][r]
+      if (work && b1 > b0) {
+        if (warp < 4) {
+          // Thread: 16-byte piece `piece` of the rows tid / 16 + 8 k of every block, and the same piece of Q
+          // where Q has it; two 64-column blocks of P, 128-byte swizzle.
+          const int tid = threadIdx.x, piece = tid & 15, r0 = tid >> 4;
+          const bool col_ok = col0 + piece * 8 < side.D, q_ok = piece * 8 < R;
+          const uint16_t* src_p = side.P + (col_ok ? col0 + piece * 8 : 0);
+          const uint16_t* src_q = side.Q + (q_ok ? piece * 8 : 0);
+          const long ldp = side.ldp, ldq = side.ldq;
+          // row t of a block sits at t * 128, its piece c at c ^ (t % 8); t % 8 == r0 for all of this thread's rows
+          const uint32_t place = static_cast<uint32_t>((piece >> 3) * Cfg::kBlockBytes + r0 * 128 + (((piece & 7) ^ r0) << 4));
+          // The rows' places in the batch, eight per warp and block: a lane loads one of four blocks' entries, two
+          // such loads ahead of their use (fetched one block ahead, their latency was every block's time).
+          auto fetch_rows = [&](int b) {
+            const int e = static_cast<int>(lane) & 7;
+            const int block = b + (static_cast<int>(lane) >> 3), at = first + block * kRows + warp * 2 + (e >> 2) + 8 * (e & 3);
+            return block < b1 && at < last ? v.order[at] : -1;
+          };
+          int rows_now = fetch_rows(b0), rows_next = fetch_rows(b0 + 4);
+          int taken = 0;                                 // stages filled in this unit
+          for (int b = b0; b < b1; ++b, ++taken) {
+            const uint32_t at = n + static_cast<uint32_t>(taken), s = at % kStages;
+            if (!wait_bounded(empty + 8u * s, ((at / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) break;
+            const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + static_cast<uint32_t>((r + e) * pitch + i) * 4u), "r"(x[e])
-                           : "memory");
-          } else {
-            const uint32_t dst = base + static_cast<uint32_t>(i * pitch + r) * 4u;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
-                         : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 16u), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-                         : "memory");
+            for (int k = 0; k < kRows / 8; ++k) {
+              const int row = __shfl_sync(0xffffffffu, rows_now, (taken & 3) * 8 + static_cast<int>(lane >> 4) * 4 + k);
+              const bool live = row >= 0;
+              const long m = live ? row : 0;
+              cp_async_16(dst_p + k * 1024u, src_p + m * ldp, live && col_ok);
+              if (q_ok) cp_async_16(dst_q + k * 1024u, src_q + m * ldq, live);
+            }
+            cp_async_arrive(full + 8u * s);
+            if ((taken & 3) == 3) {
+              rows_now = rows_next;
+              rows_next = fetch_rows(b + 5);
+            }
+          }
+          __syncwarp();
+          if (wait_bounded(done, rounds & 1u, ctx, kStatusTimeoutEpilogue)) {
+            // the partial sums, into the idle ring
+            tc_fence_after_sync();
+            const int i = warp * 32 + static_cast<int>(lane);
+            for (int r = 0; r < R; r += 8) {
+              uint32_t x[8];
+              tmem_ld_32x8(tmem + (static_cast<uint32_t>(warp * 32) << 16) + r, x);
+              tmem_ld_wait();
+              if (side.rank_outer) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + static_cast<uint32_t>((r + e) * pitch + i) * 4u), "r"(x[e])
+                               : "memory");
+              } else {
+                const uint32_t dst = base + static_cast<uint32_t>(i * pitch + r) * 4u;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                             : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 16u), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                             : "memory");
+              }
+            }
+            tc_fence_before_sync();
+          }
+        } else {
+          const bool issuer = elect_one();
+          const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>((R + 15) / 16 * 16), 1u, 1u);
+          uint32_t at = n;
+          for (int b = b0; b < b1; ++b, ++at) {
+            const uint32_t s = at % kStages;
+            if (!wait_bounded(full + 8u * s, (at / kStages) & 1u, ctx, kStatusTimeoutMma)) break;
+            // The copies are generic-proxy writes.  The fence stands here, behind the barrier: a gathering
+            // thread's own fence would wait for every copy it has in flight.
+            fence_proxy_async_smem();
+            tc_fence_after_sync();
+            if (issuer) {
+              const uint64_t dp = make_smem_desc_sw128_mn(smem_p + s * Cfg::kPBytes, Cfg::kBlockBytes);
+              const uint64_t dq = make_smem_desc_sw128_mn(smem_q + s * Cfg::kQBytes, Cfg::kBlockBytes);
+#pragma unroll
+              for (int k = 0; k < kRows / 16; ++k) umma_f16<1>(tmem, dp + 128u * k, dq + 128u * k, idesc, b > b0 || k > 0);
+              umma_commit<1>(empty + 8u * s);
+              if (b == b1 - 1) umma_commit<1>(done);
+            }
+            __syncwarp();
           }
         }
-        tc_fence_before_sync();
+        n += static_cast<uint32_t>(b1 - b0);
+        ++rounds;
+      }
+      __syncthreads();
+      if (splits > 1) {
+        cluster_arrive();
+        cluster_wait();
+      }
+      if (work) {
+        // This CTA's share of its tile's sums, four neighbours at a time, added over the parts in rank order.
+        const int per_row = (side.rank_outer ? 128 : R) / 4, quads = 32 * R, leader = rank - part;
+        const int q0 = quads * part / splits, q1 = quads * (part + 1) / splits;
+        uint16_t* out = side.out + static_cast<long>(g) * side.D * R;
+        uint32_t live = 0;                                 // (a part without rows has left nothing)
+        for (int c = 0; c < splits; ++c) live |= block_of(c) != block_of(c + 1) ? 1u << c : 0u;
+        for (int q = q0 + static_cast<int>(threadIdx.x); q < q1; q += Cfg::kThreads) {
+          const int y = q / per_row, x = q % per_row * 4;
+          const int i = col0 + (side.rank_outer ? x : y);
+          if (i >= side.D) continue;
+          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const uint32_t src = base + static_cast<uint32_t>(y * pitch + x) * 4u;
+          float4 t[kGradCluster];
+#pragma unroll
+          for (int c = 0; c < kGradCluster; ++c) {
+            t[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if ((live >> c) & 1u)
+              t[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(leader + c)));
+          }
+#pragma unroll
+          for (int c = 0; c < kGradCluster; ++c) sum.x += t[c].x, sum.y += t[c].y, sum.z += t[c].z, sum.w += t[c].w;
+          const long at = side.rank_outer ? static_cast<long>(y) * side.D + i : static_cast<long>(i) * R + x;
+          *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x), __float_as_uint(sum.y)),
+                                                           pack2<kIsBf16>(__float_as_uint(sum.z), __float_as_uint(sum.w)));
+        }
+      }
+      // the ring goes back to the copies
+      if (splits > 1) {
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        __syncthreads();
       }
     }
+    batch_start = batch_end;
   }
-  __syncthreads();
-  cluster_arrive();
-  cluster_wait();
-  // This CTA's share of the sums, four neighbours at a time, added over the cluster in rank order.
-  {
-    const int per_row = (side.rank_outer ? 128 : R) / 4, quads = 32 * R;
-    const int q0 = quads * rank / splits, q1 = quads * (rank + 1) / splits;
-    uint16_t* out = side.out + static_cast<long>(g) * side.D * R;
-    for (int q = q0 + static_cast<int>(threadIdx.x); q < q1; q += Cfg::kThreads) {
-      const int y = q / per_row, x = q % per_row * 4;
-      const int i = col0 + (side.rank_outer ? x : y);
-      if (i >= side.D) continue;
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const uint32_t src = base + static_cast<uint32_t>(y * pitch + x) * 4u;
-      float4 t[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        t[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        // (a CTA without rows has left nothing)
-        if (c < splits && block_of(c) != block_of(c + 1)) t[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
-      }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) sum.x += t[c].x, sum.y += t[c].y, sum.z += t[c].z, sum.w += t[c].w;
-      const long at = side.rank_outer ? static_cast<long>(y) * side.D + i : static_cast<long>(i) * R + x;
-      *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x), __float_as_uint(sum.y)),
-                                                       pack2<kIsBf16>(__float_as_uint(sum.z), __float_as_uint(sum.w)));
-    }
-  }
-  cluster_arrive();
-  cluster_wait();
+
   if (*abort_flag != 0) {
 #pragma unroll 1
     for (int t = 0; t < 200; ++t) __nanosleep(1000);

@@ -310,14 +310,24 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   p.plan = a.plan;
   p.M = a.M, p.R = a.R, p.adapters = a.adapters;
   p.tiles0 = static_cast<int>(ceil_div(down.D, 128));
+  p.tiles = p.tiles0 + static_cast<int>(ceil_div(up.D, 128));
   p.status = st->status_ptr;
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
-  // The rows may all belong to one adapter: a CTA gets at most 1024 of them where a cluster can do that.
-  int splits = 8;
-  while (splits > 1 && a.M <= 512L * splits) splits /= 2;
-  const long units = (ceil_div(down.D, 128) + ceil_div(up.D, 128)) * a.adapters;
-  if (units * splits > 0x7fffffffL) return GEMM_SM100_ERR_BAD_SHAPE;
-  e = launch_cluster(kernel, units * splits, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  // How far to cut the rows: the rows may all belong to one adapter, so the cut that finishes that case first
+  // sets the number of rows a CTA takes at once; adapters with fewer rows are cut less.
+  const long clusters = static_cast<long>(st->sm_count) * Cfg::kCtasPerSm / kGradCluster;
+  int splits = 1;
+  double best = 1e300;
+  for (int c = 1; c <= kGradCluster; c *= 2) {
+    const double t = static_cast<double>(ceil_div(ceil_div(p.tiles, kGradCluster / c), clusters)) *
+                     (static_cast<double>(ceil_div(a.M, c)) + 128.0);      // (a unit costs about two blocks of rows besides)
+    if (t < best) best = t, splits = c;
+  }
+  p.split_rows = static_cast<int>(ceil_div(a.M, splits));
+  if (p.split_rows < 128) p.split_rows = 128;
+  const long most = ceil_div(p.tiles, 1) * a.adapters;
+  e = launch_cluster(kernel, (most < clusters ? most : clusters) * kGradCluster, kGradCluster, Cfg::kThreads, Cfg::kSmemBytes,
+                     stream, p);
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
