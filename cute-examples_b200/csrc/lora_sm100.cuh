@@ -387,9 +387,9 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
 // an adapter may be anywhere in the batch, so threads gather them (plan order) with 16-byte asynchronous
 // copies into the swizzled tiles; places behind the last row are filled with zeros in both operands and read
 // nothing.  One read of P bounds it.
-// Work: a column tile of one adapter, whose rows are cut over `splits` CTAs of a cluster of eight (1, 2, 4 or 8: the
+// Work: a column tile of one adapter, whose rows are cut over `splits` CTAs of a cluster of four (1, 2 or 4: the
 // fewest with at most `split_rows` rows each), which add their partial sums through distributed shared
-// memory in rank order.  The cluster takes 8 / splits neighbouring tiles at once, and a grid that fills the
+// memory in rank order.  The cluster takes 4 / splits neighbouring tiles at once, and a grid that fills the
 // device walks over all adapters' groups of tiles.
 struct GradSide {
   const uint16_t* P;
@@ -409,12 +409,12 @@ struct GradParams {
   unsigned long long timeout_ns;
 };
 
-constexpr int kGradCluster = 8;
+constexpr int kGradCluster = 4;
 template <int kRankBlocks>   // 64-element blocks of ranks: 1 or 2
 struct GradConfig {
   static constexpr int kThreads = 160;                 // four warps gather and store, one issues
-  static constexpr int kRows = 32;                     // rows per ring stage (the entries a warp fetches ahead assume 32)
-  static constexpr int kStages = 6;
+  static constexpr int kRows = 64;                     // rows per ring stage
+  static constexpr int kStages = 3;
   static constexpr int kBlockBytes = kRows * 128;      // 64 columns of a stage
   static constexpr int kPBytes = 2 * kBlockBytes, kQBytes = kRankBlocks * kBlockBytes;
   static constexpr int kStageBytes = kPBytes + kQBytes;
@@ -511,14 +511,14 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
           const long ldp = side.ldp, ldq = side.ldq;
           // row t of a block sits at t * 128, its piece c at c ^ (t % 8); t % 8 == r0 for all of this thread's rows
           const uint32_t place = static_cast<uint32_t>((piece >> 3) * Cfg::kBlockBytes + r0 * 128 + (((piece & 7) ^ r0) << 4));
-          // The rows' places in the batch, eight per warp and block: a lane loads one of four blocks' entries, two
-          // such loads ahead of their use (fetched one block ahead, their latency was every block's time).
+          // The rows' places in the batch, kRows / 4 per warp and block: a lane loads one of the next two blocks'
+          // entries, two blocks ahead of their use (one block ahead, their latency was every block's time).
           auto fetch_rows = [&](int b) {
-            const int e = static_cast<int>(lane) & 7;
-            const int block = b + (static_cast<int>(lane) >> 3), at = first + block * kRows + warp * 2 + (e >> 2) + 8 * (e & 3);
+            const int e = static_cast<int>(lane) & 15;
+            const int block = b + (static_cast<int>(lane) >> 4), at = first + block * kRows + warp * 2 + (e >> 3) + 8 * (e & 7);
             return block < b1 && at < last ? v.order[at] : -1;
           };
-          int rows_now = fetch_rows(b0), rows_next = fetch_rows(b0 + 4);
+          int rows_now = fetch_rows(b0), rows_next = fetch_rows(b0 + 2);
           int taken = 0;                                 // stages filled in this unit
           for (int b = b0; b < b1; ++b, ++taken) {
             const uint32_t at = n + static_cast<uint32_t>(taken), s = at % kStages;
@@ -526,16 +526,16 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
             const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place;
 #pragma unroll
             for (int k = 0; k < kRows / 8; ++k) {
-              const int row = __shfl_sync(0xffffffffu, rows_now, (taken & 3) * 8 + static_cast<int>(lane >> 4) * 4 + k);
+              const int row = __shfl_sync(0xffffffffu, rows_now, (taken & 1) * 16 + static_cast<int>(lane >> 4) * 8 + k);
               const bool live = row >= 0;
               const long m = live ? row : 0;
               cp_async_16(dst_p + k * 1024u, src_p + m * ldp, live && col_ok);
               if (q_ok) cp_async_16(dst_q + k * 1024u, src_q + m * ldq, live);
             }
             cp_async_arrive(full + 8u * s);
-            if ((taken & 3) == 3) {
+            if (taken & 1) {
               rows_now = rows_next;
-              rows_next = fetch_rows(b + 5);
+              rows_next = fetch_rows(b + 3);
             }
           }
           __syncwarp();
@@ -547,7 +547,22 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
               uint32_t x[8];
               tmem_ld_32x8(tmem + (static_cast<uint32_t>(warp * 32) << 16) + r, x);
               tmem_ld_wait();
-              if (side.rank_outer) {
+              if (splits == 1) {
+                // nobody to add: straight to memory
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = pack2<kIsBf16>(x[2 * e], x[2 * e + 1]);
+                uint16_t* out = side.out + static_cast<long>(g) * side.D * R;
+                if (col0 + i < side.D) {
+                  if (side.rank_outer) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                      out[static_cast<long>(r + e) * side.D + col0 + i] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+                  } else {
+                    *reinterpret_cast<uint4*>(out + static_cast<long>(col0 + i) * R + r) = make_uint4(w[0], w[1], w[2], w[3]);
+                  }
+                }
+              } else if (side.rank_outer) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + static_cast<uint32_t>((r + e) * pitch + i) * 4u), "r"(x[e])
@@ -592,7 +607,7 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
         cluster_arrive();
         cluster_wait();
       }
-      if (work) {
+      if (work && (splits > 1 || b1 == b0)) {             // (an adapter without rows: zeros)
         // This CTA's share of its tile's sums, four neighbours at a time, added over the parts in rank order.
         const int per_row = (side.rank_outer ? 128 : R) / 4, quads = 32 * R, leader = rank - part;
         const int q0 = quads * part / splits, q1 = quads * (part + 1) / splits;

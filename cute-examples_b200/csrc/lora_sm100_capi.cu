@@ -315,7 +315,9 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
   // How far to cut the rows: the rows may all belong to one adapter, so the cut that finishes that case first
   // sets the number of rows a CTA takes at once; adapters with fewer rows are cut less.
-  const long clusters = static_cast<long>(st->sm_count) * Cfg::kCtasPerSm / kGradCluster;
+  // (nine tenths of the CTAs that the SMs hold: a cluster sits inside one GPC, and what is left over there must not make
+  // a second wave)
+  const long clusters = static_cast<long>(st->sm_count) * Cfg::kCtasPerSm * 9 / (10 * kGradCluster);
   int splits = 1;
   double best = 1e300;
   for (int c = 1; c <= kGradCluster; c *= 2) {
