@@ -141,6 +141,9 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids
   }
 }
 
+// The ranks that make one swizzle row of 32, 64 or 128 bytes in shared memory.
+__host__ __device__ constexpr int rank_chunk(int R) { return R <= 16 ? 16 : (R <= 32 ? 32 : 64); }
+
 // ------------------------------------------------------------------------------ low-rank rows
 // low[m] = s_g P[m] W_g^T over the long axis L: P = A and W = down [R, L], or (kRankInner) P = dC and W = up
 // [L, R].  A tile of 128 rows is one MMA operand; the adapters of the tile's rows lie side by side along
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids
 // add their partial rows through distributed shared memory in rank order.
 struct LowParams {
   CUtensorMap tmap_p;    // [M, L]: boxes of 64 x p_rows
-  CUtensorMap tmap_w;    // [adapters, R, L]: boxes of 64 x R, or [adapters, L, R]: boxes of 64 ranks x 64
+  CUtensorMap tmap_w;    // [adapters, R, L]: boxes of 64 x R, or [adapters, L, R]: boxes of a chunk of ranks x 64
   const void* plan;
   const float* scales;
   float scale;
@@ -224,8 +227,8 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
   // The CTAs of a cluster take the K blocks in turn: what they read of a row of P at any moment is contiguous.
   const int steps = (k_blocks - rank + splits - 1) / splits;
   const int R = p.R;
-  // columns of the accumulator per adapter: the ranks, or whole 64-element blocks of them
-  const int slot_cols = kRankInner ? (R > 64 ? 128 : 64) : R;
+  // columns of the accumulator per adapter: the ranks, or whole chunks of them
+  const int chunk = rank_chunk(R), slot_cols = kRankInner ? (R + chunk - 1) / chunk * chunk : R;
   const int groups = slots == 0 ? 1 : (slots + p.group_slots - 1) / p.group_slots;   // (no slot: zeros are written)
   const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
   uint32_t step = 0;                                   // ring position, running on over the groups
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
       if (warp == 0) {
         const uint64_t pol = policy_evict_normal();
         const bool issuer = elect_one();
-        const uint32_t w_bytes = kRankInner ? static_cast<uint32_t>(slot_cols) * 128u : static_cast<uint32_t>(R) * 128u;
+        const uint32_t w_bytes = static_cast<uint32_t>(slot_cols) * 128u;
         const uint32_t bytes = static_cast<uint32_t>(p.p_rows) * 128u + n_slots * w_bytes;
         const int my_adapter = static_cast<int>(lane) < n_slots ? adapters[slot0 + lane] : 0;
         uint32_t at = step;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
               if constexpr (!kRankInner) {
                 tma_load_3d<1>(dst, &p.tmap_w, full + 8u * s, kb * 64, 0, g, pol);
               } else {
-                for (int b = 0; b * 64 < R; ++b) tma_load_3d<1>(dst + b * 8192, &p.tmap_w, full + 8u * s, b * 64, kb * 64, g, pol);
+                for (int r = 0; r < R; r += chunk) tma_load_3d<1>(dst + r * 128, &p.tmap_w, full + 8u * s, r, kb * 64, g, pol);
               }
             }
           }
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
         }
       } else if (warp == 1) {
         const bool issuer = elect_one();
-        const int n = kRankInner ? (R + 15) / 16 * 16 : (n_slots * R + 15) / 16 * 16;
+        const int n = (n_slots * slot_cols + 15) / 16 * 16;
         const uint32_t idesc = make_idesc_f16(kIsBf16 ? 1u : 0u, 128, static_cast<uint32_t>(n), kRankInner ? 1u : 0u, 0);
         uint32_t at = step;
         for (int i = 0; i < steps; ++i, ++at) {
@@ -288,12 +291,9 @@ __global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const 
 #pragma unroll
               for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * k, idesc, i > 0 || k > 0);
             } else {
-              for (int j = 0; j < n_slots; ++j) {
-                const uint64_t dw = make_smem_desc_sw128_mn(smem_w + s * Cfg::kWBytes + j * slot_cols * 128, 8192);
+              const uint64_t dw = make_smem_desc_rows_mn(smem_w + s * Cfg::kWBytes, chunk * 2u, chunk * 128u);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  umma_f16<1>(tmem + j * slot_cols, dp + 2u * k, dw + 128u * k, idesc, i > 0 || k > 0);
-              }
+              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * chunk * k, idesc, i > 0 || k > 0);
             }
             umma_commit<1>(empty + 8u * s);
             if (i == steps - 1) umma_commit<1>(done);
@@ -410,23 +410,27 @@ struct GradParams {
 };
 
 constexpr int kGradCluster = 4;
-template <int kRankBlocks>   // 64-element blocks of ranks: 1 or 2
+template <int kRanks>   // R rounded up to whole chunks: 16, 32, 64 or 128
 struct GradConfig {
   static constexpr int kThreads = 160;                 // four warps gather and store, one issues
   static constexpr int kRows = 64;                     // rows per ring stage
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kRanks <= 16 ? 4 : 3;
   static constexpr int kBlockBytes = kRows * 128;      // 64 columns of a stage
-  static constexpr int kPBytes = 2 * kBlockBytes, kQBytes = kRankBlocks * kBlockBytes;
+  static constexpr int kPBytes = 2 * kBlockBytes, kQBytes = kRows * kRanks * 2;
+  static constexpr int kChunk = rank_chunk(kRanks);
   static constexpr int kStageBytes = kPBytes + kQBytes;
-  static constexpr int kTmemCols = kRankBlocks * 64;
+  static constexpr int kTmemCols = kRanks < 32 ? 32 : kRanks;
+  static constexpr int kCtasPerSm = kRanks <= 64 ? 3 : 2;
+  // the partial sums of a cut tile lie in the ring: 128 columns x (R + 4), or R x (128 + 4) floats
+  static_assert(kStages * kStageBytes >= 128 * (kRanks + 4) * 4 && kStages * kStageBytes >= kRanks * 132 * 4, "partial sums");
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 128;
-  static constexpr int kCtasPerSm = kRankBlocks == 1 ? 3 : 2;
+  static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 233472, "shared memory of an SM");
 };
 
-template <bool kIsBf16, int kRankBlocks>
-__global__ void __launch_bounds__(160, GradConfig<kRankBlocks>::kCtasPerSm)
+template <bool kIsBf16, int kRanks>
+__global__ void __launch_bounds__(160, GradConfig<kRanks>::kCtasPerSm)
 lora_grad_kernel(const __grid_constant__ GradParams p) {
-  using Cfg = GradConfig<kRankBlocks>;
+  using Cfg = GradConfig<kRanks>;
   constexpr int kStages = Cfg::kStages, kRows = Cfg::kRows;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -511,6 +515,11 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
           const long ldp = side.ldp, ldq = side.ldq;
           // row t of a block sits at t * 128, its piece c at c ^ (t % 8); t % 8 == r0 for all of this thread's rows
           const uint32_t place = static_cast<uint32_t>((piece >> 3) * Cfg::kBlockBytes + r0 * 128 + (((piece & 7) ^ r0) << 4));
+          // Q likewise, in rows of one chunk of ranks with the swizzle of that width
+          constexpr int kPieces = Cfg::kChunk / 8;
+          const int turn = kPieces == 8 ? r0 : (kPieces == 4 ? r0 >> 1 : r0 >> 2);
+          const uint32_t place_q = static_cast<uint32_t>((piece / kPieces) * (kRows * Cfg::kChunk * 2) + r0 * Cfg::kChunk * 2 +
+                                                         (((piece % kPieces) ^ turn) << 4));
           // The rows' places in the batch, kRows / 4 per warp and block: a lane loads one of the next two blocks'
           // entries, two blocks ahead of their use (one block ahead, their latency was every block's time).
           auto fetch_rows = [&](int b) {
@@ -523,14 +532,14 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
           for (int b = b0; b < b1; ++b, ++taken) {
             const uint32_t at = n + static_cast<uint32_t>(taken), s = at % kStages;
             if (!wait_bounded(empty + 8u * s, ((at / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) break;
-            const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place;
+            const uint32_t dst_p = smem_p + s * Cfg::kPBytes + place, dst_q = smem_q + s * Cfg::kQBytes + place_q;
 #pragma unroll
             for (int k = 0; k < kRows / 8; ++k) {
               const int row = __shfl_sync(0xffffffffu, rows_now, (taken & 1) * 16 + static_cast<int>(lane >> 4) * 8 + k);
               const bool live = row >= 0;
               const long m = live ? row : 0;
               cp_async_16(dst_p + k * 1024u, src_p + m * ldp, live && col_ok);
-              if (q_ok) cp_async_16(dst_q + k * 1024u, src_q + m * ldq, live);
+              if (q_ok) cp_async_16(dst_q + k * (8u * Cfg::kChunk * 2u), src_q + m * ldq, live);
             }
             cp_async_arrive(full + 8u * s);
             if (taken & 1) {
@@ -590,9 +599,9 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
             tc_fence_after_sync();
             if (issuer) {
               const uint64_t dp = make_smem_desc_sw128_mn(smem_p + s * Cfg::kPBytes, Cfg::kBlockBytes);
-              const uint64_t dq = make_smem_desc_sw128_mn(smem_q + s * Cfg::kQBytes, Cfg::kBlockBytes);
+              const uint64_t dq = make_smem_desc_rows_mn(smem_q + s * Cfg::kQBytes, Cfg::kChunk * 2u, kRows * Cfg::kChunk * 2u);
 #pragma unroll
-              for (int k = 0; k < kRows / 16; ++k) umma_f16<1>(tmem, dp + 128u * k, dq + 128u * k, idesc, b > b0 || k > 0);
+              for (int k = 0; k < kRows / 16; ++k) umma_f16<1>(tmem, dp + 128u * k, dq + 2u * Cfg::kChunk * k, idesc, b > b0 || k > 0);
               umma_commit<1>(empty + 8u * s);
               if (b == b1 - 1) umma_commit<1>(done);
             }

@@ -54,8 +54,6 @@ int ready(DeviceState** st, int* cuda_error_out) {
   return rc != GEMM_SM100_OK ? rc : get_encoder(cuda_error_out);
 }
 
-// The ranks one adapter item covers: one swizzle row of 32, 64 or 128 bytes.
-int rank_chunk(int R) { return R <= 16 ? 16 : (R <= 32 ? 32 : 64); }
 
 // Tensor map of a 16-bit array of two or three dimensions, innermost first, whose rows of `box[0]` elements
 // land in shared memory with the swizzle of that width.
@@ -262,7 +260,8 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   p.p_rows = a.M >= 128 ? 128 : static_cast<int>(ceil_div(a.M, 8) * 8);
   rc = encode_rows(&p.tmap_p, P, a.dtype, 2, {L, a.M, 1}, {ldp, 0}, {64, p.p_rows, 1}, cuda_error_out);
   if (rc) return rc;
-  rc = kRankInner ? encode_rows(&p.tmap_w, W, a.dtype, 3, {a.R, L, a.adapters}, {ld_w, stride_w}, {64, 64, 1}, cuda_error_out)
+  rc = kRankInner ? encode_rows(&p.tmap_w, W, a.dtype, 3, {a.R, L, a.adapters}, {ld_w, stride_w}, {rank_chunk(a.R), 64, 1},
+                                cuda_error_out)
                   : encode_rows(&p.tmap_w, W, a.dtype, 3, {L, a.R, a.adapters}, {ld_w, stride_w}, {64, a.R, 1}, cuda_error_out);
   if (rc) return rc;
   p.plan = a.plan;
@@ -271,7 +270,7 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   p.out = out;
   p.ld_out = ld_out;
   p.M = a.M, p.R = a.R, p.L = L;
-  p.group_slots = kRankInner ? (a.R > 64 ? 1 : 2) : 128 / a.R;
+  p.group_slots = 128 / (kRankInner ? static_cast<int>(ceil_div(a.R, rank_chunk(a.R))) * rank_chunk(a.R) : a.R);
   p.status = st->status_ptr;
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
 
@@ -292,14 +291,14 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
 }
 
 // Both adapters' gradients in one launch.
-template <bool kIsBf16, int kRankBlocks>
+template <bool kIsBf16, int kRanks>
 int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradSide& up, cudaStream_t stream,
                 int* cuda_error_out) {
-  using Cfg = GradConfig<kRankBlocks>;
+  using Cfg = GradConfig<kRanks>;
   DeviceState* st = nullptr;
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
-  auto kernel = lora_grad_kernel<kIsBf16, kRankBlocks>;
+  auto kernel = lora_grad_kernel<kIsBf16, kRanks>;
   static bool allowed[kMaxDevices];
   cudaError_t e = allow_smem(kernel, Cfg::kSmemBytes, allowed, st->device);
   if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
@@ -427,8 +426,10 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
   if (!d_down && !d_up) return GEMM_SM100_OK;
   const GradSide down{u16(a.A), u16(d_low), u16(d_down), a.lda, ld_d_low, d_down ? a.K : 0, 1};
   const GradSide up{u16(dC), u16(low), u16(d_up), ld_dc, ld_low, d_up ? a.N : 0, 0};
-  if (a.R <= 64) return (bf16 ? launch_grad<true, 1> : launch_grad<false, 1>)(a, down, up, stream, cuda_error_out);
-  return (bf16 ? launch_grad<true, 2> : launch_grad<false, 2>)(a, down, up, stream, cuda_error_out);
+  if (a.R <= 16) return (bf16 ? launch_grad<true, 16> : launch_grad<false, 16>)(a, down, up, stream, cuda_error_out);
+  if (a.R <= 32) return (bf16 ? launch_grad<true, 32> : launch_grad<false, 32>)(a, down, up, stream, cuda_error_out);
+  if (a.R <= 64) return (bf16 ? launch_grad<true, 64> : launch_grad<false, 64>)(a, down, up, stream, cuda_error_out);
+  return (bf16 ? launch_grad<true, 128> : launch_grad<false, 128>)(a, down, up, stream, cuda_error_out);
 }
 
 }  // extern "C"

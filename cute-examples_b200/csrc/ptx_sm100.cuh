@@ -464,6 +464,18 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128_mn(uint32_t smem_addr, 
   return d;
 }
 
+// The same for K rows of 32, 64 or 128 bytes (16, 32 or 64 MN elements) with the swizzle of that width.
+__device__ __forceinline__ uint64_t make_smem_desc_rows_mn(uint32_t smem_addr, uint32_t row_bytes, uint32_t mn_block_bytes) {
+  const uint64_t layout = row_bytes == 128u ? 2u : (row_bytes == 64u ? 4u : 6u);   // SWIZZLE_128B, _64B, _32B
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>((mn_block_bytes >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((8u * row_bytes) >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= layout << 61;
+  return d;
+}
+
 // Instruction descriptor for kind::f16: fp32 accumulate; A and B each K-major (0) or MN-major (1).
 // `ab_format`: 0 = fp16, 1 = bf16.  M and N are the full (pair-wide) extents.
 __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t ab_format, uint32_t m, uint32_t n,
