@@ -96,8 +96,8 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
                           int* cuda_error_out) {
   using Cfg = LoraConfig<ConfigOf<kCfgIndex, kIsBf16>>;
   auto kernel = gemm_lora_kernel<Cfg, false, kBIsKN>;
-  if constexpr (!kBIsKN && has_cluster_split(kCfgIndex)) {
-    if (plan.split_k) kernel = gemm_lora_kernel<Cfg, true, false>;
+  if constexpr (has_cluster_split(kCfgIndex)) {
+    if (plan.split_k) kernel = gemm_lora_kernel<Cfg, true, kBIsKN>;
   }
   // Attributes of this instantiation and the persistent grid's limit, once per device.
   static int max_ctas[kMaxDevices][2];
@@ -187,7 +187,8 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   if (p.b_is_kn) {
-    const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/false, kProductConfigsKN, /*allow_balance=*/false);
+    const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigsKN, /*allow_balance=*/false,
+                               /*allow_workspace=*/false);
     switch (plan.config) {
       case 0: return launch_product_config<0, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
       case 1: return launch_product_config<1, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
