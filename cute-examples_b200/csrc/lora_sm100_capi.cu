@@ -56,7 +56,8 @@ int ready(DeviceState** st, int* cuda_error_out) {
 
 
 // Tensor map of a 16-bit array of two or three dimensions, innermost first, whose rows of `box[0]` elements
-// land in shared memory with the swizzle of that width.
+// land in shared memory with the swizzle of that width.  (L2 fetches of 128 bytes: with 256, 64 adapters of rank 16 beside
+// 128 x 14336 x 512 took 28.7 us instead of 27.7.)
 int encode_rows(CUtensorMap* map, const void* base, int dtype, int rank, const long (&dims)[3], const long (&pitches)[2],
                 const int (&box)[3], int* cuda_error_out) {
   const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]), static_cast<cuuint64_t>(dims[2])};
@@ -68,7 +69,7 @@ int encode_rows(CUtensorMap* map, const void* base, int dtype, int rank, const l
   const CUtensorMapDataType type =
       dtype == GEMM_SM100_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult r = g_encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, strides, b, ones,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, cudaErrorInvalidValue);
 }
