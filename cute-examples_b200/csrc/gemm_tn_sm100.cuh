@@ -128,6 +128,7 @@ struct LoraParams {
   const int* slot_adapter;        // [tiles][256]
   const unsigned int* slot_mask;  // [tiles][256][8]
   int chunk, chunks;              // ranks per item (16, 32 or 64: one swizzle row) and items per slot
+  int R;
 };
 
 // Experiment switches (results are garbage with any of them set).
@@ -413,6 +414,15 @@ struct LoraWork {
 };
 constexpr int kLoraEntries = 32;
 
+// Single-CTA tiles whose slots are one chunk load the tile of low rows once, with the first adapter stage, whose A part the
+// later ones leave alone: all CTAs read the same few KB at the same moment, and fetching them again with every stage
+// cost 5 us of the 17 us that 64 adapters of rank 16 took beside 128 x 14336 x 512.  (Pair tiles rarely have a second stage, and
+// the wait it costs before the next tile's loads.)
+template <class Cfg>
+__device__ __forceinline__ bool lora_low_once(const LoraParams& lora) {
+  return Cfg::kCtaGroup == 1 && lora.chunks == 1;
+}
+
 template <class Cfg>
 __device__ __forceinline__ LoraWork lora_begin(const LoraParams& lora, int m_tile, int part, int factor, uint32_t count_dst) {
   LoraWork w;
@@ -459,6 +469,7 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
   const uint32_t full_leader = (G == 2) ? map_to_cta(ring.full, pair_base) : ring.full;
   const int num_tiles = p.m_tiles * p.n_tiles, k_blocks = p.k_blocks, b_box = p.b_box_rows, a_rows = p.a_box_rows;
   const int chunk = lora.chunk, chunks = lora.chunks;
+  const bool low_once = lora_low_once<Cfg>(lora);
   uint32_t s = 0, phase = 0;
   int tiles_done = 0;
   bool low_ready = false;
@@ -525,16 +536,16 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
       }
       if (!wait_bounded(ring.empty + 8u * s, phase ^ 1u, ctx, kStatusTimeoutProducer + s)) return;
       const uint32_t full = full_leader + 8u * s, dst_a = ring.smem_a + s * Cfg::kABytes, dst_b = ring.smem_b + s * Cfg::kBBytes;
+      const int low_tiles = chunks > 1 ? items : (low_once && stage > 0 ? 0 : 1);   // slots of one chunk share a tile of low rows
       if (issuer && is_leader)
-        mbar_arrive_expect_tx(ring.full + 8u * s, (uint32_t)(G * chunk * 2 * ((chunks == 1 ? 1 : items) * a_rows +
+        mbar_arrive_expect_tx(ring.full + 8u * s, (uint32_t)(G * chunk * 2 * (low_tiles * a_rows +
                                                                              items * (rows_b[0] + rows_b[1]))));
 #pragma unroll 1
       for (int i = 0; i < items; ++i) {
         const int g = __shfl_sync(0xffffffffu, entry_adapter, (entry + i) % kLoraEntries);
         const int r = (chunks == 1 ? 0 : (first + i) % chunks) * chunk;
         if (issuer) {
-          // slots of one chunk share the tile of low rows
-          if (i == 0 || chunks > 1)
+          if (i < low_tiles)
             tma_load_2d<G>(dst_a + (uint32_t)(i * Cfg::kARows * chunk * 2), &lora.tmap_low, full, r, row_a, pol);
 #pragma unroll
           for (int h = 0; h < Cfg::kHalves; ++h) {
@@ -552,6 +563,11 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
         }
       }
       if (++s == Cfg::kStages) s = 0, phase ^= 1u;
+    }
+    if (low_once && lw.stages > 1) {
+      // the next tile's operands may go where the low rows are only when the last adapter stage has read them
+      const uint32_t last = s == 0 ? Cfg::kStages - 1 : s - 1;
+      if (!wait_bounded(ring.empty + 8u * last, s == 0 ? phase ^ 1u : phase, ctx, kStatusTimeoutProducer + last)) return;
     }
   }
 }
@@ -572,6 +588,7 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
   const uint32_t a_sub = (uint32_t)p.a_box_rows * 8u;       // 16-byte units between a stage's K blocks of A
   constexpr uint32_t kBSub = (uint32_t)(Cfg::kBHalfBytes / Cfg::kKSub) >> 4;
   const int chunk = lora.chunk, chunks = lora.chunks;
+  const bool low_once = lora_low_once<Cfg>(lora);
   const uint64_t dl0 = make_smem_desc_rows(ring.smem_a, (uint32_t)chunk * 2u);
   const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(ring.smem_b, (uint32_t)chunk * 128u)
                               : make_smem_desc_rows(ring.smem_b, (uint32_t)chunk * 2u);
@@ -625,6 +642,7 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
       if (++s == Cfg::kStages) s = 0, phase ^= 1u;
     }
     lora_resolve(lw, lora, count_smem);
+    const uint32_t first_stage = s;
     uint4 entry_rows[G];                                 // lane i: row mask of entry i of the current 32
 #pragma unroll
     for (int v = 0; v < G; ++v)
@@ -644,10 +662,9 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
       }
       if (!wait_bounded(ring.full + 8u * s, phase, ctx, kStatusTimeoutMma + s)) return;
       tc_fence_after_sync();
-      const uint64_t dls = dl0 + (uint64_t)((s * Cfg::kABytes) >> 4), dws = dw0 + (uint64_t)((s * Cfg::kBBytes) >> 4);
-#pragma unroll 1
-      for (int i = 0; i < items; ++i) {
-        uint32_t skip[4 * G];
+      const uint64_t dls = dl0 + (uint64_t)(((low_once ? first_stage : s) * Cfg::kABytes) >> 4), dws = dw0 + (uint64_t)((s * Cfg::kBBytes) >> 4);
+      // rows that item i leaves alone; fetched one item ahead
+      auto rows_to_skip = [&](int i, uint32_t (&skip)[4 * G]) {
 #pragma unroll
         for (int v = 0; v < G; ++v) {
           skip[4 * v] = ~__shfl_sync(0xffffffffu, entry_rows[v].x, (entry + i) % kLoraEntries);
@@ -655,12 +672,23 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
           skip[4 * v + 2] = ~__shfl_sync(0xffffffffu, entry_rows[v].z, (entry + i) % kLoraEntries);
           skip[4 * v + 3] = ~__shfl_sync(0xffffffffu, entry_rows[v].w, (entry + i) % kLoraEntries);
         }
+      };
+      uint32_t next[4 * G];
+      rows_to_skip(0, next);
+#pragma unroll 1
+      for (int i = 0; i < items; ++i) {
+        uint32_t skip[4 * G];
+#pragma unroll
+        for (int v = 0; v < 4 * G; ++v) skip[v] = next[v];
+        rows_to_skip(i + 1, next);
+        // whole 16-rank steps that exist
+        const int ranks = min(chunk, lora.R - (chunks == 1 ? 0 : (first + i) % chunks) * chunk);
         const uint64_t dl = dls + (uint64_t)((chunks == 1 ? 0u : (uint32_t)(i * Cfg::kARows * chunk * 2)) >> 4);
         const uint64_t dw = dws + (uint64_t)((uint32_t)(i * Cfg::kBRows * chunk * 2) >> 4);
         if (issuer) {
 #pragma unroll
           for (int h = 0; h < Cfg::kHalves; ++h)
-            for (int k = 0; k < chunk / Cfg::kUmmaK; ++k)
+            for (int k = 0; k * Cfg::kUmmaK < ranks; ++k)
               umma_f16_rows<G>(tmem_base + (slot0 + h) * Cfg::kSlotCols, dl + 2u * k,
                                dw + (uint64_t)((h * Cfg::kBHalfBytes) >> 4) + kBStepK * k, idesc[h], skip);
         }

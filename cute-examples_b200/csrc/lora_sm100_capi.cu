@@ -161,6 +161,7 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
   if (rc) return rc;
   LoraParams lora;
   std::memset(&lora, 0, sizeof(lora));
+  lora.R = o.R;
   lora.chunk = rank_chunk(o.R);
   lora.chunks = static_cast<int>(ceil_div(o.R, lora.chunk));
   rc = encode_rows(&lora.tmap_low, o.low, p.dtype, 2, {o.R, p.M, 1}, {o.ld_low, 0}, {lora.chunk, tp.a_box_rows, 1}, cuda_error_out);
