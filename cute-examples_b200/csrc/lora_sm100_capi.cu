@@ -74,10 +74,9 @@ int encode_rows(CUtensorMap* map, const void* base, int dtype, int rank, const l
   return r == CUDA_SUCCESS ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, cudaErrorInvalidValue);
 }
 
-// Tile configurations with an adapter kernel: every one the planner chooses by itself, but the few-tile ones
-// that it only takes through the workspace; the layouts' four for B as [K, N].
-constexpr unsigned kProductConfigs = (1u << 0) | (1u << 1) | (1u << 2) | (1u << 9) | (1u << 10) | (1u << 11) | (1u << 12) |
-                                     (1u << 13) | (1u << 14) | (1u << 15);
+// Tile configurations with an adapter kernel: those the planner chooses by itself, and the layouts' four for B as [K, N].
+constexpr unsigned kProductConfigs = (1u << 0) | (1u << 1) | (1u << 2) | (1u << 3) | (1u << 7) | (1u << 9) | (1u << 10) |
+                                     (1u << 11) | (1u << 12) | (1u << 13) | (1u << 14) | (1u << 15);
 constexpr unsigned kProductConfigsKN = 0xfu;
 // those whose K can be cut inside a cluster
 constexpr bool has_cluster_split(int config) { return config == 0 || config == 2 || config == 11 || config == 12; }
@@ -204,6 +203,8 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
     case 0: return launch_product_config<0, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 1: return launch_product_config<1, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 2: return launch_product_config<2, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 3: return launch_product_config<3, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
+    case 7: return launch_product_config<7, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 9: return launch_product_config<9, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 10: return launch_product_config<10, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 11: return launch_product_config<11, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);

@@ -173,7 +173,8 @@ FORCED = [
     (0, 0, 600, 776, 320, 24, 5), (0, 2, 300, 520, 2048, 16, 9), (0, 4, 300, 520, 4096, 96, 3), (1, 0, 700, 1504, 200, 40, 4),
     (2, 0, 300, 520, 320, 16, 7), (2, 2, 200, 520, 2048, 64, 40), (2, 4, 129, 264, 2112, 128, 6), (9, 0, 16, 1000, 264, 16, 16),
     (10, 0, 64, 520, 328, 72, 30), (11, 0, 300, 648, 640, 8, 12), (11, 2, 257, 264, 2048, 32, 11), (12, 0, 128, 520, 640, 48, 90),
-    (12, 4, 100, 392, 4096, 16, 100), (12, 2, 100, 392, 2048, 80, 4), (13, 0, 16, 648, 576, 8, 16), (14, 0, 63, 648, 576, 128, 20),
+    (12, 4, 100, 392, 4096, 16, 100), (12, 2, 100, 392, 2048, 80, 4), (13, 0, 16, 648, 576, 8, 16), (14, 0, 63, 648, 576, 128, 20), (3, 0, 140, 392, 328, 24, 7),
+    (7, 0, 300, 520, 392, 40, 5),
     (14, 0, 64, 200, 256, 16, 64), (15, 0, 9, 776, 640, 104, 4),
 ]
 
