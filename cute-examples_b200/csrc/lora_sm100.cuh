@@ -167,19 +167,21 @@ struct LowParams {
   unsigned long long timeout_ns;
 };
 
+// kDeep: six stages and one CTA per SM instead of three and two, for launches that do not fill the SMs twice.
+template <bool kDeep>
 struct LowConfig {
   static constexpr int kThreads = 192;                 // producer, MMA issuer, four epilogue warps
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kDeep ? 6 : 3;
   static constexpr int kPBytes = 128 * 64 * 2, kWBytes = 128 * 64 * 2;
   static constexpr int kStageBytes = kPBytes + kWBytes;
   static constexpr int kTmemCols = 128;
   static constexpr int kBarrierBytes = 128;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + 128 * 8;   // two CTAs per SM
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + 128 * 8;
 };
 
-template <bool kIsBf16, bool kRankInner>
-__global__ void __launch_bounds__(LowConfig::kThreads, 2) lora_low_kernel(const __grid_constant__ LowParams p) {
-  using Cfg = LowConfig;
+template <bool kIsBf16, bool kRankInner, bool kDeep>
+__global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __grid_constant__ LowParams p) {
+  using Cfg = LowConfig<kDeep>;
   constexpr int kStages = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -479,13 +481,25 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
       my_first = v.offsets[g0 + lane];
       my_last = v.offsets[g0 + lane + 1];
       while (my_splits < kGradCluster && my_last - my_first > p.split_rows * my_splits) my_splits *= 2;
-      my_end = (p.tiles * my_splits + kGradCluster - 1) / kGradCluster;
+      if (my_last > my_first) my_end = (p.tiles * my_splits + kGradCluster - 1) / kGradCluster;
     }
     for (int o = 1; o < 32; o *= 2) {
       const int below = __shfl_up_sync(0xffffffffu, my_end, o);
       if (static_cast<int>(lane) >= o) my_end += below;
     }
     my_end += batch_start;                               // where this lane's adapter ends in the grid's units
+    // Adapters without rows have no units: the whole grid writes their zeros, contiguous memory.
+    uint32_t without = __ballot_sync(0xffffffffu, my_last == my_first && g0 + static_cast<int>(lane) < p.adapters);
+    for (; without != 0; without &= without - 1) {
+      const long g = g0 + __ffs(static_cast<int>(without)) - 1;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const long pieces = static_cast<long>(p.side[x].D) * R / 8;          // of 16 bytes
+        uint4* out = reinterpret_cast<uint4*>(p.side[x].out + g * p.side[x].D * R);
+        for (long i = static_cast<long>(blockIdx.x) * Cfg::kThreads + threadIdx.x; i < pieces; i += static_cast<long>(gridDim.x) * Cfg::kThreads)
+          out[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
     const int batch_end = __shfl_sync(0xffffffffu, my_end, 31);
 #pragma unroll 1
     for (; u < batch_end; u += clusters) {
@@ -616,7 +630,7 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
         cluster_arrive();
         cluster_wait();
       }
-      if (work && (splits > 1 || b1 == b0)) {             // (an adapter without rows: zeros)
+      if (work && splits > 1) {
         // This CTA's share of its tile's sums, four neighbours at a time, added over the parts in rank order.
         const int per_row = (side.rank_outer ? 128 : R) / 4, quads = 32 * R, leader = rank - part;
         const int q0 = quads * part / splits, q1 = quads * (part + 1) / splits;

@@ -247,6 +247,16 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices], int 
   return e;
 }
 
+template <bool kIsBf16, bool kRankInner, bool kDeep>
+int launch_low_kernel(const LowParams& p, long ctas, int splits, DeviceState& st, cudaStream_t stream, int* cuda_error_out) {
+  using Cfg = LowConfig<kDeep>;
+  auto kernel = lora_low_kernel<kIsBf16, kRankInner, kDeep>;
+  static bool allowed[kMaxDevices];
+  cudaError_t e = allow_smem(kernel, Cfg::kSmemBytes, allowed, st.device);
+  if (e == cudaSuccess) e = launch_cluster(kernel, ctas, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+}
+
 // low rows of P [M, L] through W: down [adapters, R, L], or (kRankInner) up [adapters, L, R].
 template <bool kIsBf16, bool kRankInner>
 int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
@@ -254,11 +264,6 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   DeviceState* st = nullptr;
   int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
-  auto kernel = lora_low_kernel<kIsBf16, kRankInner>;
-  static bool allowed[kMaxDevices];
-  cudaError_t e = allow_smem(kernel, LowConfig::kSmemBytes, allowed, st->device);
-  if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
-
   LowParams p;
   std::memset(&p, 0, sizeof(p));
   p.p_rows = a.M >= 128 ? 128 : static_cast<int>(ceil_div(a.M, 8) * 8);
@@ -290,8 +295,13 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   long groups = room / (tiles * splits);
   groups = groups < 1 ? 1 : (groups > most_groups ? most_groups : groups);
   p.groups = static_cast<int>(groups);
-  e = launch_cluster(kernel, tiles * groups * splits, splits, LowConfig::kThreads, LowConfig::kSmemBytes, stream, p);
-  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+  // The deep ring for long runs of K blocks, when that leaves no SM with two CTAs, or hardly (every further group may turn
+  // out to be empty): 64 x 4096 x 14336 with 32 adapters of rank 64 takes 45.8 us that way, 49.2 with the short ring.  With few
+  // K blocks the SMs it takes from the product kernel behind cost more: 128 x 14336 x 4096 with 64 adapters of
+  // rank 16 takes 44.6 us deep and 40.7 short (8 blocks per CTA).
+  const bool deep = k_blocks >= 12L * splits && tiles * splits * (groups < 2 ? groups : 2) <= st->sm_count;
+  return deep ? launch_low_kernel<kIsBf16, kRankInner, true>(p, tiles * groups * splits, splits, *st, stream, cuda_error_out)
+              : launch_low_kernel<kIsBf16, kRankInner, false>(p, tiles * groups * splits, splits, *st, stream, cuda_error_out);
 }
 
 // Both adapters' gradients in one launch.
