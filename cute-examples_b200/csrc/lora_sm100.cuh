@@ -474,6 +474,9 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
   // The adapters' groups of tiles, one adapter after another, are the units of the grid; clusters take them in
   // turn.  Every warp finds its units by itself, 32 adapters at a time.
   int u = cluster, batch_start = 0;
+  int empties = 0;
+  const long zeros = (static_cast<long>(p.side[0].D) + p.side[1].D) * R / 8;     // 16-byte pieces per adapter
+  const int fill = static_cast<int>(min(static_cast<long>(gridDim.x), zeros / (Cfg::kThreads * 4) + 1));
 #pragma unroll 1
   for (int g0 = 0; g0 < p.adapters; g0 += 32) {
     int my_first = 0, my_last = 0, my_splits = 1, my_end = 0;
@@ -488,15 +491,23 @@ lora_grad_kernel(const __grid_constant__ GradParams p) {
       if (static_cast<int>(lane) >= o) my_end += below;
     }
     my_end += batch_start;                               // where this lane's adapter ends in the grid's units
-    // Adapters without rows have no units: the whole grid writes their zeros, contiguous memory.
-    uint32_t without = __ballot_sync(0xffffffffu, my_last == my_first && g0 + static_cast<int>(lane) < p.adapters);
-    for (; without != 0; without &= without - 1) {
-      const long g = g0 + __ffs(static_cast<int>(without)) - 1;
+    // Adapters without rows have no units.  Their zeros are contiguous memory, written by `fill` CTAs per adapter, the
+    // next ones for every further adapter; a lane finds out whether this CTA writes for its adapter.
+    const bool empty_here = my_last == my_first && g0 + static_cast<int>(lane) < p.adapters;
+    const uint32_t all_empty = __ballot_sync(0xffffffffu, empty_here);
+    const int order = empties + __popc(all_empty & ((1u << lane) - 1u));
+    empties += __popc(all_empty);
+    const int grid = static_cast<int>(gridDim.x);
+    const int turn = static_cast<int>((static_cast<long>(grid) + blockIdx.x - static_cast<long>(order) * fill % grid) % grid);
+    for (uint32_t mine = __ballot_sync(0xffffffffu, empty_here && turn < fill); mine != 0; mine &= mine - 1) {
+      const int from = __ffs(static_cast<int>(mine)) - 1;
+      const long g = g0 + from;
+      const int part = __shfl_sync(0xffffffffu, turn, from);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const long pieces = static_cast<long>(p.side[x].D) * R / 8;          // of 16 bytes
         uint4* out = reinterpret_cast<uint4*>(p.side[x].out + g * p.side[x].D * R);
-        for (long i = static_cast<long>(blockIdx.x) * Cfg::kThreads + threadIdx.x; i < pieces; i += static_cast<long>(gridDim.x) * Cfg::kThreads)
+        for (long i = static_cast<long>(part) * Cfg::kThreads + threadIdx.x; i < pieces; i += static_cast<long>(fill) * Cfg::kThreads)
           out[i] = make_uint4(0u, 0u, 0u, 0u);
       }
     }
