@@ -175,6 +175,9 @@ struct Plan {
   bool cluster = false;      // even split whose contributors form a cluster and exchange partial sums in shared memory
 };
 
+// One-time set-up of every adapter kernel on the device (part of gemm_sm100_init).
+int lora_prepare(DeviceState& st, int* cuda_error_out);
+
 // The plan of a problem under the current options, cached per thread.  `allow_workspace` false: no K-split
 // that needs a workspace; `config_mask`: the configurations the caller has kernels for.
 Plan plan_for(int M, int N, int K, int sm_count, bool allow_split = true, unsigned config_mask = ~0u,

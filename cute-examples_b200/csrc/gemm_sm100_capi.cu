@@ -1290,5 +1290,6 @@ extern "C" int gemm_sm100_init(int* cuda_error_out) {
       st->static_scratch = ptr;
     }
   }
-  return ensure_all(*st, cuda_error_out, std::make_integer_sequence<int, kNumConfigs>{});
+  const int rc = ensure_all(*st, cuda_error_out, std::make_integer_sequence<int, kNumConfigs>{});
+  return rc ? rc : lora_prepare(*st, cuda_error_out);
 }

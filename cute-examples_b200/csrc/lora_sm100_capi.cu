@@ -3,6 +3,9 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstring>
+#include <mutex>
+#include <utility>
 
 #include "gemm_host_sm100.cuh"
 #include "lora_sm100.cuh"
@@ -91,48 +94,61 @@ struct AdapterOperands {
   const void* plan;
 };
 
+template <class Cfg, int kCfgIndex, bool kBIsKN>
+auto product_kernel(bool split_k) {
+  auto kernel = gemm_lora_kernel<Cfg, false, kBIsKN>;
+  if constexpr (has_cluster_split(kCfgIndex)) {
+    if (split_k) kernel = gemm_lora_kernel<Cfg, true, kBIsKN>;
+  }
+  return kernel;
+}
+
+// One-time set-up of an instantiation on a device: its shared-memory limit, and how many CTAs of it are co-resident.
+template <int kCfgIndex, bool kIsBf16, bool kBIsKN>
+int product_limit(bool split_k, DeviceState& st, int* limit, int* cuda_error_out) {
+  using Cfg = LoraConfig<ConfigOf<kCfgIndex, kIsBf16>>;
+  static int max_ctas[kMaxDevices][2];
+  std::lock_guard<std::mutex> lock(g_mutex);
+  int& known = max_ctas[st.device][split_k ? 1 : 0];
+  if (known == 0) {
+    const auto kernel = product_kernel<Cfg, kCfgIndex, kBIsKN>(split_k);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+    int held = 0;
+    if (Cfg::kCtaGroup == 1) {
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, Cfg::kThreads, Cfg::kSmemBytes);
+      held *= st.sm_count;
+    } else {
+      cudaLaunchConfig_t qc = {};
+      qc.gridDim = dim3(static_cast<unsigned>(st.sm_count - st.sm_count % 2));
+      qc.blockDim = dim3(Cfg::kThreads);
+      qc.dynamicSmemBytes = Cfg::kSmemBytes;
+      cudaLaunchAttribute qa[1];
+      qa[0].id = cudaLaunchAttributeClusterDimension;
+      qa[0].val.clusterDim.x = 2;
+      qa[0].val.clusterDim.y = 1;
+      qa[0].val.clusterDim.z = 1;
+      qc.attrs = qa;
+      qc.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&held, kernel, &qc);
+      held *= 2;
+    }
+    if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+    if (held < 1) return set_cuda_error(cuda_error_out, cudaErrorLaunchOutOfResources);
+    known = held < st.sm_count ? held : st.sm_count - st.sm_count % Cfg::kCtaGroup;
+  }
+  *limit = known;
+  return GEMM_SM100_OK;
+}
+
 template <int kCfgIndex, bool kIsBf16, bool kBIsKN>
 int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan& plan, DeviceState& st, cudaStream_t stream,
                           int* cuda_error_out) {
   using Cfg = LoraConfig<ConfigOf<kCfgIndex, kIsBf16>>;
-  auto kernel = gemm_lora_kernel<Cfg, false, kBIsKN>;
-  if constexpr (has_cluster_split(kCfgIndex)) {
-    if (plan.split_k) kernel = gemm_lora_kernel<Cfg, true, kBIsKN>;
-  }
-  // Attributes of this instantiation and the persistent grid's limit, once per device.
-  static int max_ctas[kMaxDevices][2];
-  int limit;
-  {
-    std::lock_guard<std::mutex> lock(g_mutex);
-    int& known = max_ctas[st.device][plan.split_k ? 1 : 0];
-    if (known == 0) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
-      if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
-      int held = 0;
-      if (Cfg::kCtaGroup == 1) {
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, Cfg::kThreads, Cfg::kSmemBytes);
-        held *= st.sm_count;
-      } else {
-        cudaLaunchConfig_t qc = {};
-        qc.gridDim = dim3(static_cast<unsigned>(st.sm_count - st.sm_count % 2));
-        qc.blockDim = dim3(Cfg::kThreads);
-        qc.dynamicSmemBytes = Cfg::kSmemBytes;
-        cudaLaunchAttribute qa[1];
-        qa[0].id = cudaLaunchAttributeClusterDimension;
-        qa[0].val.clusterDim.x = 2;
-        qa[0].val.clusterDim.y = 1;
-        qa[0].val.clusterDim.z = 1;
-        qc.attrs = qa;
-        qc.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&held, kernel, &qc);
-        held *= 2;
-      }
-      if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
-      if (held < 1) return set_cuda_error(cuda_error_out, cudaErrorLaunchOutOfResources);
-      known = held < st.sm_count ? held : st.sm_count - st.sm_count % Cfg::kCtaGroup;
-    }
-    limit = known;
-  }
+  const auto kernel = product_kernel<Cfg, kCfgIndex, kBIsKN>(plan.split_k);
+  int limit = 0;
+  int rc = product_limit<kCfgIndex, kIsBf16, kBIsKN>(plan.split_k, st, &limit, cuda_error_out);
+  if (rc) return rc;
 
   TileParams tp = base_tile_params<Cfg>(p, st);
   int b_box = Cfg::kBRows;
@@ -151,7 +167,7 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
     tp.sk_cluster = 1;
   }
   CUtensorMap map_a, map_b, map_c;
-  int rc = encode_2d(&map_a, p.A, p.dtype, p.M, p.K, p.lda, tp.a_box_rows, cuda_error_out, Cfg::kKSub);
+  rc = encode_2d(&map_a, p.A, p.dtype, p.M, p.K, p.lda, tp.a_box_rows, cuda_error_out, Cfg::kKSub);
   if (rc) return rc;
   rc = kBIsKN ? encode_2d(&map_b, p.B, p.dtype, p.K, p.N, p.ldb, 64, cuda_error_out)
               : encode_2d(&map_b, p.B, p.dtype, p.N, p.K, p.ldb, b_box, cuda_error_out, Cfg::kKSub);
@@ -248,12 +264,16 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices], int 
 }
 
 template <bool kIsBf16, bool kRankInner, bool kDeep>
+cudaError_t allow_low(DeviceState& st) {
+  static bool allowed[kMaxDevices];
+  return allow_smem(lora_low_kernel<kIsBf16, kRankInner, kDeep>, LowConfig<kDeep>::kSmemBytes, allowed, st.device);
+}
+
+template <bool kIsBf16, bool kRankInner, bool kDeep>
 int launch_low_kernel(const LowParams& p, long ctas, int splits, DeviceState& st, cudaStream_t stream, int* cuda_error_out) {
   using Cfg = LowConfig<kDeep>;
-  auto kernel = lora_low_kernel<kIsBf16, kRankInner, kDeep>;
-  static bool allowed[kMaxDevices];
-  cudaError_t e = allow_smem(kernel, Cfg::kSmemBytes, allowed, st.device);
-  if (e == cudaSuccess) e = launch_cluster(kernel, ctas, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  cudaError_t e = allow_low<kIsBf16, kRankInner, kDeep>(st);
+  if (e == cudaSuccess) e = launch_cluster(lora_low_kernel<kIsBf16, kRankInner, kDeep>, ctas, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
@@ -304,6 +324,12 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
               : launch_low_kernel<kIsBf16, kRankInner, false>(p, tiles * groups * splits, splits, *st, stream, cuda_error_out);
 }
 
+template <bool kIsBf16, int kRanks>
+cudaError_t allow_grad(DeviceState& st) {
+  static bool allowed[kMaxDevices];
+  return allow_smem(lora_grad_kernel<kIsBf16, kRanks>, GradConfig<kRanks>::kSmemBytes, allowed, st.device);
+}
+
 // Both adapters' gradients in one launch.
 template <bool kIsBf16, int kRanks>
 int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradSide& up, cudaStream_t stream,
@@ -313,8 +339,7 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   auto kernel = lora_grad_kernel<kIsBf16, kRanks>;
-  static bool allowed[kMaxDevices];
-  cudaError_t e = allow_smem(kernel, Cfg::kSmemBytes, allowed, st->device);
+  cudaError_t e = allow_grad<kIsBf16, kRanks>(*st);
   if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
   GradParams p;
   std::memset(&p, 0, sizeof(p));
@@ -346,7 +371,49 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
+template <int kCfgIndex, bool kIsBf16>
+int prepare_config(DeviceState& st, int* cuda_error_out) {
+  int limit = 0, rc = GEMM_SM100_OK;
+  for (int split = 0; split < (has_cluster_split(kCfgIndex) ? 2 : 1) && rc == GEMM_SM100_OK; ++split) {
+    if constexpr (((kProductConfigs >> kCfgIndex) & 1u) != 0)
+      rc = product_limit<kCfgIndex, kIsBf16, false>(split != 0, st, &limit, cuda_error_out);
+    if constexpr (((kProductConfigsKN >> kCfgIndex) & 1u) != 0)
+      if (rc == GEMM_SM100_OK) rc = product_limit<kCfgIndex, kIsBf16, true>(split != 0, st, &limit, cuda_error_out);
+  }
+  return rc;
+}
+
+template <bool kIsBf16, int... kIndices>
+int prepare_type(DeviceState& st, int* cuda_error_out, std::integer_sequence<int, kIndices...>) {
+  int rc = GEMM_SM100_OK;
+  (void)((rc = prepare_config<kIndices, kIsBf16>(st, cuda_error_out), rc == GEMM_SM100_OK) && ...);
+  if (rc != GEMM_SM100_OK) return rc;
+  cudaError_t e = allow_low<kIsBf16, false, false>(st);
+  if (e == cudaSuccess) e = allow_low<kIsBf16, false, true>(st);
+  if (e == cudaSuccess) e = allow_low<kIsBf16, true, false>(st);
+  if (e == cudaSuccess) e = allow_low<kIsBf16, true, true>(st);
+  if (e == cudaSuccess) e = allow_grad<kIsBf16, 16>(st);
+  if (e == cudaSuccess) e = allow_grad<kIsBf16, 32>(st);
+  if (e == cudaSuccess) e = allow_grad<kIsBf16, 64>(st);
+  if (e == cudaSuccess) e = allow_grad<kIsBf16, 128>(st);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+}
+
 }  // namespace
+
+namespace gemm_sm100 {
+namespace host {
+
+int lora_prepare(DeviceState& st, int* cuda_error_out) {
+  cudaFuncAttributes attributes;
+  const cudaError_t e = cudaFuncGetAttributes(&attributes, lora_plan_kernel);   // loads it
+  if (e != cudaSuccess) return set_cuda_error(cuda_error_out, e);
+  const int rc = prepare_type<true>(st, cuda_error_out, std::make_integer_sequence<int, kNumConfigs>{});
+  return rc ? rc : prepare_type<false>(st, cuda_error_out, std::make_integer_sequence<int, kNumConfigs>{});
+}
+
+}  // namespace host
+}  // namespace gemm_sm100
 
 extern "C" {
 

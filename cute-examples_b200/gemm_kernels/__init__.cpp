@@ -247,10 +247,6 @@ gemm_sm100_lora_args lora_args(const torch::Tensor& A, const torch::Tensor& B, c
                 "scale must be a number or a contiguous float32 tensor with one value per adapter");
     a.scales = static_cast<const float*>(scales->const_data_ptr());
   }
-  for (const auto& t : {std::make_pair(&A, "A"), std::make_pair(&B, "B"), std::make_pair(&down, "down"),
-                        std::make_pair(&up, "up"), std::make_pair(&plan, "plan")})
-    check_placed(*t.first, t.second, A);
-  if (scales.has_value()) check_placed(*scales, "scale", A);
   a.M = static_cast<int>(M), a.N = static_cast<int>(N), a.K = static_cast<int>(K);
   a.R = static_cast<int>(R), a.adapters = static_cast<int>(G);
   a.A = A.const_data_ptr(), a.B = B.const_data_ptr(), a.down = down.const_data_ptr(), a.up = up.const_data_ptr();
@@ -261,6 +257,15 @@ gemm_sm100_lora_args lora_args(const torch::Tensor& A, const torch::Tensor& B, c
   return a;
 }
 
+// Placement of the same tensors, after every check that needs no device.
+void lora_placed(const torch::Tensor& A, const torch::Tensor& B, const torch::Tensor& down, const torch::Tensor& up,
+                 const torch::Tensor& plan, const OptTensor& scales) {
+  for (const auto& t : {std::make_pair(&A, "A"), std::make_pair(&B, "B"), std::make_pair(&down, "down"),
+                        std::make_pair(&up, "up"), std::make_pair(&plan, "plan")})
+    check_placed(*t.first, t.second, A);
+  if (scales.has_value()) check_placed(*scales, "scale", A);
+}
+
 }  // namespace
 
 torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torch::Tensor down, const torch::Tensor up,
@@ -269,6 +274,7 @@ torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torc
   const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
   check_like(C, "out", A, {a.M, a.N});
   check_like(low, "low", A, {a.M, a.R});
+  lora_placed(A, B, down, up, plan, scales);
   check_placed(C, "out", A);
   check_placed(low, "low", A);
   if (a.M == 0) return C;
@@ -293,15 +299,17 @@ void gemm_lora_backward(const torch::Tensor dC, const torch::Tensor A, const tor
   const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
   TORCH_CHECK(dC.dim() == 2, "dC must be a 2D (matrix) tensor");
   check_like(dC, "dC", A, {a.M, a.N});
-  check_placed(dC, "dC", A);
   TORCH_CHECK(a.N % 8 == 0, "N must be a multiple of 8 (it is the inner dimension of dC * B), got ", a.N);
-  if (low.has_value()) {
-    check_like(*low, "low", A, {a.M, a.R});
-    check_placed(*low, "low", A);
-  }
-  if (dA.has_value()) check_like(*dA, "dA", A, {a.M, a.K}), check_placed(*dA, "dA", A);
-  if (d_down.has_value()) check_like(*d_down, "d_down", A, {a.adapters, a.R, a.K}, true), check_placed(*d_down, "d_down", A);
-  if (d_up.has_value()) check_like(*d_up, "d_up", A, {a.adapters, a.N, a.R}, true), check_placed(*d_up, "d_up", A);
+  if (low.has_value()) check_like(*low, "low", A, {a.M, a.R});
+  if (dA.has_value()) check_like(*dA, "dA", A, {a.M, a.K});
+  if (d_down.has_value()) check_like(*d_down, "d_down", A, {a.adapters, a.R, a.K}, true);
+  if (d_up.has_value()) check_like(*d_up, "d_up", A, {a.adapters, a.N, a.R}, true);
+  lora_placed(A, B, down, up, plan, scales);
+  check_placed(dC, "dC", A);
+  if (low.has_value()) check_placed(*low, "low", A);
+  if (dA.has_value()) check_placed(*dA, "dA", A);
+  if (d_down.has_value()) check_placed(*d_down, "d_down", A);
+  if (d_up.has_value()) check_placed(*d_up, "d_up", A);
   c10::cuda::CUDAGuard guard(A.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(A.device().index()).stream();
   // scratch from the caching allocator: safe in stream order, and part of the graph's own memory under capture

@@ -423,3 +423,136 @@ def test_gradients_against_differences(gk):
         _, tol = want(t)
         bound = float((tol["dA" if name == "A" else "d_" + name] * direction.abs()).sum()) + 1e-6
         assert abs(float((grad * direction).sum()) - slope) <= bound
+
+
+@pytest.mark.parametrize("M,G,kind", [(1, 1, "one"), (255, 30, "random"), (256, 256, "own"), (700, 9, "random"), (1000, 4096, "own"),
+                                      (513, 5, "none")])
+@pytest.mark.parametrize("wide", [False, True])
+def test_plan_contents(gk, M, G, kind, wide):
+    """The slot lists, row masks and per-adapter row lists against a plain construction."""
+    ids = id_pattern(kind, M, G, M)
+    if wide:
+        ids = ids.long()
+        ids[ids < 0] = 2 ** 40 + 1                          # no adapter, although its low 32 bits are 1
+    plan = gk.LoraPlan(ids.cuda(), G)
+    words = plan.buffer.view(torch.int32).cpu().tolist()
+    up64 = lambda n: (n + 63) // 64 * 64  # noqa: E731
+    tiles = -(-M // 256)
+    at = up64(tiles)
+    adapters, masks = at, at + tiles * 256
+    row_slot = masks + tiles * 256 * 8
+    order = row_slot + up64(M)
+    offsets = order + up64(M)
+    clean = [i if 0 <= i < G else -1 for i in ids.tolist()]
+    for t in range(tiles):
+        rows = clean[t * 256:(t + 1) * 256]
+        slots = list(dict.fromkeys(i for i in rows if i >= 0))
+        assert words[t] == len(slots)
+        assert words[adapters + t * 256:adapters + t * 256 + len(slots)] == slots
+        for j, g in enumerate(slots):
+            mask = sum(1 << r for r, i in enumerate(rows) if i == g)
+            got = words[masks + (t * 256 + j) * 8:masks + (t * 256 + j) * 8 + 8]
+            assert sum((w & 0xffffffff) << (32 * k) for k, w in enumerate(got)) == mask
+        assert words[row_slot + t * 256:row_slot + t * 256 + len(rows)] == [slots.index(i) if i >= 0 else -1 for i in rows]
+    want_order = [m for g in sorted(set(clean) - {-1}) for m in range(M) if clean[m] == g]
+    assert words[order:order + len(want_order)] == want_order
+    counts = [0] * G
+    for i in clean:
+        if i >= 0:
+            counts[i] += 1
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    assert words[offsets:offsets + G + 1] == starts
+
+
+@pytest.mark.parametrize("N", [1, 3, 9, 63])
+def test_columns_that_fill_no_piece(gk, N):
+    """A handful of columns inside a wider buffer: the columns behind them keep what they held."""
+    M, K, R, G = 70, 72, 8, 3
+    t = make(M, 64, K, R, G, torch.bfloat16, 60 + N, id_pattern("random", M, G, 5))
+    t["B"], t["up"], t["dC"] = t["B"][:N], t["up"][:, :N].contiguous(), t["dC"][:, :N]
+    out = torch.full((M, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    forward_only(gk, t, out=out[:, :N])
+    res, tol = want(t)
+    check("C", out[:, :N], res, tol)
+    assert bool((out[:, N:] == 3).all())
+
+
+def test_first_use_inside_a_capture():
+    """In a fresh process: init(), then a plan, a forward and a backward pass captured as the first calls of all."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import sys; sys.path[:0] = [{repo!r}, {pkg!r}]
+import torch, gemm_kernels as gk
+gk.init()
+dt, M, N, K, R, G = torch.bfloat16, 200, 264, 320, 24, 5
+r = lambda *s: torch.randn(*s, device="cuda").to(dt)
+A, B, down, up, dC = r(M, K), r(N, K), r(G, R, K), r(G, N, R), r(M, N)
+ids = torch.arange(M, device="cuda", dtype=torch.int32) % G
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    plan = gk.LoraPlan(ids, G)
+    C = gk.gemm_lora(A, B, down, up, plan)
+    grads = gk.gemm_lora_backward(dC, A, B, down, up, plan)
+graph.replay()
+torch.cuda.synchronize()
+plan2 = gk.LoraPlan(ids, G)
+assert torch.equal(C, gk.gemm_lora(A, B, down, up, plan2))
+for x, y in zip(grads, gk.gemm_lora_backward(dC, A, B, down, up, plan2)):
+    assert torch.equal(x, y)
+gk.device_status()
+print("captured")
+"""
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code.format(repo=repo, pkg=os.path.join(repo, "cute-examples_b200"))],
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_one_step_after_another(gk):
+    """A run as a training loop makes it: plan refilled, forward, backward, the adapters updated in place, twice, next
+    to plain products of the library; against the same loop in 64 bits within the first step's tolerances."""
+    M, N, K, R, G = 512, 264, 328, 16, 3
+    t = make(M, N, K, R, G, torch.bfloat16, 80, id_pattern("runs", M, G, 3))
+    plan = gk.LoraPlan(t["ids"], G)
+    for step in range(2):
+        t["ids"] = id_pattern("runs", M, G, 10 + step).cuda()
+        plan.update(t["ids"])
+        low = torch.empty(M, R, dtype=torch.bfloat16, device="cuda")
+        plain = gk.gemm_tn(t["A"], t["B"])
+        C = gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low)
+        after = gk.gemm_tn(t["A"], t["B"])
+        dA, d_down, d_up = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low)
+        assert torch.equal(plain, after)
+        res, tol = want(t)
+        for name, value in (("C", C), ("low", low), ("dA", dA), ("d_down", d_down), ("d_up", d_up)):
+            check(name, value, res, tol)
+        t["down"] -= 0.01 * d_down
+        t["up"] -= 0.01 * d_up
+    gk.device_status()
+
+
+def test_long_rows_and_far_adapters(gk):
+    """Offsets that pass 32 bits: adapters whose weights lie more than 4 GiB apart."""
+    N, K, R, G, M = 64, 64, 8, 3, 5
+    gap = (2 ** 31 + 2 ** 20) // 2                         # elements between adapters: the third starts behind 4 GiB
+    big = torch.empty(2 * gap + N * K, dtype=torch.bfloat16, device="cuda")
+    t = make(M, N, K, R, G, torch.bfloat16, 90, torch.tensor([2, 0, 1, 2, -1]))
+    down = big.as_strided((G, R, K), (gap, K, 1))
+    down.copy_(t["down"])
+    plan = gk.LoraPlan(t["ids"], G)
+    C = gk.gemm_lora(t["A"], t["B"], down, t["up"], plan, scale=t["scale"])
+    res, tol = want(t)
+    check("C", C, res, tol)
+    up = big.as_strided((G, N, R), (gap, R, 1))
+    up.copy_(t["up"])
+    C = gk.gemm_lora(t["A"], t["B"], t["down"], up, plan, scale=t["scale"])
+    check("C", C, res, tol)
+    grads = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], up, plan, scale=t["scale"])
+    for name, value in zip(("dA", "d_down", "d_up"), grads):
+        check(name, value, res, tol)

@@ -1,0 +1,157 @@
+"""Adapter entry points without a GPU: the C ABI and the binding refuse bad arguments before they touch CUDA."""
+import ctypes
+
+import pytest
+import torch
+
+from conftest import load_capi
+
+I, L, P, Z, F = ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_float
+
+
+class LoraArgs(ctypes.Structure):
+    _fields_ = [("M", I), ("N", I), ("K", I), ("R", I), ("adapters", I), ("dtype", I), ("A", P), ("B", P), ("down", P),
+                ("up", P), ("lda", L), ("ldb", L), ("ld_down", L), ("stride_down", L), ("ld_up", L), ("stride_up", L),
+                ("scales", P), ("scale", F), ("plan", P)]
+
+
+def good(**changes):
+    """A call that would be accepted; the addresses are never followed because every test breaks something."""
+    values = dict(M=32, N=64, K=128, R=16, adapters=4, dtype=0, A=0x1000, B=0x2000, down=0x3000, up=0x4000, lda=128, ldb=128,
+                  ld_down=128, stride_down=16 * 128, ld_up=16, stride_up=64 * 16, scales=None, scale=1.0, plan=0x5000)
+    values.update(changes)
+    return LoraArgs(**values)
+
+
+@pytest.fixture(scope="module")
+def lora():
+    lib = load_capi()
+    lib.gemm_sm100_lora_plan_bytes.argtypes, lib.gemm_sm100_lora_plan_bytes.restype = [I, I], Z
+    lib.gemm_sm100_lora_plan.argtypes = [P, I, I, I, P, Z, P, ctypes.POINTER(I)]
+    lib.gemm_sm100_lora_low.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, ctypes.POINTER(I)]
+    lib.gemm_sm100_lora.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, L, P, ctypes.POINTER(I)]
+    lib.gemm_sm100_lora_backward.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, L, P, L, P, L, P, P, P, ctypes.POINTER(I)]
+    return lib
+
+
+NULL, SHAPE, ALIGN, DTYPE, WORKSPACE = 1, 2, 3, 4, 7
+
+COMMON = [
+    (dict(M=-1), SHAPE), (dict(N=0), SHAPE), (dict(K=0), SHAPE), (dict(K=124, lda=128), SHAPE), (dict(R=0), SHAPE),
+    (dict(R=12), SHAPE), (dict(R=136), SHAPE), (dict(adapters=0), SHAPE), (dict(adapters=4097), SHAPE), (dict(dtype=2), DTYPE),
+    (dict(plan=None), NULL),
+]
+FORWARD = COMMON + [
+    (dict(A=None), NULL), (dict(B=None), NULL), (dict(down=None), NULL), (dict(up=None), NULL),
+    (dict(A=0x1008), ALIGN), (dict(B=0x2002), ALIGN), (dict(down=0x3004), ALIGN), (dict(up=0x4008), ALIGN),
+    (dict(lda=120), SHAPE), (dict(ldb=64), SHAPE), (dict(ld_down=64), SHAPE), (dict(ld_up=8), SHAPE),
+    (dict(lda=132), ALIGN), (dict(ld_up=20), ALIGN), (dict(stride_down=16 * 128 - 8), SHAPE), (dict(stride_up=0), SHAPE),
+    (dict(stride_down=16 * 128 + 4), ALIGN), (dict(stride_up=64 * 16 + 2), ALIGN),
+]
+
+
+@pytest.mark.parametrize("changes,want", FORWARD)
+def test_forward_refuses(lora, changes, want):
+    err = I(-7)
+    assert lora.gemm_sm100_lora(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, None, ctypes.byref(err)) == want
+    assert err.value == 0
+
+
+@pytest.mark.parametrize("C,ldc,low,ld_low,want", [
+    (None, 64, 0x7000, 16, NULL), (0x6000, 64, None, 16, NULL), (0x6000, 56, 0x7000, 16, SHAPE), (0x6000, 64, 0x7000, 8, SHAPE),
+    (0x6004, 64, 0x7000, 16, ALIGN), (0x6000, 64, 0x7008, 16, ALIGN), (0x6000, 68, 0x7000, 16, ALIGN), (0x6000, 64, 0x7000, 20, ALIGN)])
+def test_forward_refuses_outputs(lora, C, ldc, low, ld_low, want):
+    err = I(0)
+    assert lora.gemm_sm100_lora(ctypes.byref(good()), C, ldc, low, ld_low, None, ctypes.byref(err)) == want
+
+
+@pytest.mark.parametrize("changes,want", COMMON + [(dict(N=60, stride_up=60 * 16), SHAPE), (dict(up=None), NULL), (dict(B=None), NULL),
+                                                   (dict(down=None), NULL), (dict(A=None), NULL)])
+def test_backward_refuses(lora, changes, want):
+    err = I(-7)
+    rc = lora.gemm_sm100_lora_backward(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, 0x8000, 16, 0x9000, 128, 0xA000,
+                                       0xB000, None, ctypes.byref(err))
+    assert rc == want and err.value == 0
+
+
+@pytest.mark.parametrize("dC,ld_dc,low,d_low,dA,ld_da,d_down,d_up,want", [
+    (None, 64, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB000, NULL), (0x6000, 56, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB000, SHAPE),
+    (0x6000, 64, None, 0x8000, 0x9000, 128, 0xA000, 0xB000, NULL), (0x6000, 64, 0x7000, None, 0x9000, 128, 0xA000, 0xB000, NULL),
+    (0x6000, 64, 0x7000, 0x8000, 0x9000, 120, 0xA000, 0xB000, SHAPE), (0x6000, 64, 0x7000, 0x8000, 0x9000, 128, 0xA004, 0xB000, ALIGN),
+    (0x6000, 64, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB008, ALIGN), (0x6002, 64, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB000, ALIGN)])
+def test_backward_refuses_tensors(lora, dC, ld_dc, low, d_low, dA, ld_da, d_down, d_up, want):
+    err = I(0)
+    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), dC, ld_dc, low, 16, d_low, 16, dA, ld_da, d_down, d_up, None,
+                                         ctypes.byref(err)) == want
+
+
+def test_calls_with_nothing_to_do(lora):
+    err = I(0)
+    assert lora.gemm_sm100_lora(ctypes.byref(good(M=0, A=None, plan=None)), None, 64, None, 16, None, ctypes.byref(err)) == 0
+    assert lora.gemm_sm100_lora_low(ctypes.byref(good(M=0)), None, 16, None, ctypes.byref(err)) == 0
+    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), None, 64, None, 16, None, 16, None, 128, None, None, None,
+                                         ctypes.byref(err)) == 0
+    assert lora.gemm_sm100_lora(None, None, 0, None, 0, None, ctypes.byref(err)) == NULL
+
+
+def test_plan_arguments(lora):
+    assert lora.gemm_sm100_lora_plan_bytes(-1, 4) == 0 and lora.gemm_sm100_lora_plan_bytes(4, 0) == 0
+    assert lora.gemm_sm100_lora_plan_bytes(4, 4097) == 0
+    need = lora.gemm_sm100_lora_plan_bytes(300, 7)
+    # two tiles of 256 slots (adapter and mask), two lists of the rows, starts of the adapters
+    assert need >= 4 * (2 * 256 * 9 + 2 * 300 + 8) and need % 256 == 0
+    err = I(0)
+    plan = lambda *a: lora.gemm_sm100_lora_plan(*a, None, ctypes.byref(err))  # noqa: E731
+    assert plan(0x1000, 0, 300, 7, 0x2000, need - 1) == WORKSPACE
+    assert plan(0x1000, 0, 300, 7, 0x2010, need) == WORKSPACE
+    assert plan(0x1002, 0, 300, 7, 0x2000, need) == ALIGN
+    assert plan(0x1004, 1, 300, 7, 0x2000, need) == ALIGN
+    assert plan(None, 0, 300, 7, 0x2000, need) == NULL and plan(0x1000, 0, 300, 7, None, need) == NULL
+    assert plan(0x1000, 0, -1, 7, 0x2000, need) == SHAPE and plan(0x1000, 0, 300, 0, 0x2000, need) == SHAPE
+
+
+def tensors(M=32, N=64, K=128, R=16, G=4, dt=torch.bfloat16):
+    z = lambda *s: torch.zeros(*s, dtype=dt)  # noqa: E731
+    return dict(A=z(M, K), B=z(N, K), down=z(G, R, K), up=z(G, N, R), plan=torch.zeros(8, dtype=torch.uint8), plan_rows=M,
+                plan_adapters=G, scales=None, scale=1.0, C=z(M, N), low=z(M, R))
+
+
+Z16 = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+
+
+@pytest.mark.parametrize("changes,message", [
+    (dict(A=Z16(128)), "2D"), (dict(down=Z16(16, 128)), "3D"), (dict(B=Z16(64, 120)), "Inner dimensions"),
+    (dict(B=torch.zeros(64, 128)), "same dtype"), (dict(up=Z16(4, 64, 8)), "up must be of shape"),
+    (dict(up=Z16(3, 64, 16)), "up must be of shape"), (dict(down=Z16(4, 16, 120)), "down must be of shape"),
+    (dict(plan_rows=31), "31 rows"), (dict(plan_adapters=5), "5 adapters"), (dict(C=Z16(32, 72)), "out must be of shape"),
+    (dict(low=Z16(32, 8)), "low must be of shape"), (dict(A=Z16(32, 256)[:, ::2]), "unit stride"),
+    (dict(scales=torch.ones(3)), "scale must be"), (dict(scales=torch.ones(4, dtype=torch.float64)), "scale must be"),
+    (dict(), "CUDA tensors")])
+def test_binding_refuses(changes, message):
+    import gemm_kernels as gk
+
+    with pytest.raises(RuntimeError, match=message):
+        gk._C.gemm_lora(**{**tensors(), **changes})
+
+
+def test_binding_refuses_other_shapes_and_types():
+    import gemm_kernels as gk
+
+    with pytest.raises(RuntimeError, match="bfloat16 or float16"):
+        gk._C.gemm_lora(**tensors(dt=torch.float32))
+    with pytest.raises(RuntimeError, match="rank must be"):
+        gk._C.gemm_lora(**tensors(R=12))
+    with pytest.raises(RuntimeError, match="rank must be"):
+        gk._C.gemm_lora(**tensors(R=136))
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        gk._C.gemm_lora(**tensors(K=124))
+    with pytest.raises(ValueError, match="1D"):
+        gk.LoraPlan(torch.zeros(3, 3, dtype=torch.int32), 4)
+    with pytest.raises(ValueError, match="num_adapters"):
+        gk.LoraPlan(torch.zeros(3, dtype=torch.int32), 0)
+    with pytest.raises(ValueError, match="CUDA"):
+        gk.LoraPlan(torch.zeros(3, dtype=torch.int32), 4)
+    with pytest.raises(RuntimeError, match="int32 or int64"):
+        gk._C.lora_plan(torch.zeros(3, dtype=torch.int16), 4, torch.zeros(8, dtype=torch.uint8))
+    with pytest.raises(RuntimeError, match="contiguous"):
+        gk._C.lora_plan(torch.zeros(6, dtype=torch.int32)[::2], 4, torch.zeros(8, dtype=torch.uint8))
