@@ -180,7 +180,7 @@ struct LowConfig {
 };
 
 template <bool kIsBf16, bool kRankInner, bool kDeep>
-__global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __grid_constant__ LowParams p) {
+__device__ __forceinline__ void lora_low_body(const LowParams& p, const int block) {
   using Cfg = LowConfig<kDeep>;
   constexpr int kStages = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __gr
   uint32_t splits_reg;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits_reg));
   const int splits = static_cast<int>(splits_reg);
-  const int unit = static_cast<int>(blockIdx.x) / splits;
+  const int unit = block / splits;
   const int tile = unit / p.groups, group0 = unit % p.groups;
   WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
 
@@ -380,6 +380,22 @@ __global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __gr
     tc_fence_after_sync();
     tmem_dealloc<1>(tmem, Cfg::kTmemCols);
   }
+}
+
+template <bool kIsBf16, bool kRankInner, bool kDeep>
+__global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __grid_constant__ LowParams p) {
+  lora_low_body<kIsBf16, kRankInner, kDeep>(p, static_cast<int>(blockIdx.x));
+}
+
+// Both kinds of rows in one launch, for a backward pass that computes the low rows again: the first `blocks` CTAs
+// low, the others d_low.
+template <bool kIsBf16, bool kDeep>
+__global__ void __launch_bounds__(192, kDeep ? 1 : 2)
+lora_low_pair_kernel(const __grid_constant__ LowParams low, const __grid_constant__ LowParams d_low, const int blocks) {
+  if (static_cast<int>(blockIdx.x) < blocks)
+    lora_low_body<kIsBf16, false, kDeep>(low, static_cast<int>(blockIdx.x));
+  else
+    lora_low_body<kIsBf16, true, kDeep>(d_low, static_cast<int>(blockIdx.x) - blocks);
 }
 
 // ------------------------------------------------------------------------------ adapters' gradients

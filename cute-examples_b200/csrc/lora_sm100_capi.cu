@@ -233,9 +233,9 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
 }
 
 // Launch in clusters of `cluster` CTAs; a programmatic dependent of the kernel before it like the GEMM's kernels.
-template <class Kernel, class Params>
+template <class Kernel, class... Params>
 cudaError_t launch_cluster(Kernel kernel, long ctas, int cluster, int threads, int smem_bytes, cudaStream_t stream,
-                           const Params& params) {
+                           const Params&... params) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -250,7 +250,7 @@ cudaError_t launch_cluster(Kernel kernel, long ctas, int cluster, int threads, i
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
   cfg.numAttrs = g_opt_pdl.load() != 0 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, params);
+  return cudaLaunchKernelEx(&cfg, kernel, params...);
 }
 
 // The dynamic shared-memory limit of a kernel, set once per device.
@@ -268,28 +268,21 @@ cudaError_t allow_low(DeviceState& st) {
   static bool allowed[kMaxDevices];
   return allow_smem(lora_low_kernel<kIsBf16, kRankInner, kDeep>, LowConfig<kDeep>::kSmemBytes, allowed, st.device);
 }
-
-template <bool kIsBf16, bool kRankInner, bool kDeep>
-int launch_low_kernel(const LowParams& p, long ctas, int splits, DeviceState& st, cudaStream_t stream, int* cuda_error_out) {
-  using Cfg = LowConfig<kDeep>;
-  cudaError_t e = allow_low<kIsBf16, kRankInner, kDeep>(st);
-  if (e == cudaSuccess) e = launch_cluster(lora_low_kernel<kIsBf16, kRankInner, kDeep>, ctas, splits, Cfg::kThreads, Cfg::kSmemBytes, stream, p);
-  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+template <bool kIsBf16, bool kDeep>
+cudaError_t allow_low_pair(DeviceState& st) {
+  static bool allowed[kMaxDevices];
+  return allow_smem(lora_low_pair_kernel<kIsBf16, kDeep>, LowConfig<kDeep>::kSmemBytes, allowed, st.device);
 }
 
-// low rows of P [M, L] through W: down [adapters, R, L], or (kRankInner) up [adapters, L, R].
-template <bool kIsBf16, bool kRankInner>
-int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
-               long ld_out, cudaStream_t stream, int* cuda_error_out) {
-  DeviceState* st = nullptr;
-  int rc = ready(&st, cuda_error_out);
-  if (rc != GEMM_SM100_OK) return rc;
-  LowParams p;
+// Parameters of the low-rank rows of P [M, L] through W: down [adapters, R, L], or (rank_inner) up [adapters, L, R].
+int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_inner, const void* P, long ldp, const void* W,
+               long ld_w, long stride_w, int L, void* out, long ld_out, const DeviceState& st, int* cuda_error_out) {
+  LowParams& p = *out_params;
   std::memset(&p, 0, sizeof(p));
   p.p_rows = a.M >= 128 ? 128 : static_cast<int>(ceil_div(a.M, 8) * 8);
-  rc = encode_rows(&p.tmap_p, P, a.dtype, 2, {L, a.M, 1}, {ldp, 0}, {64, p.p_rows, 1}, cuda_error_out);
+  int rc = encode_rows(&p.tmap_p, P, a.dtype, 2, {L, a.M, 1}, {ldp, 0}, {64, p.p_rows, 1}, cuda_error_out);
   if (rc) return rc;
-  rc = kRankInner ? encode_rows(&p.tmap_w, W, a.dtype, 3, {a.R, L, a.adapters}, {ld_w, stride_w}, {rank_chunk(a.R), 64, 1},
+  rc = rank_inner ? encode_rows(&p.tmap_w, W, a.dtype, 3, {a.R, L, a.adapters}, {ld_w, stride_w}, {rank_chunk(a.R), 64, 1},
                                 cuda_error_out)
                   : encode_rows(&p.tmap_w, W, a.dtype, 3, {L, a.R, a.adapters}, {ld_w, stride_w}, {64, a.R, 1}, cuda_error_out);
   if (rc) return rc;
@@ -299,29 +292,94 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   p.out = out;
   p.ld_out = ld_out;
   p.M = a.M, p.R = a.R, p.L = L;
-  p.group_slots = 128 / (kRankInner ? static_cast<int>(ceil_div(a.R, rank_chunk(a.R))) * rank_chunk(a.R) : a.R);
-  p.status = st->status_ptr;
+  p.group_slots = 128 / (rank_inner ? static_cast<int>(ceil_div(a.R, rank_chunk(a.R))) * rank_chunk(a.R) : a.R);
+  p.status = st.status_ptr;
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
+  return GEMM_SM100_OK;
+}
 
-  // Two CTAs fit on an SM.  L is cut over as many CTAs of a cluster as leave them all at work at once;
-  // what is free beyond that takes groups of adapters of the same tile (how many a tile really has is
-  // known on the device only: a CTA without a group has nothing to do).
-  const long tiles = ceil_div(a.M, 128), room = 2L * st->sm_count, k_blocks = ceil_div(L, 64);
-  int splits = 8;
-  while (splits > 1 && (tiles * splits > room || splits > k_blocks)) splits /= 2;
-  const long most_slots = a.adapters < (a.M < kLoraTileRows ? a.M : kLoraTileRows) ? a.adapters
-                                                                                 : (a.M < kLoraTileRows ? a.M : kLoraTileRows);
-  const long most_groups = ceil_div(most_slots, p.group_slots);
-  long groups = room / (tiles * splits);
-  groups = groups < 1 ? 1 : (groups > most_groups ? most_groups : groups);
-  p.groups = static_cast<int>(groups);
+// CTAs of a launch.  Two fit on an SM.  L is cut over as many CTAs of a cluster as leave them all at work at once;
+// what is free beyond that takes groups of adapters of the same tile (how many a tile really has is
+// known on the device only: a CTA without a group has nothing to do).  `problems`: how many share the launch.
+struct LowGrid {
+  long tiles;
+  int splits;
+  bool deep;
+};
+LowGrid low_grid(LowParams* const* params, int problems, int adapters, const DeviceState& st) {
+  const int M = params[0]->M;
+  LowGrid g;
+  g.tiles = ceil_div(M, 128);
+  const long room = 2L * st.sm_count / problems;
+  long k_blocks = ceil_div(params[0]->L, 64), shortest = k_blocks;
+  for (int i = 1; i < problems; ++i) {
+    const long k = ceil_div(params[i]->L, 64);
+    if (k > k_blocks) k_blocks = k;
+    if (k < shortest) shortest = k;
+  }
+  g.splits = 8;
+  while (g.splits > 1 && (g.tiles * g.splits > room || g.splits > shortest)) g.splits /= 2;
+  const long most_slots = adapters < (M < kLoraTileRows ? M : kLoraTileRows) ? adapters : (M < kLoraTileRows ? M : kLoraTileRows);
+  long busy = 0;
+  for (int i = 0; i < problems; ++i) {
+    const long most_groups = ceil_div(most_slots, params[i]->group_slots);
+    long groups = room / (g.tiles * g.splits);
+    groups = groups < 1 ? 1 : (groups > most_groups ? most_groups : groups);
+    params[i]->groups = static_cast<int>(groups);
+    busy += g.tiles * g.splits * (groups < 2 ? groups : 2);
+  }
   // The deep ring for long runs of K blocks, when that leaves no SM with two CTAs, or hardly (every further group may turn
   // out to be empty): 64 x 4096 x 14336 with 32 adapters of rank 64 takes 45.8 us that way, 49.2 with the short ring.  With few
   // K blocks the SMs it takes from the product kernel behind cost more: 128 x 14336 x 4096 with 64 adapters of
   // rank 16 takes 44.6 us deep and 40.7 short (8 blocks per CTA).
-  const bool deep = k_blocks >= 12L * splits && tiles * splits * (groups < 2 ? groups : 2) <= st->sm_count;
-  return deep ? launch_low_kernel<kIsBf16, kRankInner, true>(p, tiles * groups * splits, splits, *st, stream, cuda_error_out)
-              : launch_low_kernel<kIsBf16, kRankInner, false>(p, tiles * groups * splits, splits, *st, stream, cuda_error_out);
+  g.deep = k_blocks >= 12L * g.splits && busy <= st.sm_count;
+  return g;
+}
+
+template <bool kIsBf16, bool kRankInner>
+int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
+               long ld_out, cudaStream_t stream, int* cuda_error_out) {
+  DeviceState* st = nullptr;
+  int rc = ready(&st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  LowParams p;
+  rc = low_params(&p, a, kRankInner, P, ldp, W, ld_w, stride_w, L, out, ld_out, *st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  LowParams* const one[1] = {&p};
+  const LowGrid g = low_grid(one, 1, a.adapters, *st);
+  const long ctas = g.tiles * p.groups * g.splits;
+  cudaError_t e = g.deep ? allow_low<kIsBf16, kRankInner, true>(*st) : allow_low<kIsBf16, kRankInner, false>(*st);
+  if (e == cudaSuccess)
+    e = g.deep ? launch_cluster(lora_low_kernel<kIsBf16, kRankInner, true>, ctas, g.splits, LowConfig<true>::kThreads,
+                                LowConfig<true>::kSmemBytes, stream, p)
+               : launch_cluster(lora_low_kernel<kIsBf16, kRankInner, false>, ctas, g.splits, LowConfig<false>::kThreads,
+                                LowConfig<false>::kSmemBytes, stream, p);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+}
+
+// low (from A and down) and d_low (from dC and up) in one launch.
+template <bool kIsBf16>
+int launch_low_pair(const gemm_sm100_lora_args& a, void* low, long ld_low, const void* dC, long ld_dc, void* d_low, long ld_d_low,
+                    cudaStream_t stream, int* cuda_error_out) {
+  DeviceState* st = nullptr;
+  int rc = ready(&st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  LowParams p, q;
+  rc = low_params(&p, a, false, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low, ld_low, *st, cuda_error_out);
+  if (rc == GEMM_SM100_OK)
+    rc = low_params(&q, a, true, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low, ld_d_low, *st, cuda_error_out);
+  if (rc != GEMM_SM100_OK) return rc;
+  LowParams* const both[2] = {&p, &q};
+  const LowGrid g = low_grid(both, 2, a.adapters, *st);
+  const int first = static_cast<int>(g.tiles * p.groups * g.splits);
+  const long ctas = first + g.tiles * q.groups * g.splits;
+  cudaError_t e = g.deep ? allow_low_pair<kIsBf16, true>(*st) : allow_low_pair<kIsBf16, false>(*st);
+  if (e == cudaSuccess)
+    e = g.deep ? launch_cluster(lora_low_pair_kernel<kIsBf16, true>, ctas, g.splits, LowConfig<true>::kThreads,
+                                LowConfig<true>::kSmemBytes, stream, p, q, first)
+               : launch_cluster(lora_low_pair_kernel<kIsBf16, false>, ctas, g.splits, LowConfig<false>::kThreads,
+                                LowConfig<false>::kSmemBytes, stream, p, q, first);
+  return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
 template <bool kIsBf16, int kRanks>
@@ -392,6 +450,8 @@ int prepare_type(DeviceState& st, int* cuda_error_out, std::integer_sequence<int
   if (e == cudaSuccess) e = allow_low<kIsBf16, false, true>(st);
   if (e == cudaSuccess) e = allow_low<kIsBf16, true, false>(st);
   if (e == cudaSuccess) e = allow_low<kIsBf16, true, true>(st);
+  if (e == cudaSuccess) e = allow_low_pair<kIsBf16, false>(st);
+  if (e == cudaSuccess) e = allow_low_pair<kIsBf16, true>(st);
   if (e == cudaSuccess) e = allow_grad<kIsBf16, 16>(st);
   if (e == cudaSuccess) e = allow_grad<kIsBf16, 32>(st);
   if (e == cudaSuccess) e = allow_grad<kIsBf16, 64>(st);
@@ -467,8 +527,8 @@ int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* l
       p, o, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
 }
 
-int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, const void* low, long ld_low,
-                             void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up, void* cuda_stream,
+int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, void* low, long ld_low,
+                             int recompute_low, void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up, void* cuda_stream,
                              int* cuda_error_out) {
   if (cuda_error_out) *cuda_error_out = 0;
   if (!args) return GEMM_SM100_ERR_NULL_POINTER;
@@ -492,12 +552,20 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
   if (d_up && (rc = check_matrix(low, a.R, ld_low))) return rc;
   if (dA && ((rc = check_matrix(a.B, a.K, a.ldb)) || (rc = check_down(a)) || (rc = check_matrix(dA, a.K, ld_da)))) return rc;
   const bool bf16 = a.dtype == GEMM_SM100_BF16;
+  const bool again = recompute_low != 0 && d_up != nullptr;
+  if (again && ((rc = check_matrix(a.A, a.K, a.lda)) || (rc = check_down(a)))) return rc;
   if (dA || d_down) {
     if ((rc = check_up(a)) || (rc = check_matrix(d_low, a.R, ld_d_low))) return rc;
-    rc = (bf16 ? launch_low<true, true> : launch_low<false, true>)(a, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low,
-                                                                   ld_d_low, stream, cuda_error_out);
-    if (rc != GEMM_SM100_OK) return rc;
+    if (again)
+      rc = (bf16 ? launch_low_pair<true> : launch_low_pair<false>)(a, low, ld_low, dC, ld_dc, d_low, ld_d_low, stream, cuda_error_out);
+    else
+      rc = (bf16 ? launch_low<true, true> : launch_low<false, true>)(a, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low,
+                                                                     ld_d_low, stream, cuda_error_out);
+  } else if (again) {
+    rc = (bf16 ? launch_low<true, false> : launch_low<false, false>)(a, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low,
+                                                                     ld_low, stream, cuda_error_out);
   }
+  if (rc != GEMM_SM100_OK) return rc;
   if (dA) {
     const Problem p{dC, a.B, dA, a.M, a.K, a.N, ld_dc, a.ldb, ld_da, a.dtype, /*b_is_kn=*/true};
     const AdapterOperands o{d_low, ld_d_low, a.down, a.ld_down, a.stride_down, a.R, a.adapters, a.plan};

@@ -268,76 +268,80 @@ void lora_placed(const torch::Tensor& A, const torch::Tensor& B, const torch::Te
 
 }  // namespace
 
+// The plan's memory belongs to the stream it was made on; for work on another one the allocator is told, so that the
+// memory is not handed out again while that work is queued.
+void hold_plan(const torch::Tensor& plan, int64_t made_on, const c10::cuda::CUDAStream& stream) {
+  if (reinterpret_cast<int64_t>(stream.stream()) != made_on) plan.record_stream(stream.unwrap());
+}
+
+// `out` and `low` undefined: allocated here.
 torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torch::Tensor down, const torch::Tensor up,
-                        const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters, const OptTensor scales,
-                        double scale, torch::Tensor C, torch::Tensor low) {
+                        const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters, int64_t plan_stream,
+                        const OptTensor scales, double scale, const OptTensor out, const OptTensor low_out) {
   const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
-  check_like(C, "out", A, {a.M, a.N});
-  check_like(low, "low", A, {a.M, a.R});
+  if (out.has_value()) check_like(*out, "out", A, {a.M, a.N});
+  if (low_out.has_value()) check_like(*low_out, "low", A, {a.M, a.R});
   lora_placed(A, B, down, up, plan, scales);
-  check_placed(C, "out", A);
-  check_placed(low, "low", A);
-  if (a.M == 0) return C;
+  if (out.has_value()) check_placed(*out, "out", A);
+  if (low_out.has_value()) check_placed(*low_out, "low", A);
   c10::cuda::CUDAGuard guard(A.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(A.device().index()).stream();
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(A.device().index());
+  // from the caching allocator: safe in stream order, and part of the graph's own memory under capture
+  torch::Tensor C = out.has_value() ? *out : torch::empty({a.M, a.N}, A.options());
+  if (a.M == 0) return C;
+  const torch::Tensor low = low_out.has_value() ? *low_out : torch::empty({a.M, a.R}, A.options());
+  hold_plan(plan, plan_stream, stream);
   int cuda_error = 0;
   int rc;
   {
     pybind11::gil_scoped_release release;
-    rc = gemm_sm100_lora(&a, C.mutable_data_ptr(), pitch(C), low.mutable_data_ptr(), pitch(low), static_cast<void*>(stream),
-                         &cuda_error);
+    rc = gemm_sm100_lora(&a, C.mutable_data_ptr(), pitch(C), low.mutable_data_ptr(), pitch(low),
+                         static_cast<void*>(stream.stream()), &cuda_error);
   }
   raise_for(rc, cuda_error, "gemm_lora");
   return C;
 }
 
-// `low` undefined: the low-rank rows are computed again.  dA, d_down, d_up undefined: not wanted.
-void gemm_lora_backward(const torch::Tensor dC, const torch::Tensor A, const torch::Tensor B, const torch::Tensor down,
-                        const torch::Tensor up, const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters,
-                        const OptTensor scales, double scale, const OptTensor low, const OptTensor dA,
-                        const OptTensor d_down, const OptTensor d_up) {
+// `low` undefined: the low-rank rows are computed again.  Returns dA, d_down and d_up, undefined where not needed.
+std::vector<OptTensor> gemm_lora_backward(const torch::Tensor dC, const torch::Tensor A, const torch::Tensor B,
+                                          const torch::Tensor down, const torch::Tensor up, const torch::Tensor plan,
+                                          int64_t plan_rows, int64_t plan_adapters, int64_t plan_stream, const OptTensor scales,
+                                          double scale, const OptTensor low, bool need_a, bool need_down, bool need_up) {
   const gemm_sm100_lora_args a = lora_args(A, B, down, up, plan, plan_rows, plan_adapters, scales, scale);
   TORCH_CHECK(dC.dim() == 2, "dC must be a 2D (matrix) tensor");
   check_like(dC, "dC", A, {a.M, a.N});
   TORCH_CHECK(a.N % 8 == 0, "N must be a multiple of 8 (it is the inner dimension of dC * B), got ", a.N);
   if (low.has_value()) check_like(*low, "low", A, {a.M, a.R});
-  if (dA.has_value()) check_like(*dA, "dA", A, {a.M, a.K});
-  if (d_down.has_value()) check_like(*d_down, "d_down", A, {a.adapters, a.R, a.K}, true);
-  if (d_up.has_value()) check_like(*d_up, "d_up", A, {a.adapters, a.N, a.R}, true);
   lora_placed(A, B, down, up, plan, scales);
   check_placed(dC, "dC", A);
   if (low.has_value()) check_placed(*low, "low", A);
-  if (dA.has_value()) check_placed(*dA, "dA", A);
-  if (d_down.has_value()) check_placed(*d_down, "d_down", A);
-  if (d_up.has_value()) check_placed(*d_up, "d_up", A);
   c10::cuda::CUDAGuard guard(A.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(A.device().index()).stream();
-  // scratch from the caching allocator: safe in stream order, and part of the graph's own memory under capture
-  const auto options = torch::TensorOptions().dtype(A.scalar_type()).device(A.device());
-  torch::Tensor d_low, low_rows;
-  if (dA.has_value() || d_down.has_value()) d_low = torch::empty({a.M, a.R}, options);
-  int cuda_error = 0;
-  int rc = GEMM_SM100_OK;
-  const char* what = "gemm_lora_backward";
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(A.device().index());
+  const auto options = A.options();
+  torch::Tensor dA, d_down, d_up, d_low, low_rows;
+  if (need_a) dA = torch::empty({a.M, a.K}, options);
+  if (need_down) d_down = torch::empty({a.adapters, a.R, a.K}, options);
+  if (need_up) d_up = torch::empty({a.adapters, a.N, a.R}, options);
+  if (need_a || need_down) d_low = torch::empty({a.M, a.R}, options);
   if (low.has_value()) {
     low_rows = *low;
-  } else if (d_up.has_value()) {
+  } else if (need_up) {
     low_rows = torch::empty({a.M, a.R}, options);
   }
+  hold_plan(plan, plan_stream, stream);
+  auto address = [](const torch::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+  int cuda_error = 0;
+  int rc;
   {
     pybind11::gil_scoped_release release;
-    if (!low.has_value() && d_up.has_value())
-      rc = gemm_sm100_lora_low(&a, low_rows.mutable_data_ptr(), a.R, static_cast<void*>(stream), &cuda_error);
-    if (rc == GEMM_SM100_OK)
-      rc = gemm_sm100_lora_backward(&a, dC.const_data_ptr(), pitch(dC), low_rows.defined() ? low_rows.const_data_ptr() : nullptr,
-                                    low_rows.defined() ? pitch(low_rows) : a.R,
-                                    d_low.defined() ? d_low.mutable_data_ptr() : nullptr, a.R,
-                                    dA.has_value() ? dA->mutable_data_ptr() : nullptr, dA.has_value() ? pitch(*dA) : a.K,
-                                    d_down.has_value() ? d_down->mutable_data_ptr() : nullptr,
-                                    d_up.has_value() ? d_up->mutable_data_ptr() : nullptr, static_cast<void*>(stream),
-                                    &cuda_error);
+    rc = gemm_sm100_lora_backward(&a, dC.const_data_ptr(), pitch(dC), address(low_rows),
+                                  low_rows.defined() ? pitch(low_rows) : a.R, low.has_value() ? 0 : 1, address(d_low), a.R,
+                                  address(dA), a.K, address(d_down), address(d_up), static_cast<void*>(stream.stream()),
+                                  &cuda_error);
   }
-  raise_for(rc, cuda_error, what);
+  raise_for(rc, cuda_error, "gemm_lora_backward");
+  auto optional = [](const torch::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+  return {optional(dA), optional(d_down), optional(d_up)};
 }
 
 // Waits for the current device and raises if a kernel reported a timed-out wait.
@@ -407,12 +411,12 @@ PYBIND11_MODULE(_C, m) {
   m.def("lora_plan_bytes", &gemm_sm100_lora_plan_bytes, pybind11::arg("M"), pybind11::arg("adapters"));
   m.def("gemm_lora", &gemm_lora, "C = A * B^T + low * up^T, low = scale * A * down^T with the adapter of each row",
         pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("down"), pybind11::arg("up"), pybind11::arg("plan"),
-        pybind11::arg("plan_rows"), pybind11::arg("plan_adapters"), pybind11::arg("scales"), pybind11::arg("scale"),
-        pybind11::arg("C"), pybind11::arg("low"));
+        pybind11::arg("plan_rows"), pybind11::arg("plan_adapters"), pybind11::arg("plan_stream"), pybind11::arg("scales"),
+        pybind11::arg("scale"), pybind11::arg("out"), pybind11::arg("low"));
   m.def("gemm_lora_backward", &gemm_lora_backward, "Gradients of gemm_lora", pybind11::arg("dC"), pybind11::arg("A"),
         pybind11::arg("B"), pybind11::arg("down"), pybind11::arg("up"), pybind11::arg("plan"), pybind11::arg("plan_rows"),
-        pybind11::arg("plan_adapters"), pybind11::arg("scales"), pybind11::arg("scale"), pybind11::arg("low"),
-        pybind11::arg("dA"), pybind11::arg("d_down"), pybind11::arg("d_up"));
+        pybind11::arg("plan_adapters"), pybind11::arg("plan_stream"), pybind11::arg("scales"), pybind11::arg("scale"),
+        pybind11::arg("low"), pybind11::arg("need_a"), pybind11::arg("need_down"), pybind11::arg("need_up"));
   m.def("device_status", &device_status,
         "Synchronise the current device and raise if a GEMM kernel reported a failed wait");
   m.def("init", &init, "One-time set-up of the current device; call before capturing a CUDA graph");

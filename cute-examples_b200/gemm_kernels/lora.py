@@ -38,22 +38,17 @@ class LoraPlan:
         self.rows = ids.shape[0]
         self.num_adapters = num_adapters
         self.buffer = torch.empty(_C.lora_plan_bytes(self.rows, num_adapters), dtype=torch.uint8, device=ids.device)
-        self._stream = torch.cuda.current_stream(ids.device)
+        self.stream = torch.cuda.current_stream(ids.device).cuda_stream   # the memory's own stream
         _C.lora_plan(ids, num_adapters, self.buffer)
 
     def update(self, ids: torch.Tensor) -> "LoraPlan":
         if ids.dim() != 1 or ids.shape[0] != self.rows:
             raise ValueError(f"the plan is for {self.rows} rows, ids has shape {tuple(ids.shape)}")
-        self._hold()
+        stream = torch.cuda.current_stream(self.buffer.device)
+        if stream.cuda_stream != self.stream:
+            self.buffer.record_stream(stream)
         _C.lora_plan(ids, self.num_adapters, self.buffer)
         return self
-
-    def _hold(self) -> torch.Tensor:
-        """The plan's memory for use on the current stream, kept from reuse until that work is done."""
-        stream = torch.cuda.current_stream(self.buffer.device)
-        if stream != self._stream:
-            self.buffer.record_stream(stream)
-        return self.buffer
 
 
 def _scales(scale) -> tuple[torch.Tensor | None, float]:
@@ -70,12 +65,8 @@ def gemm_lora(A: torch.Tensor, B: torch.Tensor, down: torch.Tensor, up: torch.Te
     value per adapter.  ``low`` (``[M,R]``) receives the scaled low-rank rows, which the backward pass
     can use again.  ``out`` may have a row pitch (a multiple of 8 elements).
     """
-    if out is None:
-        out = torch.empty((A.shape[0], B.shape[0]), dtype=A.dtype, device=A.device)
-    if low is None:
-        low = torch.empty((A.shape[0], down.shape[-2]), dtype=A.dtype, device=A.device)
     scales, factor = _scales(scale)
-    return _C.gemm_lora(A, B, down, up, plan._hold(), plan.rows, plan.num_adapters, scales, factor, out, low)
+    return _C.gemm_lora(A, B, down, up, plan.buffer, plan.rows, plan.num_adapters, plan.stream, scales, factor, out, low)
 
 
 def gemm_lora_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
@@ -86,10 +77,6 @@ def gemm_lora_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, down:
     ``low`` is what `gemm_lora` was given (computed again when None).  Entries of ``needs`` that are
     False come back as None and are not computed.  Adapters without rows get zeros.
     """
-    dA = torch.empty_like(A, memory_format=torch.contiguous_format) if needs[0] else None
-    d_down = torch.empty_like(down, memory_format=torch.contiguous_format) if needs[1] else None
-    d_up = torch.empty_like(up, memory_format=torch.contiguous_format) if needs[2] else None
     scales, factor = _scales(scale)
-    _C.gemm_lora_backward(dC, A, B, down, up, plan._hold(), plan.rows, plan.num_adapters, scales, factor, low, dA, d_down,
-                          d_up)
-    return dA, d_down, d_up
+    return tuple(_C.gemm_lora_backward(dC, A, B, down, up, plan.buffer, plan.rows, plan.num_adapters, plan.stream, scales,
+                                       factor, low, *needs))

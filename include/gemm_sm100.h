@@ -327,12 +327,13 @@ int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* l
                     int* cuda_error_out);
 
 /* Gradients from dC [M, N] (pitch ld_dc); N % 8 == 0.  dA [M, K] (pitch ld_da), d_down [adapters, R, K] and
- * d_up [adapters, N, R] (both contiguous) may each be NULL: it is then not computed.  `low` is what the
- * forward pass (or gemm_sm100_lora_low) wrote, needed for d_up only; `d_low` [M, R] (pitch ld_d_low)
- * is scratch, needed for dA and d_down.  With M == 0 the adapters' gradients are filled with zeros. */
-int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, const void* low, long ld_low,
-                             void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up, void* cuda_stream,
-                             int* cuda_error_out);
+ * d_up [adapters, N, R] (both contiguous) may each be NULL: it is then not computed.  `low` [M, R] (pitch ld_low),
+ * needed for d_up only, is what the forward pass (or gemm_sm100_lora_low) wrote, or with recompute_low
+ * non-zero scratch in which it is computed again.  `d_low` [M, R] (pitch ld_d_low) is scratch, needed for dA and
+ * d_down.  With M == 0 the adapters' gradients are filled with zeros. */
+int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, void* low, long ld_low,
+                             int recompute_low, void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up,
+                             void* cuda_stream, int* cuda_error_out);
 
 /* Static, human-readable name of a return code. */
 const char* gemm_sm100_error_string(int code);

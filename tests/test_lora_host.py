@@ -30,7 +30,7 @@ def lora():
     lib.gemm_sm100_lora_plan.argtypes = [P, I, I, I, P, Z, P, ctypes.POINTER(I)]
     lib.gemm_sm100_lora_low.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, ctypes.POINTER(I)]
     lib.gemm_sm100_lora.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, L, P, ctypes.POINTER(I)]
-    lib.gemm_sm100_lora_backward.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, L, P, L, P, L, P, P, P, ctypes.POINTER(I)]
+    lib.gemm_sm100_lora_backward.argtypes = [ctypes.POINTER(LoraArgs), P, L, P, L, I, P, L, P, L, P, P, P, ctypes.POINTER(I)]
     return lib
 
 
@@ -69,7 +69,7 @@ def test_forward_refuses_outputs(lora, C, ldc, low, ld_low, want):
                                                    (dict(down=None), NULL), (dict(A=None), NULL)])
 def test_backward_refuses(lora, changes, want):
     err = I(-7)
-    rc = lora.gemm_sm100_lora_backward(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, 0x8000, 16, 0x9000, 128, 0xA000,
+    rc = lora.gemm_sm100_lora_backward(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, 0, 0x8000, 16, 0x9000, 128, 0xA000,
                                        0xB000, None, ctypes.byref(err))
     assert rc == want and err.value == 0
 
@@ -81,7 +81,7 @@ def test_backward_refuses(lora, changes, want):
     (0x6000, 64, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB008, ALIGN), (0x6002, 64, 0x7000, 0x8000, 0x9000, 128, 0xA000, 0xB000, ALIGN)])
 def test_backward_refuses_tensors(lora, dC, ld_dc, low, d_low, dA, ld_da, d_down, d_up, want):
     err = I(0)
-    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), dC, ld_dc, low, 16, d_low, 16, dA, ld_da, d_down, d_up, None,
+    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), dC, ld_dc, low, 16, 0, d_low, 16, dA, ld_da, d_down, d_up, None,
                                          ctypes.byref(err)) == want
 
 
@@ -89,7 +89,7 @@ def test_calls_with_nothing_to_do(lora):
     err = I(0)
     assert lora.gemm_sm100_lora(ctypes.byref(good(M=0, A=None, plan=None)), None, 64, None, 16, None, ctypes.byref(err)) == 0
     assert lora.gemm_sm100_lora_low(ctypes.byref(good(M=0)), None, 16, None, ctypes.byref(err)) == 0
-    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), None, 64, None, 16, None, 16, None, 128, None, None, None,
+    assert lora.gemm_sm100_lora_backward(ctypes.byref(good()), None, 64, None, 16, 0, None, 16, None, 128, None, None, None,
                                          ctypes.byref(err)) == 0
     assert lora.gemm_sm100_lora(None, None, 0, None, 0, None, ctypes.byref(err)) == NULL
 
@@ -113,7 +113,7 @@ def test_plan_arguments(lora):
 def tensors(M=32, N=64, K=128, R=16, G=4, dt=torch.bfloat16):
     z = lambda *s: torch.zeros(*s, dtype=dt)  # noqa: E731
     return dict(A=z(M, K), B=z(N, K), down=z(G, R, K), up=z(G, N, R), plan=torch.zeros(8, dtype=torch.uint8), plan_rows=M,
-                plan_adapters=G, scales=None, scale=1.0, C=z(M, N), low=z(M, R))
+                plan_adapters=G, plan_stream=0, scales=None, scale=1.0, out=z(M, N), low=z(M, R))
 
 
 Z16 = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
@@ -123,7 +123,7 @@ Z16 = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
     (dict(A=Z16(128)), "2D"), (dict(down=Z16(16, 128)), "3D"), (dict(B=Z16(64, 120)), "Inner dimensions"),
     (dict(B=torch.zeros(64, 128)), "same dtype"), (dict(up=Z16(4, 64, 8)), "up must be of shape"),
     (dict(up=Z16(3, 64, 16)), "up must be of shape"), (dict(down=Z16(4, 16, 120)), "down must be of shape"),
-    (dict(plan_rows=31), "31 rows"), (dict(plan_adapters=5), "5 adapters"), (dict(C=Z16(32, 72)), "out must be of shape"),
+    (dict(plan_rows=31), "31 rows"), (dict(plan_adapters=5), "5 adapters"), (dict(out=Z16(32, 72)), "out must be of shape"),
     (dict(low=Z16(32, 8)), "low must be of shape"), (dict(A=Z16(32, 256)[:, ::2]), "unit stride"),
     (dict(scales=torch.ones(3)), "scale must be"), (dict(scales=torch.ones(4, dtype=torch.float64)), "scale must be"),
     (dict(), "CUDA tensors")])
@@ -155,3 +155,10 @@ def test_binding_refuses_other_shapes_and_types():
         gk._C.lora_plan(torch.zeros(3, dtype=torch.int16), 4, torch.zeros(8, dtype=torch.uint8))
     with pytest.raises(RuntimeError, match="contiguous"):
         gk._C.lora_plan(torch.zeros(6, dtype=torch.int32)[::2], 4, torch.zeros(8, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("changes,want", [(dict(A=None), NULL), (dict(down=None), NULL), (dict(down=0x3008), ALIGN)])
+def test_backward_refuses_what_recomputing_needs(lora, changes, want):
+    err = I(0)
+    assert lora.gemm_sm100_lora_backward(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, 1, None, 16, None, 128, None, 0xB000,
+                                         None, ctypes.byref(err)) == want
