@@ -223,7 +223,8 @@ struct GemmConfig {
 // Where the adapter kernels keep a segment's plan entries, behind the barriers.
 template <class Cfg>
 struct LoraConfig : Cfg {
-  static constexpr int kSmemBytes = Cfg::kSmemBytes + 256 + 32 * 32;
+  static constexpr int kEntryBytes = 16 + 32 * 16 + 16 + 32 * 32;   // producer: count, adapters; MMA issuer: count, row masks
+  static constexpr int kSmemBytes = Cfg::kSmemBytes + kEntryBytes;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
@@ -404,6 +405,8 @@ __device__ __forceinline__ TileCols tile_columns(int n_tile, const TileParams& p
 // issuing warp that waited for such a load in the middle of its loop left the tensor core idle for one to two
 // microseconds per load (8192 x 4096 x 4096, rank 16: 90 us more than without adapters), so the first 32 entries of
 // a segment are copied to shared memory while its K blocks run and picked up behind them.
+// All reads of the plan go to L2 (16-byte copies, __ldcg): they come before this kernel has waited for the one in front of
+// it, so this SM's L1 may still hold what a plan at the same address said to an earlier kernel.
 struct LoraWork {
   int stages, items, per_stage, part, factor;
   int base;                                // the tile's first slot in the plan
@@ -432,15 +435,15 @@ __device__ __forceinline__ LoraWork lora_begin(const LoraParams& lora, int m_til
   w.stages = w.items = 0;
   const int tile = Cfg::kCtaGroup == 2 ? m_tile : m_tile >> 1;
   w.base = tile * 256;
-  if (lane_id() == 0) cp_async_4(count_dst, lora.slot_count + tile);
+  if (lane_id() == 0) cp_async_16(count_dst, lora.slot_count + (tile & ~3), true);
   return w;
 }
 // The entries have arrived: how many stages they make.
-__device__ __forceinline__ void lora_resolve(LoraWork& w, const LoraParams& lora, uint32_t count_src) {
-  cp_async_wait<0>();
+__device__ __forceinline__ void lora_resolve(LoraWork& w, const LoraParams& lora, uint32_t count_src) {   // (lora_begin's)
+  cp_async_wait_all();
   __syncwarp();
   int count;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(count) : "r"(count_src) : "memory");
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(count) : "r"(count_src + (uint32_t)((w.base >> 8) & 3) * 4u) : "memory");
   w.items = count * lora.chunks;
   const int all = (w.items + w.per_stage - 1) / w.per_stage;
   const int stages = all > w.part ? (all - w.part + w.factor - 1) / w.factor : 0;
@@ -488,7 +491,7 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
     LoraWork lw = lora_begin<Cfg>(lora, m_tile, kSplitK ? seg.part : 0, kSplitK ? p.sk_factor : 1, ring.entries);
     {
       const int slot = lw.slot_of((int)lane, chunks);
-      if (slot < 256) cp_async_4(ring.entries + 16u + lane * 4u, lora.slot_adapter + lw.base + slot);
+      if (slot < 256) cp_async_16(ring.entries + 16u + lane * 16u, lora.slot_adapter + lw.base + (slot & ~3), true);
     }
 #pragma unroll 1
     for (int kb = seg.kb0; kb < seg.kb1; ++kb) {
@@ -521,7 +524,10 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
     }
     lora_resolve(lw, lora, ring.entries);
     int entry_adapter;                                   // lane i: adapter of entry i of the current 32
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(entry_adapter) : "r"(ring.entries + 16u + lane * 4u) : "memory");
+    asm volatile("ld.shared.b32 %0, [%1];"
+                 : "=r"(entry_adapter)
+                 : "r"(ring.entries + 16u + lane * 16u + (uint32_t)(lw.slot_of((int)lane, chunks) & 3) * 4u)
+                 : "memory");
     if (lw.stages > 0 && !low_ready) {
       grid_dependency_wait();
       low_ready = true;
@@ -532,7 +538,7 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
       const int items = min(lw.per_stage, lw.items - first);
       if (entry >= kLoraEntries && entry % kLoraEntries == 0) {
         const int slot = lw.slot_of(entry + (int)lane, chunks);
-        entry_adapter = slot < 256 ? lora.slot_adapter[lw.base + slot] : 0;
+        entry_adapter = slot < 256 ? __ldcg(lora.slot_adapter + lw.base + slot) : 0;
       }
       if (!wait_bounded(ring.empty + 8u * s, phase ^ 1u, ctx, kStatusTimeoutProducer + s)) return;
       const uint32_t full = full_leader + 8u * s, dst_a = ring.smem_a + s * Cfg::kABytes, dst_b = ring.smem_b + s * Cfg::kBBytes;
@@ -592,7 +598,7 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
   const uint64_t dl0 = make_smem_desc_rows(ring.smem_a, (uint32_t)chunk * 2u);
   const uint64_t dw0 = kBIsKN ? make_smem_desc_sw128_mn(ring.smem_b, (uint32_t)chunk * 128u)
                               : make_smem_desc_rows(ring.smem_b, (uint32_t)chunk * 2u);
-  const uint32_t count_smem = ring.entries + 160u, mask_smem = ring.entries + 256u;
+  const uint32_t count_smem = ring.entries + 16u + 32u * 16u, mask_smem = count_smem + 16u;
   uint32_t s = 0, phase = 0;
   int iter = 0;
   Segment seg;
@@ -658,7 +664,7 @@ __device__ __forceinline__ void lora_issue(const TileParams& p, const LoraParams
         const int slot = lw.slot_of(entry + (int)lane, chunks);
         if (slot < 256)
 #pragma unroll
-          for (int v = 0; v < G; ++v) entry_rows[v] = masks[2 * slot + v];
+          for (int v = 0; v < G; ++v) entry_rows[v] = __ldcg(masks + 2 * slot + v);
       }
       if (!wait_bounded(ring.full + 8u * s, phase, ctx, kStatusTimeoutMma + s)) return;
       tc_fence_after_sync();

@@ -567,3 +567,41 @@ def test_few_rows_under_the_own_plan(gk, M, N, K, R, G):
     gk.device_status()
     res, tol = want(t)
     check("C", C, res, tol)
+
+
+def test_plan_refilled_before_every_call(gk):
+    """A plan that changes in place just before the product reads it: a stale copy of the old plan, in some SM's cache,
+    would give wrong rows or leave the kernel's warps at odds about the number of adapters."""
+    M, N, K, R, G = 40, 8192, 256, 16, 40
+    t = make(M, N, K, R, G, torch.bfloat16, 120, id_pattern("own", M, G, 1))
+    patterns = [id_pattern("own", M, G, 1).cuda(), id_pattern("one", M, G, 1).cuda(), id_pattern("random", M, 5, 2).cuda(),
+                id_pattern("none", M, G, 1).cuda(), id_pattern("random", M, G, 3).cuda()]
+    wanted = []
+    for ids in patterns:
+        t["ids"] = ids
+        wanted.append(forward_only(gk, t))
+    res, tol = want(t)
+    check("C", wanted[-1], res, tol)
+    plan = gk.LoraPlan(patterns[0], G)
+    outs = [torch.empty(M, N, dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+    for step in range(0, 400, 8):
+        for i in range(8):
+            plan.update(patterns[(step + 3 * i) % 5])
+            gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], out=outs[i])
+        for i in range(8):
+            assert torch.equal(outs[i], wanted[(step + 3 * i) % 5]), (step, i)
+    gk.device_status()
+
+
+@pytest.mark.parametrize("M,N,K,R", [(5, 4096, 512, 16), (7, 20320, 320, 24), (3, 1024, 64, 8), (100, 512, 64, 16), (300, 776, 64, 24)])
+def test_short_main_loops_many_times(gk, M, N, K, R):
+    """A main loop of one or two ring stages: the plan's entries are needed almost at once.  Fresh plans and inputs
+    every time, as the first pass over a new batch has them."""
+    G = 9
+    for seed in range(40):
+        t = make(M, N, K, R, G, torch.bfloat16, 200 + seed, id_pattern("random", M, G, seed))
+        torch.empty(1 << 26, dtype=torch.uint8, device="cuda").fill_(seed)      # other data in the caches
+        C = forward_only(gk, t)
+        res, tol = want(t)
+        check("C", C, res, tol)
+    gk.device_status()
