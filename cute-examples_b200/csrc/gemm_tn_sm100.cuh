@@ -528,10 +528,6 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
                  : "=r"(entry_adapter)
                  : "r"(ring.entries + 16u + lane * 16u + (uint32_t)(lw.slot_of((int)lane, chunks) & 3) * 4u)
                  : "memory");
-    if (lw.stages > 0 && !low_ready) {
-      grid_dependency_wait();
-      low_ready = true;
-    }
 #pragma unroll 1
     for (int stage = 0; stage < lw.stages; ++stage) {
       const int first = (lw.part + stage * lw.factor) * lw.per_stage, entry = stage * lw.per_stage;
@@ -551,8 +547,6 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
         const int g = __shfl_sync(0xffffffffu, entry_adapter, (entry + i) % kLoraEntries);
         const int r = (chunks == 1 ? 0 : (first + i) % chunks) * chunk;
         if (issuer) {
-          if (i < low_tiles)
-            tma_load_2d<G>(dst_a + (uint32_t)(i * Cfg::kARows * chunk * 2), &lora.tmap_low, full, r, row_a, pol);
 #pragma unroll
           for (int h = 0; h < Cfg::kHalves; ++h) {
             const uint32_t dst = dst_b + h * Cfg::kBHalfBytes + (uint32_t)(i * Cfg::kBRows * chunk * 2);
@@ -568,6 +562,16 @@ __device__ __forceinline__ void lora_produce(const CUtensorMap& tmap_a, const CU
           }
         }
       }
+      // the weights do not wait for the kernel in front, the low rows do
+      if (!low_ready) {
+        grid_dependency_wait();
+        low_ready = true;
+      }
+      if (issuer)
+        for (int i = 0; i < low_tiles; ++i)
+          tma_load_2d<G>(dst_a + (uint32_t)(i * Cfg::kARows * chunk * 2), &lora.tmap_low, full,
+                         chunks == 1 ? 0 : (first + i) % chunks * chunk, row_a, pol);
+      __syncwarp();
       if (++s == Cfg::kStages) s = 0, phase ^= 1u;
     }
     if (low_once && lw.stages > 1) {

@@ -166,7 +166,7 @@ struct LowParams {
   int M, R, L;
   int p_rows;            // rows per box of P: 128, or fewer when M is
   int group_slots;       // adapters per group
-  int groups;            // CTA clusters per tile: groups are dealt to them round-robin
+  int groups;            // clusters per tile; the tile's groups are dealt to them
   unsigned int* status;
   unsigned long long timeout_ns;
 };
@@ -230,12 +230,17 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   const int slots = v.slot_count[tile256];
   const int* adapters = v.slot_adapter + tile256 * kLoraTileRows;
   const int k_blocks = (p.L + 63) / 64;
-  // The CTAs of a cluster take the K blocks in turn: what they read of a row of P at any moment is contiguous.
-  const int steps = (k_blocks - rank + splits - 1) / splits;
   const int R = p.R;
   // columns of the accumulator per adapter: the ranks, or whole chunks of them
   const int chunk = rank_chunk(R), slot_cols = kRankInner ? (R + chunk - 1) / chunk * chunk : R;
   const int groups = slots == 0 ? 1 : (slots + p.group_slots - 1) / p.group_slots;   // (no slot: zeros are written)
+  // A tile with more groups than clusters: the cluster takes up to `splits` groups at once and cuts L over fewer CTAs each
+  // (one exchange instead of one per group: 2048 x (4096 + 4096), 16 adapters of rank 32 in every tile, 38 us one after another).
+  int at_once = 1;
+  while (at_once < splits && at_once * p.groups < groups) at_once *= 2;
+  const int parts = splits / at_once, part = rank % parts, leader = rank - part;
+  // The CTAs of a part take the K blocks in turn: what they read of a row of P at any moment is contiguous.
+  const int steps = (k_blocks - part + parts - 1) / parts;
   const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
   uint32_t step = 0;                                   // ring position, running on over the groups
   uint32_t parity = 0;
@@ -249,9 +254,10 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
     __syncwarp();
   }
 #pragma unroll 1
-  for (int group = group0; group < groups; group += p.groups, parity ^= 1u) {
+  for (int first = group0 * at_once; first < groups; first += p.groups * at_once) {
+    const int group = first + rank / parts;
     const int slot0 = group * p.group_slots;
-    const int n_slots = min(p.group_slots, slots - slot0);
+    const int n_slots = min(p.group_slots, slots - slot0);   // (none left: the CTA only takes part in the exchange)
     const bool ok = *abort_flag == 0;
     if (n_slots > 0 && ok) {
       if (warp == 0) {
@@ -261,7 +267,7 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
         const uint32_t bytes = static_cast<uint32_t>(p.p_rows) * 128u + n_slots * w_bytes;
         const int my_adapter = static_cast<int>(lane) < n_slots ? adapters[slot0 + lane] : 0;
         uint32_t at = step;
-        for (int kb = rank; kb < k_blocks; kb += splits, ++at) {
+        for (int kb = part; kb < k_blocks; kb += parts, ++at) {
           const uint32_t s = at % kStages;
           if (!wait_bounded(empty + 8u * s, ((at / kStages) & 1u) ^ 1u, ctx, kStatusTimeoutProducer)) break;
           if (issuer) {
@@ -335,15 +341,16 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
         }
       }
       step += static_cast<uint32_t>(steps);
+      parity ^= 1u;
     }
     // every CTA's partial rows are written
     __syncthreads();
     cluster_arrive();
     cluster_wait();
     // This CTA's share of the rows, summed over the cluster in rank order.
-    const int share = 128 / splits, quads = R / 4;
+    const int share = 128 / parts, quads = R / 4;
     for (int i = threadIdx.x; i < share * quads; i += Cfg::kThreads) {
-      const int row = rank * share + i / quads, r = i % quads * 4;
+      const int row = part * share + i / quads, r = i % quads * 4;
       const long m = static_cast<long>(tile) * 128 + row;
       if (m >= p.M) break;
       const int slot = row_slot[row];
@@ -357,11 +364,11 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
       float4 x[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        if (c < splits) x[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(c)));
+        if (c < parts) x[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(leader + c)));
       float4 sum = x[0];
 #pragma unroll
       for (int c = 1; c < 8; ++c)
-        if (c < splits) sum.x += x[c].x, sum.y += x[c].y, sum.z += x[c].z, sum.w += x[c].w;
+        if (c < parts) sum.x += x[c].x, sum.y += x[c].y, sum.z += x[c].z, sum.w += x[c].w;
       const float f = row_factor[row];
       *reinterpret_cast<uint2*>(out) =
           make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x * f), __float_as_uint(sum.y * f)),
