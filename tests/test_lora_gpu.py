@@ -605,3 +605,39 @@ def test_short_main_loops_many_times(gk, M, N, K, R):
         res, tol = want(t)
         check("C", C, res, tol)
     gk.device_status()
+
+
+@pytest.mark.parametrize("M,N,K,R,G,kind", [(70001, 64, 64, 8, 300, "random"), (3, 150000, 64, 16, 3, "own"), (130, 72, 40000, 24, 4, "runs")])
+def test_one_long_extent(gk, M, N, K, R, G, kind):
+    t = make(M, N, K, R, G, torch.bfloat16, 300, id_pattern(kind, M, G, 9))
+    got = run_all(gk, t)
+    gk.device_status()
+    res, tol = want(t)
+    for name, value in got.items():
+        check(name, value, res, tol)
+
+
+def test_threads_that_call_at_once(gk):
+    """Four host threads on streams of their own, each with its plans and sizes."""
+    import threading
+
+    cases = [make(100 + 60 * i, 264 + 8 * i, 320, 16, 3 + i, torch.bfloat16, 400 + i, id_pattern("random", 100 + 60 * i, 3 + i, i))
+             for i in range(4)]
+    alone = [run_all(gk, t) for t in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = run_all(gk, cases[i])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend((i, name) for name in got if not torch.equal(got[name], alone[i][name]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+    gk.device_status()
