@@ -199,18 +199,18 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
 }
 
 // Tiles for few rows (at most 128, K a multiple of 64), where the shared planner, which does not know what adapter
-// stages cost on a tile, is up to 40 % off.  From forced runs of every configuration (M 4 to 128, N 2048 to 16384, K 2048 to 28672,
+// stages cost on a tile, is up to 40 % off.  From forced runs of every configuration (M 2 to 128, N 128 to 16384, K 256 to 28672,
 // 4 to 16 adapters of rank 16 and 64), planner's choice against this one:
 //  * more than half as many 128-column tiles as SMs, at most one each: those, whole (32 x 10240 x 5120 39.9 against
 //    30.7 us, 64 x 12288 x 8192 59.8 / 57.0, 4 x 16384 x 2048 19.6 / 17.7; 64-column tiles would need two waves);
-//  * fewer, and K at most twice N: 64-column tiles, whole (1 x 4096 x 4096 18.7 / 14.9, 64 x 4096 x 4096 23.2 / 18.4, 16 x 5120 x 8192
-//    34.2 / 28.8; for 65 to 128 rows there is no such tile);
+//  * fewer, and K at most twice N or at most 2048: 64-column tiles, whole (1 x 4096 x 4096 18.7 / 14.9, 64 x 4096 x 4096 23.2 /
+//    18.4, 16 x 5120 x 8192 34.2 / 28.8, 2 x 512 x 2048 12.5 / 9.3, 64 x 256 x 256 10.6 / 9.3; for 65 to 128 rows there is no such tile);
 //  * K longer: 128-column tiles cut in four while their clusters fit at once (16 x 2048 x 8192 29.6 / 20.3, 32 x 3584 x 28672 72.7 /
 //    48.4), else 256-column tiles cut in four (8 x 4096 x 14336 41.5 / 35.9, 128 x 5120 x 28672 76.5 / 70.0).  Where the
 //    clusters of the narrow tiles just fit, many adapter ranks (`adapter_ranks`: those that a tile's rows can use, all
 //    adapters together) want their twice as many CTAs: 64 x 4096 x 14336 with 32 adapters of rank 64 51.5 / 45.0.
 bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* out) {
-  if (M > 128 || K % 64 != 0 || N < 1024) return false;
+  if (M > 128 || K % 64 != 0) return false;
   if (g_opt_tile_config >= 0 || g_opt_split_k >= 0 || g_opt_sk_cluster >= 0 || g_opt_tiles_n > 0 || g_opt_max_ctas > 0)
     return false;                                          // forced choices go to the planner
   const long t64 = ceil_div(N, 64), t128 = ceil_div(N, 128), t256 = ceil_div(N, 256);
@@ -219,7 +219,7 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
     if (t128 > sm_count) return false;
     plan.config = 12;
     plan.ctas = static_cast<int>(t128);
-  } else if (K <= 2L * N) {
+  } else if (K <= 2L * N || K <= 2048) {
     if (M > 64) return false;
     plan.config = M <= 16 ? 13 : 14;
     plan.ctas = static_cast<int>(t64);

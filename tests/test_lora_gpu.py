@@ -559,7 +559,8 @@ def test_long_rows_and_far_adapters(gk):
 
 
 @pytest.mark.parametrize("M,N,K,R,G", [(5, 4096, 512, 16, 5), (40, 2048, 1024, 24, 40), (100, 9600, 256, 8, 60), (128, 1152, 4096, 16, 9),
-                                       (64, 4096, 8448, 64, 20), (64, 4096, 8448, 16, 3), (33, 8448, 17408, 8, 2)])
+                                       (64, 4096, 8448, 64, 20), (64, 4096, 8448, 16, 3), (33, 8448, 17408, 8, 2),
+                                       (40, 264, 2048, 24, 12), (3, 8, 1024, 8, 3), (9, 136, 8192, 16, 9)])
 def test_few_rows_under_the_own_plan(gk, M, N, K, R, G):
     """A case for each branch of the tile choice for few rows."""
     t = make(M, N, K, R, G, torch.bfloat16, 100 + M, id_pattern("random", M, G, 8))
