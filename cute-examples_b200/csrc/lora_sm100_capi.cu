@@ -198,6 +198,11 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
+// Forced choices go to the planner.
+bool choice_forced() {
+  return g_opt_tile_config >= 0 || g_opt_split_k >= 0 || g_opt_sk_cluster >= 0 || g_opt_tiles_n > 0 || g_opt_max_ctas > 0;
+}
+
 // Tiles for few rows (at most 128, K a multiple of 64), where the shared planner, which does not know what adapter
 // stages cost on a tile, is up to 40 % off.  From forced runs of every configuration (M 2 to 128, N 128 to 16384, K 256 to 28672,
 // 4 to 16 adapters of rank 16 and 64), planner's choice against this one:
@@ -210,9 +215,7 @@ int launch_product_config(const Problem& p, const AdapterOperands& o, const Plan
 //    clusters of the narrow tiles just fit, many adapter ranks (`adapter_ranks`: those that a tile's rows can use, all
 //    adapters together) want their twice as many CTAs: 64 x 4096 x 14336 with 32 adapters of rank 64 51.5 / 45.0.
 bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* out) {
-  if (M > 128 || K % 64 != 0) return false;
-  if (g_opt_tile_config >= 0 || g_opt_split_k >= 0 || g_opt_sk_cluster >= 0 || g_opt_tiles_n > 0 || g_opt_max_ctas > 0)
-    return false;                                          // forced choices go to the planner
+  if (M > 128 || K % 64 != 0 || choice_forced()) return false;
   const long t64 = ceil_div(N, 64), t128 = ceil_div(N, 128), t256 = ceil_div(N, 256);
   Plan plan;
   if (2 * t128 > sm_count) {
@@ -234,14 +237,80 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
   return true;
 }
 
+// Tiles for more than 128 rows whose output still is less than a wave.  The planner counts on all SMs, but the kernel
+// of the low rows still holds some when this one starts: CTAs beyond about 100 (fewer for clusters, which want neighbouring
+// SMs) wait for it, and the whole product with them.  About half of the SMs, busy from the start, are then the
+// better choice.  Forced runs of every configuration (M 129 to 1024, output columns 512 to 12288, K 512 to 16384), and the choice below
+// against the planner's as part of a longer sequence (dA: a training step; forward: behind a 2048 x 2048 x 2048 GEMM of 17 us), in us
+// for one adapter of rank 64 / runs of four of rank 32 / 16 of rank 16 in every tile.  M x output columns x K:
+//  [K,N] operand (dA):
+//  * 64 to 74 CTAs of 256 x 256 pair tiles: those, whole; with 64 to 66 the planner's clusters of four all fit and are as
+//    good from K = 8192 (512 x 4352 x 1024 46.1, 41.7, 49.3 -> 37.5, 33.4, 40.4; 256 x 8704 x 4096 74.7, 74.8, 89.1 -> 70.9, 70.1, 80.2);
+//  * 14 to 16 such tiles, K 4096 up to 8192: cut in two (1024 x 1024 x 4096 58.0, 50.1, 59.7 -> 51.6, 46.9, 58.0; at K = 8192 2 % slower,
+//    with 18 to 28 tiles 3 to 8 %);
+//  * 7 to 9, more than 256 rows, K from 8192: 128 x 256 tiles cut in four instead of the planner's clusters of eight (1024 x 512 x
+//    8192 62.4, 55.9, 85.0 -> 59.2, 53.6, 84.6; 512 x 1024 x 8192 52.6, 48.8, 68.6 -> 52.4, 48.9, 59.9).
+//  [N,K] operand (K a multiple of 64 for 128-column tiles):
+//  * up to 74 CTAs of 256 x 256 pair tiles, from 64 to 72 CTAs on by the rows, K at most 2048 (1024 from 513 rows on): those,
+//    whole (512 x 4352 x 1024 31.5, 30.7, 34.5 -> 29.2, 29.0, 31.9; 1024 x 2048 x 2048 with 16 adapters 38.4 -> 41.7);
+//  * 68 to 74 CTAs of 256 x 128 pair tiles, K from 8192: those, whole (256 x 4608 x 8192 58.0, 58.9, 60.5 -> 51.4, 52.1, 54.8);
+//  * 13 to 20 such tiles, K from 4096: cut in two (512 x 1024 x 4096 40.4, 39.6, 42.6 -> 34.6, 34.8, 36.2; 256 x 2048 x 14336 56.3, 57.4,
+//    62.5 -> 53.9, 54.2, 56.3);
+//  * 12, K from 4096: 128 x 128 tiles cut in four (512 x 768 x 8192 42.8, 42.5, 48.0 -> 38.9, 39.0, 49.6; 256 x 1536 x 8192 37.1, 38.1, 47.6
+//    -> 38.8, 39.5, 41.0).
+bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) {
+  if (M <= 128 || choice_forced()) return false;
+  const long rows = ceil_div(M, 256), wide = rows * ceil_div(N, 256), narrow = rows * ceil_div(N, 128);
+  const long half = sm_count / 4;                          // pair tiles on half of the SMs
+  int config = -1, factor = 1;
+  if (b_is_kn) {
+    if (wide <= half && (wide > 33 || (wide >= 32 && K <= 4096))) {
+      config = 0;
+    } else if (wide >= 14 && wide <= 16 && K >= 4096 && K < 8192) {
+      config = 0;
+      factor = 2;
+    } else if (wide >= 7 && wide <= 9 && M > 256 && K >= 8192) {
+      config = 2;
+      factor = 4;
+    }
+  } else if (wide >= 32 + (M <= 512 ? 2 : 0) + (M <= 256 ? 2 : 0) && wide <= half &&
+             K <= (M > 512 ? 1024 : 2048)) {
+    config = 0;
+  } else if (K % 64 == 0) {
+    if (narrow >= 34 && narrow <= half && K >= 8192) {
+      config = 11;
+    } else if (narrow >= 13 && narrow <= 20 && K >= 4096) {
+      config = 11;
+      factor = 2;
+    } else if (narrow == 12 && K >= 4096) {
+      config = 12;
+      factor = 4;
+    }
+  }
+  if (config < 0) return false;
+  Plan plan;
+  plan.config = config;
+  const ConfigInfo& c = kConfigs[config];
+  plan.ctas = static_cast<int>(ceil_div(M, 128L * c.cta_group) * ceil_div(N, static_cast<long>(c.mma_n) * c.halves) * factor *
+                               c.cta_group);
+  if (factor > 1) {
+    plan.split_k = plan.cluster = true;
+    plan.split_factor = factor;
+  }
+  *out = plan;
+  return true;
+}
+
 template <bool kIsBf16>
 int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   if (p.b_is_kn) {
-    const Plan plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigsKN, /*allow_balance=*/false,
-                               /*allow_workspace=*/false);
+    Plan plan;
+    if (!half_wave_plan(p.M, p.N, p.K, /*b_is_kn=*/true, st->sm_count, &plan))
+      plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigsKN, /*allow_balance=*/false,
+                      /*allow_workspace=*/false);
     switch (plan.config) {
       case 0: return launch_product_config<0, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
       case 1: return launch_product_config<1, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
@@ -250,7 +319,8 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
     }
   }
   Plan plan;
-  if (!few_row_plan(p.M, p.N, p.K, static_cast<long>(o.adapters < p.M ? o.adapters : p.M) * o.R, st->sm_count, &plan))
+  if (!few_row_plan(p.M, p.N, p.K, static_cast<long>(o.adapters < p.M ? o.adapters : p.M) * o.R, st->sm_count, &plan) &&
+      !half_wave_plan(p.M, p.N, p.K, /*b_is_kn=*/false, st->sm_count, &plan))
     plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigs, /*allow_balance=*/true,
                     /*allow_workspace=*/false);
   switch (plan.config) {

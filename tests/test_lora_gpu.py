@@ -570,6 +570,22 @@ def test_few_rows_under_the_own_plan(gk, M, N, K, R, G):
     check("C", C, res, tol)
 
 
+@pytest.mark.parametrize("M,N,K,R,G", [(256, 8704, 128, 16, 9), (256, 4480, 8192, 8, 5), (300, 1000, 4096, 24, 30), (600, 504, 4096, 16, 3),
+                                       (250, 264, 8704, 16, 9), (500, 520, 4096, 8, 40), (300, 4104, 2000, 24, 30),
+                                       (520, 8200, 640, 16, 12)])
+def test_less_than_a_wave_under_the_own_plan(gk, M, N, K, R, G):
+    """A case for each branch of the tile choice for outputs of less than a wave: four of the forward product, four of dA."""
+    t = make(M, N, K, R, G, torch.bfloat16, 140 + M, id_pattern("random", M, G, 8))
+    C = forward_only(gk, t)
+    res, tol = want(t)
+    check("C", C, res, tol)
+    plan = gk.LoraPlan(t["ids"], G)
+    grads = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"])
+    for name, value in zip(("dA", "d_down", "d_up"), grads):
+        check(name, value, res, tol)
+    gk.device_status()
+
+
 def test_plan_refilled_before_every_call(gk):
     """A plan that changes in place just before the product reads it: a stale copy of the old plan, in some SM's cache,
     would give wrong rows or leave the kernel's warps at odds about the number of adapters."""
