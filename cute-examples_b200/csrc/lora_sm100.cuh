@@ -165,8 +165,11 @@ struct LowParams {
   long ld_out;
   int M, R, L;
   int p_rows;            // rows per box of P: 128, or fewer when M is
+  int splits;            // partial sums of a row: L is cut over as many CTAs, or over half of them with two sums each
+  int workers;           // CTAs of the cluster that work (splits or splits / 2); those beyond have nothing to do
+  int clusters;          // clusters per tile; the tile's groups are dealt to them
   int group_slots;       // adapters per group
-  int groups;            // clusters per tile; the tile's groups are dealt to them
+  int groups;            // groups that are taken one to a cluster of `splits` sums; with more, fewer sums of each are formed
   unsigned int* status;
   unsigned long long timeout_ns;
 };
@@ -178,7 +181,9 @@ struct LowConfig {
   static constexpr int kStages = kDeep ? 6 : 3;
   static constexpr int kPBytes = 128 * 64 * 2, kWBytes = 128 * 64 * 2;
   static constexpr int kStageBytes = kPBytes + kWBytes;
-  static constexpr int kTmemCols = 128;
+  static constexpr int kTmemCols = 256;                // two accumulators of 128 columns
+  static constexpr int kMaxFoldedRank = kStages * kStageBytes / (2 * 128 * 4) / 8 * 8 - 8;   // two sets of partial rows in the ring
+  static_assert(2 * 128 * (kMaxFoldedRank + 4) * 4 <= kStages * kStageBytes, "partial rows");
   static constexpr int kBarrierBytes = 128;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarrierBytes + 128 * 8;
 };
@@ -199,11 +204,11 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
   const int rank = static_cast<int>(cluster_ctarank());
-  uint32_t splits_reg;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits_reg));
-  const int splits = static_cast<int>(splits_reg);
-  const int unit = block / splits;
-  const int tile = unit / p.groups, group0 = unit % p.groups;
+  uint32_t cluster_size;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_size));
+  const bool idle = rank >= p.workers;                 // (a shared launch has the clusters of the problem that is cut further)
+  const int unit = block / static_cast<int>(cluster_size);
+  const int tile = unit / p.clusters, group0 = unit % p.clusters;
   WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
 
   if (threadIdx.x == 0) {
@@ -234,11 +239,17 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   // columns of the accumulator per adapter: the ranks, or whole chunks of them
   const int chunk = rank_chunk(R), slot_cols = kRankInner ? (R + chunk - 1) / chunk * chunk : R;
   const int groups = slots == 0 ? 1 : (slots + p.group_slots - 1) / p.group_slots;   // (no slot: zeros are written)
-  // A tile with more groups than clusters: the cluster takes up to `splits` groups at once and cuts L over fewer CTAs each
-  // (one exchange instead of one per group: 2048 x (4096 + 4096), 16 adapters of rank 32 in every tile, 38 us one after another).
-  int at_once = 1;
-  while (at_once < splits && at_once * p.groups < groups) at_once *= 2;
-  const int parts = splits / at_once, part = rank % parts, leader = rank - part;
+  // A tile with more groups than clusters: the cluster takes up to `splits` groups at once and forms fewer partial sums of
+  // each (one exchange instead of one per group: 2048 x (4096 + 4096), 16 adapters of rank 32 in every tile, 38 us one after
+  // another).  `sums` follows from the problem alone, for it is the order in which a row is added up; where the CTAs are
+  // half as many, each has every second of its K blocks in a second accumulator.
+  int sums = p.splits;
+  while (sums > 1 && p.splits / sums * p.groups < groups) sums /= 2;
+  int parts = sums < p.workers ? sums : p.workers;
+  if (parts == sums && sums > 1 && p.workers / parts * p.clusters < groups) parts /= 2;
+  const int at_once = p.workers / parts;
+  const int part = rank % parts, leader = rank - part;
+  const uint32_t second = parts < sums ? 128u : 0u;    // column of the second accumulator
   // The CTAs of a part take the K blocks in turn: what they read of a row of P at any moment is contiguous.
   const int steps = (k_blocks - part + parts - 1) / parts;
   const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
@@ -254,10 +265,10 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
     __syncwarp();
   }
 #pragma unroll 1
-  for (int first = group0 * at_once; first < groups; first += p.groups * at_once) {
+  for (int first = group0 * at_once; first < groups; first += p.clusters * at_once) {
     const int group = first + rank / parts;
     const int slot0 = group * p.group_slots;
-    const int n_slots = min(p.group_slots, slots - slot0);   // (none left: the CTA only takes part in the exchange)
+    const int n_slots = idle ? 0 : min(p.group_slots, slots - slot0);   // (none left: the CTA only takes part in the exchange)
     const bool ok = *abort_flag == 0;
     if (n_slots > 0 && ok) {
       if (warp == 0) {
@@ -297,15 +308,17 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
           if (!wait_bounded(full + 8u * s, (at / kStages) & 1u, ctx, kStatusTimeoutMma)) break;
           tc_fence_after_sync();
           if (issuer) {
+            const uint32_t acc = tmem + (i & 1 ? second : 0u);
+            const bool begun = i > (second != 0u ? 1 : 0);
             const uint64_t dp = make_smem_desc_sw128(smem_p + s * Cfg::kPBytes);
             if constexpr (!kRankInner) {
               const uint64_t dw = make_smem_desc_sw128(smem_w + s * Cfg::kWBytes);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * k, idesc, i > 0 || k > 0);
+              for (int k = 0; k < 4; ++k) umma_f16<1>(acc, dp + 2u * k, dw + 2u * k, idesc, begun || k > 0);
             } else {
               const uint64_t dw = make_smem_desc_rows_mn(smem_w + s * Cfg::kWBytes, chunk * 2u, chunk * 128u);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16<1>(tmem, dp + 2u * k, dw + 2u * chunk * k, idesc, i > 0 || k > 0);
+              for (int k = 0; k < 4; ++k) umma_f16<1>(acc, dp + 2u * k, dw + 2u * chunk * k, idesc, begun || k > 0);
             }
             umma_commit<1>(empty + 8u * s);
             if (i == steps - 1) umma_commit<1>(done);
@@ -319,21 +332,23 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
         const int mine = row_slot[row] - slot0;
         if (wait_bounded(done, parity, ctx, kStatusTimeoutEpilogue)) {
           tc_fence_after_sync();
-          const uint32_t dst = base + static_cast<uint32_t>(row * pitch) * 4u;
+          const uint32_t dst = base + static_cast<uint32_t>(row * pitch) * 4u, lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
           for (int j = 0; j < n_slots; ++j) {
             if (!__any_sync(0xffffffffu, mine == j)) continue;
             for (int r = 0; r < R; r += 8) {
-              uint32_t x[8];
-              tmem_ld_32x8(tmem + (static_cast<uint32_t>(q * 32) << 16) + j * slot_cols + r, x);
-              tmem_ld_wait();
-              if (mine == j) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * 4u), "r"(x[0]), "r"(x[1]), "r"(x[2]),
-                             "r"(x[3])
-                             : "memory");
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * 4u + 16u), "r"(x[4]), "r"(x[5]),
-                             "r"(x[6]), "r"(x[7])
-                             : "memory");
+              for (uint32_t acc = 0; acc <= second; acc += 128u) {
+                uint32_t x[8];
+                tmem_ld_32x8(lanes + acc + j * slot_cols + r, x);
+                tmem_ld_wait();
+                if (mine == j) {
+                  const uint32_t to = dst + r * 4u + acc * (static_cast<uint32_t>(pitch) * 4u);   // 128 rows further on
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                               : "memory");
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16u), "r"(x[4]), "r"(x[5]), "r"(x[6]),
+                               "r"(x[7])
+                               : "memory");
+                }
               }
             }
           }
@@ -347,8 +362,8 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
     __syncthreads();
     cluster_arrive();
     cluster_wait();
-    // This CTA's share of the rows, summed over the cluster in rank order.
-    const int share = 128 / parts, quads = R / 4;
+    // This CTA's share of the rows, summed over the parts' sums in their order.
+    const int share = idle ? 0 : 128 / parts, quads = R / 4;
     for (int i = threadIdx.x; i < share * quads; i += Cfg::kThreads) {
       const int row = part * share + i / quads, r = i % quads * 4;
       const long m = static_cast<long>(tile) * 128 + row;
@@ -364,11 +379,13 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
       float4 x[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        if (c < parts) x[c] = ld_cluster_v4(map_to_cta(src, static_cast<uint32_t>(leader + c)));
+        if (c < sums)
+          x[c] = ld_cluster_v4(map_to_cta(src + (c < parts ? 0u : 128u * static_cast<uint32_t>(pitch) * 4u),
+                                          static_cast<uint32_t>(leader + (c < parts ? c : c - parts))));
       float4 sum = x[0];
 #pragma unroll
       for (int c = 1; c < 8; ++c)
-        if (c < parts) sum.x += x[c].x, sum.y += x[c].y, sum.z += x[c].z, sum.w += x[c].w;
+        if (c < sums) sum.x += x[c].x, sum.y += x[c].y, sum.z += x[c].z, sum.w += x[c].w;
       const float f = row_factor[row];
       *reinterpret_cast<uint2*>(out) =
           make_uint2(pack2<kIsBf16>(__float_as_uint(sum.x * f), __float_as_uint(sum.y * f)),
@@ -399,7 +416,7 @@ __global__ void __launch_bounds__(192, kDeep ? 1 : 2) lora_low_kernel(const __gr
 }
 
 // Both kinds of rows in one launch, for a backward pass that computes the low rows again: the first `blocks` CTAs
-// low, the others d_low.
+// low, the others d_low.  Each adds its rows up as a launch of its own does, so that they have the same bits.
 template <bool kIsBf16, bool kDeep>
 __global__ void __launch_bounds__(192, kDeep ? 1 : 2)
 lora_low_pair_kernel(const __grid_constant__ LowParams low, const __grid_constant__ LowParams d_low, const int blocks) {

@@ -658,3 +658,33 @@ def test_threads_that_call_at_once(gk):
         th.join()
     assert not wrong
     gk.device_status()
+
+
+def backward_variants(gk, t):
+    """The gradients for every way of calling the backward pass: `low` kept or computed again, any of them unwanted."""
+    plan = gk.LoraPlan(t["ids"], t["down"].shape[0])
+    low = torch.empty(t["A"].shape[0], t["down"].shape[1], dtype=t["A"].dtype, device="cuda")
+    gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low)
+    for kept in (None, low):
+        for bits in range(1, 8):
+            needs = tuple(bool(bits >> i & 1) for i in range(3))
+            yield needs, gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=kept, needs=needs)
+
+
+@pytest.mark.parametrize("M,N,K,R,G,kind", [(200, 64, 1024, 16, 3, "runs"), (300, 1024, 128, 16, 3, "runs"), (2500, 1024, 1024, 16, 4, "runs"),
+                                            (130, 72, 40000, 24, 4, "runs"), (8192, 512, 1024, 16, 2, "runs"), (700, 264, 1024, 16, 60, "random"),
+                                            (3000, 4096, 256, 40, 3, "runs"), (1100, 8, 712, 128, 30, "random")])
+def test_kept_and_recomputed_low_rows_give_the_same_bits(gk, M, N, K, R, G, kind):
+    """Extents where a launch that low and d_low share has to cut one of them less, or more, than a launch of its own would."""
+    t = make(M, N, K, R, G, torch.bfloat16, 500 + M, id_pattern(kind, M, G, 3))
+    first = None
+    for needs, grads in backward_variants(gk, t):
+        first = first or list(grads)
+        for i, (wanted, value) in enumerate(zip(needs, grads)):
+            if wanted and first[i] is None:
+                first[i] = value
+            assert torch.equal(value, first[i]) if wanted else value is None, (needs, i)
+    res, tol = want(t)
+    for name, value in zip(("dA", "d_down", "d_up"), first):
+        check(name, value, res, tol)
+    gk.device_status()
