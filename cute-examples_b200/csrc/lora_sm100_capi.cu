@@ -540,13 +540,15 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
   // How far to cut the rows: the rows may all belong to one adapter, so the cut that finishes that case first
   // sets the number of rows a CTA takes at once; adapters with fewer rows are cut less.
-  // (nine tenths of the CTAs that the SMs hold: a cluster sits inside one GPC, and what is left over there must not make
-  // a second wave)
+  // (Nine tenths of the CTAs that the SMs hold: a cluster sits inside one GPC, and what is left over there must not make
+  // a second wave.)  The cut is the order in which a gradient is added up: it is chosen for both gradients' tiles, also
+  // where only one of them is wanted, so that this one has the same bits then.
   const long clusters = static_cast<long>(st->sm_count) * Cfg::kCtasPerSm * 9 / (10 * kGradCluster);
+  const long both = ceil_div(a.K, 128) + ceil_div(a.N, 128);
   int splits = 1;
   double best = 1e300;
   for (int c = 1; c <= kGradCluster; c *= 2) {
-    const double t = static_cast<double>(ceil_div(ceil_div(p.tiles, kGradCluster / c), clusters)) *
+    const double t = static_cast<double>(ceil_div(ceil_div(both, kGradCluster / c), clusters)) *
                      (static_cast<double>(ceil_div(a.M, c)) + 128.0);      // (a unit costs about two blocks of rows besides)
     if (t < best) best = t, splits = c;
   }

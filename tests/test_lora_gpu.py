@@ -688,3 +688,20 @@ def test_kept_and_recomputed_low_rows_give_the_same_bits(gk, M, N, K, R, G, kind
     for name, value in zip(("dA", "d_down", "d_up"), first):
         check(name, value, res, tol)
     gk.device_status()
+
+
+@pytest.mark.parametrize("M,N,K,R,G,kind", [(1024, 12000, 1032, 64, 1, "one"), (1024, 1032, 12000, 48, 1, "one"), (900, 13000, 264, 128, 3, "runs")])
+def test_unwanted_gradients_leave_the_bits_of_the_others(gk, M, N, K, R, G, kind):
+    """Extents where one adapter gradient alone has fewer column tiles than the device holds CTAs, and both have more."""
+    t = make(M, N, K, R, G, torch.float16, 600 + K, id_pattern(kind, M, G, 3))
+    first = None
+    for needs, grads in backward_variants(gk, t):
+        first = first or list(grads)
+        for i, (wanted, value) in enumerate(zip(needs, grads)):
+            if wanted and first[i] is None:
+                first[i] = value
+            assert torch.equal(value, first[i]) if wanted else value is None, (needs, i)
+    res, tol = want(t)
+    for name, value in zip(("dA", "d_down", "d_up"), first):
+        check(name, value, res, tol)
+    gk.device_status()
