@@ -203,9 +203,11 @@ namespace {
 
 using OptTensor = c10::optional<torch::Tensor>;
 
-// Row pitch of the last two dimensions (the stride of a single row is not meaningful).
+// Row pitch of the last two dimensions.  The stride of a single row is not meaningful and never used: what is handed over
+// only has to be a pitch that the row could have.
+int64_t round_up_8(int64_t n) { return (n + 7) / 8 * 8; }
 long pitch(const torch::Tensor& t) {
-  return t.size(-2) > 1 ? static_cast<long>(t.stride(-2)) : static_cast<long>(t.size(-1));
+  return static_cast<long>(t.size(-2) > 1 ? t.stride(-2) : round_up_8(t.size(-1)));
 }
 long matrix_stride(const torch::Tensor& t) {
   return t.size(0) > 1 ? static_cast<long>(t.stride(0)) : static_cast<long>(t.size(1) * t.size(2));
@@ -274,7 +276,7 @@ void hold_plan(const torch::Tensor& plan, int64_t made_on, const c10::cuda::CUDA
   if (reinterpret_cast<int64_t>(stream.stream()) != made_on) plan.record_stream(stream.unwrap());
 }
 
-// `out` and `low` undefined: allocated here.
+// `out` and `low` undefined: allocated here, `out` with rows of a multiple of 8 elements.
 torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torch::Tensor down, const torch::Tensor up,
                         const torch::Tensor plan, int64_t plan_rows, int64_t plan_adapters, int64_t plan_stream,
                         const OptTensor scales, double scale, const OptTensor out, const OptTensor low_out) {
@@ -287,7 +289,8 @@ torch::Tensor gemm_lora(const torch::Tensor A, const torch::Tensor B, const torc
   c10::cuda::CUDAGuard guard(A.device());
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(A.device().index());
   // from the caching allocator: safe in stream order, and part of the graph's own memory under capture
-  torch::Tensor C = out.has_value() ? *out : torch::empty({a.M, a.N}, A.options());
+  torch::Tensor C = out.has_value() ? *out : torch::empty({a.M, round_up_8(a.N)}, A.options());
+  if (!out.has_value() && a.N % 8 != 0) C = C.narrow(1, 0, a.N);
   if (a.M == 0) return C;
   const torch::Tensor low = low_out.has_value() ? *low_out : torch::empty({a.M, a.R}, A.options());
   hold_plan(plan, plan_stream, stream);

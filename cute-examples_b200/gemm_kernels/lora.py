@@ -63,7 +63,8 @@ def gemm_lora(A: torch.Tensor, B: torch.Tensor, down: torch.Tensor, up: torch.Te
     A ``[M,K]``, B ``[N,K]``, down ``[adapters,R,K]``, up ``[adapters,N,R]``, all bf16 or all fp16; R is a
     multiple of 8 up to 128, K a multiple of 8.  ``scale`` is a number or a float32 tensor with one
     value per adapter.  ``low`` (``[M,R]``) receives the scaled low-rank rows, which the backward pass
-    can use again.  ``out`` may have a row pitch (a multiple of 8 elements).
+    can use again.  ``out`` may have a row pitch; with more than one row it has to be a multiple of 8
+    elements.  Without ``out`` and with N no multiple of 8 the result is the first N columns of such rows.
     """
     scales, factor = _scales(scale)
     return _C.gemm_lora(A, B, down, up, plan.buffer, plan.rows, plan.num_adapters, plan.stream, scales, factor, out, low)

@@ -705,3 +705,27 @@ def test_unwanted_gradients_leave_the_bits_of_the_others(gk, M, N, K, R, G, kind
     for name, value in zip(("dA", "d_down", "d_up"), first):
         check(name, value, res, tol)
     gk.device_status()
+
+
+@pytest.mark.parametrize("N", [1, 9, 397])
+@pytest.mark.parametrize("M", [1, 2, 70])
+@pytest.mark.parametrize("form", ["none", "pitched", "dense"])
+def test_columns_that_are_no_multiple_of_8(gk, M, N, form):
+    K, R, G = 72, 8, 3
+    t = make(M, 400, K, R, G, torch.bfloat16, 700 + N, id_pattern("own", M, G, 5))
+    t["B"], t["up"], t["dC"] = t["B"][:N], t["up"][:, :N].contiguous(), t["dC"][:, :N]
+    wide = torch.full((M + 1, 416), 3.0, dtype=torch.bfloat16, device="cuda")
+    line = torch.full((M * N + 64,), 3.0, dtype=torch.bfloat16, device="cuda")
+    out = {"none": None, "pitched": wide[:M, :N], "dense": line[:M * N].view(M, N)}[form]
+    if form == "dense" and M > 1:
+        with pytest.raises(RuntimeError, match="16-byte aligned"):
+            forward_only(gk, t, out=out)
+        return
+    got = forward_only(gk, t, out=out)
+    assert got.shape == (M, N) and got.stride(1) == 1
+    assert out is None or got.data_ptr() == out.data_ptr()
+    res, tol = want(t)
+    check("C", got, res, tol)
+    assert bool((wide[:, N:] == 3).all()) and bool((wide[M:] == 3).all()) and bool((line[M * N:] == 3).all())
+    again = forward_only(gk, t)
+    assert torch.equal(got, again)
