@@ -183,6 +183,12 @@ int lora_prepare(DeviceState& st, int* cuda_error_out);
 Plan plan_for(int M, int N, int K, int sm_count, bool allow_split = true, unsigned config_mask = ~0u,
               bool allow_balance = true, bool allow_workspace = true);
 
+// A plan for an output of N columns in words.
+void describe(const Plan& plan, int N, char* buf, size_t buf_bytes);
+
+// SMs of the current device (those of a B200 where there is none).
+int current_sm_count();
+
 inline int grid_cap(const ConfigInfo& c, int sm_count) {
   long cap = sm_count - sm_count % c.cta_group;
   if (g_opt_max_ctas > 0 && g_opt_max_ctas < cap) cap = g_opt_max_ctas - g_opt_max_ctas % c.cta_group;

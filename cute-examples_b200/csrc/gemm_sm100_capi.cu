@@ -818,6 +818,11 @@ int dispatch(const Plan& plan, const Problem& p, void* ws, DeviceState& st, cuda
   }
 }
 
+}  // namespace
+
+namespace gemm_sm100 {
+namespace host {
+
 int current_sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
@@ -826,7 +831,30 @@ int current_sm_count() {
   return n;
 }
 
-}  // namespace
+void describe(const Plan& plan, int N, char* buf, size_t buf_bytes) {
+  const ConfigInfo& c = kConfigs[plan.config];
+  const int block_n = c.mma_n * c.halves;
+  char tiling[128];
+  if (plan.tiles_n > 0)
+    std::snprintf(tiling, sizeof(tiling), "balanced: %d tiles per row, %d x %d + %d x %d columns (wide from %d)",
+                  plan.tiles_n, plan.bal_rem, (plan.bal_q + 1) * 64, plan.tiles_n - plan.bal_rem, plan.bal_q * 64,
+                  plan.bal_start);
+  else
+    std::snprintf(tiling, sizeof(tiling), "uniform: %ld tiles per row of %d columns", ceil_div(N, block_n), block_n);
+  char split[96];
+  if (!plan.split_k)
+    std::snprintf(split, sizeof(split), "whole tiles");
+  else if (plan.split_factor > 1)
+    std::snprintf(split, sizeof(split), "every tile cut into %d K ranges%s", plan.split_factor,
+                  plan.cluster ? " (one cluster per tile)" : "");
+  else
+    std::snprintf(split, sizeof(split), "contiguous K ranges");
+  std::snprintf(buf, buf_bytes, "config=%d tile=%dx%dx64 %s; %s; ctas=%d workspace=%zu", plan.config, 128 * c.cta_group,
+                block_n, tiling, split, plan.ctas, plan.split_k ? plan.flag_bytes + plan.partial_bytes : size_t{0});
+}
+
+}  // namespace host
+}  // namespace gemm_sm100
 
 extern "C" {
 
@@ -1208,25 +1236,7 @@ int gemm_sm100_describe_plan(int M, int N, int K, int dtype, char* buf, size_t b
   if (!buf || buf_bytes == 0) return GEMM_SM100_ERR_NULL_POINTER;
   if (M <= 0 || N <= 0 || K <= 0) return GEMM_SM100_ERR_BAD_SHAPE;
   const Plan plan = plan_for(M, N, K, current_sm_count());
-  const ConfigInfo& c = kConfigs[plan.config];
-  const int block_n = c.mma_n * c.halves;
-  char tiling[128];
-  if (plan.tiles_n > 0)
-    std::snprintf(tiling, sizeof(tiling), "balanced: %d tiles per row, %d x %d + %d x %d columns (wide from %d)",
-                  plan.tiles_n, plan.bal_rem, (plan.bal_q + 1) * 64, plan.tiles_n - plan.bal_rem, plan.bal_q * 64,
-                  plan.bal_start);
-  else
-    std::snprintf(tiling, sizeof(tiling), "uniform: %ld tiles per row of %d columns", ceil_div(N, block_n), block_n);
-  char split[96];
-  if (!plan.split_k)
-    std::snprintf(split, sizeof(split), "whole tiles");
-  else if (plan.split_factor > 1)
-    std::snprintf(split, sizeof(split), "every tile cut into %d K ranges%s", plan.split_factor,
-                  plan.cluster ? " (one cluster per tile)" : "");
-  else
-    std::snprintf(split, sizeof(split), "contiguous K ranges");
-  std::snprintf(buf, buf_bytes, "config=%d tile=%dx%dx64 %s; %s; ctas=%d workspace=%zu", plan.config, 128 * c.cta_group,
-                block_n, tiling, split, plan.ctas, plan.split_k ? plan.flag_bytes + plan.partial_bytes : size_t{0});
+  describe(plan, N, buf, buf_bytes);
   return GEMM_SM100_OK;
 }
 

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdio>
 #include <cstring>
 #include <mutex>
 #include <utility>
@@ -301,16 +302,26 @@ bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) 
   return true;
 }
 
+// What carries out a product, and in `rule` what chose it.
+Plan product_plan(int M, int N, int K, bool b_is_kn, int R, int adapters, int sm_count, const char** rule) {
+  Plan plan;
+  *rule = "few rows";
+  if (!b_is_kn && few_row_plan(M, N, K, static_cast<long>(adapters < M ? adapters : M) * R, sm_count, &plan)) return plan;
+  *rule = "less than a wave";
+  if (half_wave_plan(M, N, K, b_is_kn, sm_count, &plan)) return plan;
+  *rule = "planner";
+  return plan_for(M, N, K, sm_count, /*allow_split=*/true, b_is_kn ? kProductConfigsKN : kProductConfigs,
+                  /*allow_balance=*/!b_is_kn, /*allow_workspace=*/false);
+}
+
 template <bool kIsBf16>
 int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
+  const char* rule;
+  const Plan plan = product_plan(p.M, p.N, p.K, p.b_is_kn, o.R, o.adapters, st->sm_count, &rule);
   if (p.b_is_kn) {
-    Plan plan;
-    if (!half_wave_plan(p.M, p.N, p.K, /*b_is_kn=*/true, st->sm_count, &plan))
-      plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigsKN, /*allow_balance=*/false,
-                      /*allow_workspace=*/false);
     switch (plan.config) {
       case 0: return launch_product_config<0, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
       case 1: return launch_product_config<1, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
@@ -318,11 +329,6 @@ int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stre
       default: return launch_product_config<3, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
     }
   }
-  Plan plan;
-  if (!few_row_plan(p.M, p.N, p.K, static_cast<long>(o.adapters < p.M ? o.adapters : p.M) * o.R, st->sm_count, &plan) &&
-      !half_wave_plan(p.M, p.N, p.K, /*b_is_kn=*/false, st->sm_count, &plan))
-    plan = plan_for(p.M, p.N, p.K, st->sm_count, /*allow_split=*/true, kProductConfigs, /*allow_balance=*/true,
-                    /*allow_workspace=*/false);
   switch (plan.config) {
     case 0: return launch_product_config<0, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
     case 1: return launch_product_config<1, kIsBf16, false>(p, o, plan, *st, stream, cuda_error_out);
@@ -625,6 +631,20 @@ int gemm_sm100_lora_plan(const void* ids, int ids_are_64, int M, int adapters, v
   lora_plan_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(ids, ids_are_64, M, adapters, plan);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
+}
+
+int gemm_sm100_lora_describe_plan(int M, int N, int K, int R, int adapters, int gradient, char* buf, size_t buf_bytes) {
+  if (!buf || buf_bytes == 0) return GEMM_SM100_ERR_NULL_POINTER;
+  gemm_sm100_lora_args a = {};
+  a.M = M, a.N = N, a.K = K, a.R = R, a.adapters = adapters;
+  const int rc = check_common(a);
+  if (rc != GEMM_SM100_OK || M == 0 || (gradient && N % 8 != 0)) return rc != GEMM_SM100_OK ? rc : GEMM_SM100_ERR_BAD_SHAPE;
+  const char* rule;
+  // (dA is an [M, K] output with N contracted)
+  const Plan plan = product_plan(M, gradient ? K : N, gradient ? N : K, gradient != 0, R, adapters, current_sm_count(), &rule);
+  const int n = std::snprintf(buf, buf_bytes, "%s: ", rule);
+  if (n > 0 && static_cast<size_t>(n) < buf_bytes) describe(plan, gradient ? K : N, buf + n, buf_bytes - n);
+  return GEMM_SM100_OK;
 }
 
 int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low, void* cuda_stream, int* cuda_error_out) {

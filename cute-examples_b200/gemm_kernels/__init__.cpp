@@ -398,6 +398,12 @@ std::string describe_plan(int M, int N, int K, int dtype) {
   return std::string(buf);
 }
 
+std::string describe_lora_plan(int M, int N, int K, int R, int adapters, bool gradient) {
+  char buf[384];
+  raise_for(gemm_sm100_lora_describe_plan(M, N, K, R, adapters, gradient ? 1 : 0, buf, sizeof(buf)), 0, "describe_lora_plan");
+  return std::string(buf);
+}
+
 PYBIND11_MODULE(_C, m) {
   m.def("gemm_tn_test", &gemm_tn_test, "GEMM transpose-normal test function", pybind11::arg("A"),
         pybind11::arg("B"), pybind11::arg("C"));
@@ -428,6 +434,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("describe_config", &describe_config, pybind11::arg("index"));
   m.def("describe_plan", &describe_plan, pybind11::arg("M"), pybind11::arg("N"), pybind11::arg("K"),
         pybind11::arg("dtype"));
+  m.def("describe_lora_plan", &describe_lora_plan, pybind11::arg("M"), pybind11::arg("N"), pybind11::arg("K"),
+        pybind11::arg("R"), pybind11::arg("adapters"), pybind11::arg("gradient") = false);
   m.def("select_config", &gemm_sm100_select_config, pybind11::arg("M"), pybind11::arg("N"),
         pybind11::arg("K"), pybind11::arg("dtype"));
   m.def("workspace_bytes", &gemm_sm100_workspace_bytes, pybind11::arg("M"), pybind11::arg("N"),

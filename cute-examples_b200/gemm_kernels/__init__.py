@@ -35,6 +35,7 @@ set_option = _C.set_option
 set_trace_buffer = _C.set_trace_buffer
 describe_config = _C.describe_config
 describe_plan = _C.describe_plan
+describe_lora_plan = _C.describe_lora_plan
 select_config = _C.select_config
 workspace_bytes = _C.workspace_bytes
 num_sms = _C.num_sms
@@ -161,5 +162,5 @@ from .nsplit import FusedNSplit, NSplitPlan, fanout_pointers, gemm_tn_nsplit, sh
 
 __all__ = [
     "gemm_tn_test", "gemm_tn", "gemm_nn", "gemm", "LoraPlan", "gemm_lora", "gemm_lora_backward", "HostGemm", "gemm_tn_fanout", "gemm_tn_nsplit", "FusedNSplit", "NSplitPlan", "shard_rows", "device_status",
-    "init", "set_option", "set_trace_buffer", "trace_launch", "describe_config", "describe_plan", "select_config", "workspace_bytes", "num_sms", "LIBRARY_PATH",
+    "init", "set_option", "set_trace_buffer", "trace_launch", "describe_config", "describe_plan", "describe_lora_plan", "select_config", "workspace_bytes", "num_sms", "LIBRARY_PATH",
 ]

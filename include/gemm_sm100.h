@@ -335,6 +335,11 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
                              int recompute_low, void* d_low, long ld_d_low, void* dA, long ld_da, void* d_down, void* d_up,
                              void* cuda_stream, int* cuda_error_out);
 
+/* Writes what gemm_sm100_lora (gradient = 0) or the product dA of gemm_sm100_lora_backward (gradient = 1) would do for this
+ * problem on the current device: "few rows: ", "less than a wave: " or "planner: " for what chose it, then the words of
+ * gemm_sm100_describe_plan. */
+int gemm_sm100_lora_describe_plan(int M, int N, int K, int R, int adapters, int gradient, char* buf, size_t buf_bytes);
+
 /* Static, human-readable name of a return code. */
 const char* gemm_sm100_error_string(int code);
 

@@ -729,3 +729,14 @@ def test_columns_that_are_no_multiple_of_8(gk, M, N, form):
     assert bool((wide[:, N:] == 3).all()) and bool((wide[M:] == 3).all()) and bool((line[M * N:] == 3).all())
     again = forward_only(gk, t)
     assert torch.equal(got, again)
+
+
+def test_widest_output_of_less_than_a_wave(gk):
+    """36 pair tiles in one tile row, the fewest that such an output of at most 256 rows keeps whole."""
+    t = make(256, 9216, 128, 16, 9, torch.bfloat16, 800, id_pattern("random", 256, 9, 8))
+    assert gk.describe_lora_plan(256, 9216, 128, 16, 9).startswith("less than a wave: config=0 ")
+    got = run_all(gk, t)
+    res, tol = want(t)
+    for name, value in got.items():
+        check(name, value, res, tol)
+    gk.device_status()

@@ -162,3 +162,36 @@ def test_backward_refuses_what_recomputing_needs(lora, changes, want):
     err = I(0)
     assert lora.gemm_sm100_lora_backward(ctypes.byref(good(**changes)), 0x6000, 64, 0x7000, 16, 1, None, 16, None, 128, None, 0xB000,
                                          None, ctypes.byref(err)) == want
+
+
+@pytest.mark.parametrize("shape,gradient,chosen", [
+    # M, N, K, R, adapters of the products, and what carries them out on 148 SMs; every branch of both rules has a line, and each
+    # of these shapes is also multiplied on the GPU
+    ((5, 4096, 512, 16, 5), False, "few rows: config=13 ctas=64"), ((40, 2048, 1024, 24, 40), False, "few rows: config=14 ctas=32"),
+    ((100, 9600, 256, 8, 60), False, "few rows: config=12 ctas=75"), ((128, 1152, 4096, 16, 9), False, "few rows: config=12/4 ctas=36"),
+    ((64, 4096, 8448, 16, 3), False, "few rows: config=2/4 ctas=64"), ((9, 136, 8192, 16, 9), False, "few rows: config=12/4 ctas=8"),
+    ((256, 9216, 128, 16, 9), False, "less than a wave: config=0 ctas=72"), ((300, 4104, 2000, 24, 30), False, "less than a wave: config=0 ctas=68"),
+    ((256, 4480, 8192, 8, 5), False, "less than a wave: config=11 ctas=70"), ((300, 1000, 4096, 24, 30), False, "less than a wave: config=11/2 ctas=64"),
+    ((300, 1000, 4096, 24, 30), True, "less than a wave: config=0 ctas=64"), ((250, 264, 8704, 16, 9), True, "less than a wave: config=0 ctas=68"),
+    ((300, 4104, 2000, 24, 30), True, "less than a wave: config=0/2 ctas=64"), ((520, 8200, 640, 16, 12), True, "less than a wave: config=2/4 ctas=60"),
+    ((256, 8704, 128, 16, 9), False, "planner"), ((2048, 4096, 4096, 32, 8), False, "planner"), ((40, 264, 200, 24, 12), False, "planner"),
+    ((256, 9216, 128, 16, 9), True, "planner"),
+])
+def test_chosen_tiles(shape, gradient, chosen):
+    import re
+
+    import gemm_kernels as gk
+
+    rule, words = gk.describe_lora_plan(*shape, gradient=gradient).split(": ", 1)
+    cut = re.search(r"cut into (\d+) K ranges", words)
+    got = f"{rule}: config={re.search(r'config=([0-9]+)', words)[1]}{'/' + cut[1] if cut else ''} ctas={re.search(r'ctas=([0-9]+)', words)[1]}"
+    assert rule == "planner" if chosen == "planner" else got == chosen, got
+
+
+@pytest.mark.parametrize("shape,gradient", [((0, 64, 64, 8, 1), False), ((8, 0, 64, 8, 1), False), ((8, 64, 60, 8, 1), False),
+                                            ((8, 64, 64, 12, 1), False), ((8, 64, 64, 8, 0), False), ((8, 60, 64, 8, 1), True)])
+def test_chosen_tiles_refuses(shape, gradient):
+    import gemm_kernels as gk
+
+    with pytest.raises(RuntimeError, match="bad shape"):
+        gk.describe_lora_plan(*shape, gradient=gradient)
