@@ -238,7 +238,9 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
   return true;
 }
 
-// Tiles for more than 128 rows whose output still is less than a wave.  The planner counts on all SMs, but the kernel
+// Tiles for 129 to 1024 rows whose output still is less than a wave (at most four tile rows, so that every count of tiles below
+// means hundreds of columns; with more and narrower rows the same counts lost up to 13 %: 9000 x 64 x 512 36.4 -> 41.1,
+// 2048 x 1024 x 1024 30.7 -> 32.4).  The planner counts on all SMs, but the kernel
 // of the low rows still holds some when this one starts: CTAs beyond about 100 (fewer for clusters, which want neighbouring
 // SMs) wait for it, and the whole product with them.  About half of the SMs, busy from the start, are then the
 // better choice.  Forced runs of every configuration (M 129 to 1024, output columns 512 to 12288, K 512 to 16384), and the choice below
@@ -260,7 +262,7 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
 //  * 12, K from 4096: 128 x 128 tiles cut in four (512 x 768 x 8192 42.8, 42.5, 48.0 -> 38.9, 39.0, 49.6; 256 x 1536 x 8192 37.1, 38.1, 47.6
 //    -> 38.8, 39.5, 41.0).
 bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) {
-  if (M <= 128 || choice_forced()) return false;
+  if (M <= 128 || M > 1024 || choice_forced()) return false;
   const long rows = ceil_div(M, 256), wide = rows * ceil_div(N, 256), narrow = rows * ceil_div(N, 128);
   const long half = sm_count / 4;                          // pair tiles on half of the SMs
   int config = -1, factor = 1;

@@ -195,3 +195,12 @@ def test_chosen_tiles_refuses(shape, gradient):
 
     with pytest.raises(RuntimeError, match="bad shape"):
         gk.describe_lora_plan(*shape, gradient=gradient)
+
+
+@pytest.mark.parametrize("shape,gradient", [((8192, 64, 1024, 64, 1), False), ((9000, 64, 512, 16, 16), False), ((4096, 64, 8192, 32, 4), False),
+                                            ((2048, 1024, 1024, 32, 4), False), ((9000, 1024, 64, 64, 1), True), ((2000, 16384, 256, 16, 16), True),
+                                            ((1025, 2048, 512, 16, 4), False)])
+def test_many_rows_are_left_to_the_planner(shape, gradient):
+    import gemm_kernels as gk
+
+    assert gk.describe_lora_plan(*shape, gradient=gradient).startswith("planner: ")
