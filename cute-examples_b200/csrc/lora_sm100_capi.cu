@@ -259,8 +259,8 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
 //  * 68 to 74 CTAs of 256 x 128 pair tiles, K from 8192: those, whole (256 x 4608 x 8192 58.0, 58.9, 60.5 -> 51.4, 52.1, 54.8);
 //  * 13 to 20 such tiles, K from 4096: cut in two (512 x 1024 x 4096 40.4, 39.6, 42.6 -> 34.6, 34.8, 36.2; 256 x 2048 x 14336 56.3, 57.4,
 //    62.5 -> 53.9, 54.2, 56.3);
-//  * 12, K from 4096: 128 x 128 tiles cut in four (512 x 768 x 8192 42.8, 42.5, 48.0 -> 38.9, 39.0, 49.6; 256 x 1536 x 8192 37.1, 38.1, 47.6
-//    -> 38.8, 39.5, 41.0).
+// (12 such tiles stay with the planner: 128 x 128 tiles cut in four are up to 17 % faster or 7 % slower without a size that
+// tells which: 256 x 1536 x 14336 42.8, 43.8, 57.9 -> 45.8, 46.5, 48.3; 512 x 768 x 14336 49.4, 48.8, 58.3 -> 44.6, 44.9, 60.8.)
 bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) {
   if (M <= 128 || M > 1024 || choice_forced()) return false;
   const long rows = ceil_div(M, 256), wide = rows * ceil_div(N, 256), narrow = rows * ceil_div(N, 128);
@@ -285,9 +285,6 @@ bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) 
     } else if (narrow >= 13 && narrow <= 20 && K >= 4096) {
       config = 11;
       factor = 2;
-    } else if (narrow == 12 && K >= 4096) {
-      config = 12;
-      factor = 4;
     }
   }
   if (config < 0) return false;

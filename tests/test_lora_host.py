@@ -204,3 +204,10 @@ def test_many_rows_are_left_to_the_planner(shape, gradient):
     import gemm_kernels as gk
 
     assert gk.describe_lora_plan(*shape, gradient=gradient).startswith("planner: ")
+
+
+@pytest.mark.parametrize("shape", [(256, 1536, 8192, 16, 16), (512, 768, 8192, 64, 1), (768, 512, 4096, 32, 4), (600, 504, 4096, 16, 3)])
+def test_twelve_narrow_tiles_are_left_to_the_planner(shape):
+    import gemm_kernels as gk
+
+    assert gk.describe_lora_plan(*shape).startswith("planner: ")
