@@ -247,15 +247,18 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
 // against the planner's as part of a longer sequence (dA: a training step; forward: behind a 2048 x 2048 x 2048 GEMM of 17 us), in us
 // for one adapter of rank 64 / runs of four of rank 32 / 16 of rank 16 in every tile.  M x output columns x K:
 //  [K,N] operand (dA):
-//  * 64 to 74 CTAs of 256 x 256 pair tiles: those, whole; with 64 to 66 the planner's clusters of four all fit and are as
-//    good from K = 8192 (512 x 4352 x 1024 46.1, 41.7, 49.3 -> 37.5, 33.4, 40.4; 256 x 8704 x 4096 74.7, 74.8, 89.1 -> 70.9, 70.1, 80.2);
+//  * 64 to 74 CTAs of 256 x 256 pair tiles: those, whole (512 x 4352 x 1024 46.1, 41.7, 49.3 -> 37.5, 33.4, 40.4; 256 x 8704 x 4096
+//    74.7, 74.8, 89.1 -> 70.9, 70.1, 80.2); with 64 to 66 the planner's clusters of four all fit and are as good from K = 5120.
+//    At K = 4096 twelve of 15 lines are faster whole, three slower (700 x 2688 61.3, 56.6, 73.1 -> 56.7, 52.7, 66.1; 512 x 4096
+//    60.7, 56.0, 74.0 -> 63.0, 58.0, 67.6; 1024 x 2048 64.9, 58.9, 69.4 -> 61.2, 55.4, 72.2);
 //  * 14 to 16 such tiles, K 4096 up to 8192: cut in two (1024 x 1024 x 4096 58.0, 50.1, 59.7 -> 51.6, 46.9, 58.0; at K = 8192 2 % slower,
 //    with 18 to 28 tiles 3 to 8 %);
 //  * 7 to 9, more than 256 rows, K from 8192: 128 x 256 tiles cut in four instead of the planner's clusters of eight (1024 x 512 x
 //    8192 62.4, 55.9, 85.0 -> 59.2, 53.6, 84.6; 512 x 1024 x 8192 52.6, 48.8, 68.6 -> 52.4, 48.9, 59.9).
 //  [N,K] operand (K a multiple of 64 for 128-column tiles):
 //  * up to 74 CTAs of 256 x 256 pair tiles, from 64 to 72 CTAs on by the rows, K at most 2048 (1024 from 513 rows on): those,
-//    whole (512 x 4352 x 1024 31.5, 30.7, 34.5 -> 29.2, 29.0, 31.9; 1024 x 2048 x 2048 with 16 adapters 38.4 -> 41.7);
+//    whole (512 x 4352 x 1024 31.5, 30.7, 34.5 -> 29.2, 29.0, 31.9; 1024 x 2048 x 1024 31.1, 30.1, 34.9 -> 29.1, 28.7, 35.9, and with
+//    16 adapters at K = 2048 38.4 -> 41.7);
 //  * 68 to 74 CTAs of 256 x 128 pair tiles, K from 8192: those, whole (256 x 4608 x 8192 58.0, 58.9, 60.5 -> 51.4, 52.1, 54.8);
 //  * 13 to 20 such tiles, K from 4096: cut in two (512 x 1024 x 4096 40.4, 39.6, 42.6 -> 34.6, 34.8, 36.2; 256 x 2048 x 14336 56.3, 57.4,
 //    62.5 -> 53.9, 54.2, 56.3);
