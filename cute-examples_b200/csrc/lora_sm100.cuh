@@ -174,7 +174,7 @@ struct LowParams {
   unsigned long long timeout_ns;
 };
 
-// kDeep: six stages and one CTA per SM instead of three and two, for launches that do not fill the SMs twice.
+// kDeep: six stages and one CTA per SM instead of three and two (chosen by low_grid).
 template <bool kDeep>
 struct LowConfig {
   static constexpr int kThreads = 192;                 // producer, MMA issuer, four epilogue warps

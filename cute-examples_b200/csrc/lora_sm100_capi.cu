@@ -317,12 +317,10 @@ Plan product_plan(int M, int N, int K, bool b_is_kn, int R, int adapters, int sm
 }
 
 template <bool kIsBf16>
-int launch_product(const Problem& p, const AdapterOperands& o, cudaStream_t stream, int* cuda_error_out) {
+int launch_product(const Problem& p, const AdapterOperands& o, const Plan& plan, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   const int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
-  const char* rule;
-  const Plan plan = product_plan(p.M, p.N, p.K, p.b_is_kn, o.R, o.adapters, st->sm_count, &rule);
   if (p.b_is_kn) {
     switch (plan.config) {
       case 0: return launch_product_config<0, kIsBf16, true>(p, o, plan, *st, stream, cuda_error_out);
@@ -390,6 +388,11 @@ cudaError_t allow_low_pair(DeviceState& st) {
   return allow_smem(lora_low_pair_kernel<kIsBf16, kDeep>, LowConfig<kDeep>::kSmemBytes, allowed, st.device);
 }
 
+void low_shape(LowParams* p, int M, int R, int L, bool rank_inner) {
+  p->M = M, p->R = R, p->L = L;
+  p->group_slots = 128 / (rank_inner ? static_cast<int>(ceil_div(R, rank_chunk(R))) * rank_chunk(R) : R);
+}
+
 // Parameters of the low-rank rows of P [M, L] through W: down [adapters, R, L], or (rank_inner) up [adapters, L, R].
 int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_inner, const void* P, long ldp, const void* W,
                long ld_w, long stride_w, int L, void* out, long ld_out, const DeviceState& st, int* cuda_error_out) {
@@ -407,8 +410,7 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
   p.scale = a.scale;
   p.out = out;
   p.ld_out = ld_out;
-  p.M = a.M, p.R = a.R, p.L = L;
-  p.group_slots = 128 / (rank_inner ? static_cast<int>(ceil_div(a.R, rank_chunk(a.R))) * rank_chunk(a.R) : a.R);
+  low_shape(&p, a.M, a.R, L, rank_inner);
   p.status = st.status_ptr;
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
   return GEMM_SM100_OK;
@@ -419,9 +421,9 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
 // known on the device only: a CTA without a group has nothing to do).  The cut is the order in which a row is added up,
 // so it depends on the problem alone and not on what shares its launch: a backward pass gives the same bits
 // whether the low rows were kept or not, and whichever gradients are wanted.
-void cut_low(LowParams* p, int adapters, const DeviceState& st) {
+void cut_low(LowParams* p, int adapters, int sm_count) {
   const int M = p->M;
-  const long tiles = ceil_div(M, 128), k_blocks = ceil_div(p->L, 64), room = 2L * st.sm_count;
+  const long tiles = ceil_div(M, 128), k_blocks = ceil_div(p->L, 64), room = 2L * sm_count;
   p->splits = 8;
   while (p->splits > 1 && (tiles * p->splits > room || p->splits > k_blocks)) p->splits /= 2;
   p->workers = p->splits;
@@ -435,21 +437,28 @@ void cut_low(LowParams* p, int adapters, const DeviceState& st) {
 // CTAs of a launch that `problems` share.  Two that do not fit on the SMs together get half of the CTAs each, with up to two
 // partial sums per CTA; whole, in two waves, the backward pass with recomputed low rows takes 138.5 instead of 134.7 us
 // (4096 x 4096 x 4096, eight adapters of rank 64) and 94.1 instead of 89.3 (2048 x 4096 x 4096, 16 of rank 32 in every tile).
+//
+// Deep ring (six stages, one CTA per SM) or short (three, two CTAs): the deep one is faster by itself, but takes twice the SMs,
+// and the product kernel behind (`behind` CTAs of one per SM, 0 for none) starts on those that are left.  So it is taken where the
+// product would have to wait in any case and the launch keeps to half of the SMs: 12 to 148 tiles of M 16 to 1100, N 1024 to 8192,
+// K 4096 to 14336, the 47 such shapes of a sweep behind a GEMM 0 to 9 % faster, by themselves 0 to 11 % (64 x 8192 x 14336, 16 adapters
+// of rank 64 66.7 -> 62.0 us; 1100 x 2048 x 8192 with one 51.7 -> 49.7), none slower than 0.4 %.  Elsewhere it costs up to 30 %: 700 x 1024 x
+// 8192 with one adapter 26.1 -> 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7, 64 x 4096 x 14336 with 32 50.5 -> 56.6.  (Not
+// measured below eight K blocks per CTA.)
 struct LowGrid {
   int cluster;           // CTAs of a cluster
   long ctas[2];          // of each problem
   bool deep;
 };
-LowGrid low_grid(LowParams* const* params, int problems, int adapters, const DeviceState& st) {
+LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behind, int sm_count) {
   LowGrid g = {1, {0, 0}, false};
   const long tiles = ceil_div(params[0]->M, 128);
   long wanted = 0;
   for (int i = 0; i < problems; ++i) {
-    cut_low(params[i], adapters, st);
+    cut_low(params[i], adapters, sm_count);
     wanted += tiles * params[i]->splits * params[i]->groups;
   }
-  const bool fold = problems > 1 && wanted > 2L * st.sm_count && params[0]->R <= LowConfig<false>::kMaxFoldedRank;
-  long busy = 0;
+  const bool fold = problems > 1 && wanted > 2L * sm_count && params[0]->R <= LowConfig<false>::kMaxFoldedRank;
   bool long_runs = false;
   for (int i = 0; i < problems; ++i) {
     LowParams& p = *params[i];
@@ -458,24 +467,20 @@ LowGrid low_grid(LowParams* const* params, int problems, int adapters, const Dev
     else if (fold && p.splits > 1)
       p.workers = p.splits / 2;
     if (p.workers > g.cluster) g.cluster = p.workers;
-    if (ceil_div(p.L, 64) >= 12L * p.workers) long_runs = true;
+    if (ceil_div(p.L, 64) >= 8L * p.workers) long_runs = true;
   }
+  long total = 0;
   for (int i = 0; i < problems; ++i) {
-    const int clusters = params[i]->clusters;
-    g.ctas[i] = tiles * clusters * g.cluster;
-    busy += tiles * g.cluster * (clusters < 2 ? clusters : 2);
+    g.ctas[i] = tiles * params[i]->clusters * g.cluster;
+    total += g.ctas[i];
   }
-  // The deep ring for long runs of K blocks, when that leaves no SM with two CTAs, or hardly (every further group may turn
-  // out to be empty): 64 x 4096 x 14336 with 32 adapters of rank 64 takes 45.8 us that way, 49.2 with the short ring.  With few
-  // K blocks the SMs it takes from the product kernel behind cost more: 128 x 14336 x 4096 with 64 adapters of
-  // rank 16 takes 44.6 us deep and 40.7 short (8 blocks per CTA).
-  g.deep = long_runs && !fold && busy <= st.sm_count;
+  g.deep = long_runs && 2 * total <= sm_count && total + 2L * behind > 2L * sm_count;
   return g;
 }
 
 template <bool kIsBf16, bool kRankInner>
 int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
-               long ld_out, cudaStream_t stream, int* cuda_error_out) {
+               long ld_out, int behind, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
@@ -483,7 +488,7 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
   rc = low_params(&p, a, kRankInner, P, ldp, W, ld_w, stride_w, L, out, ld_out, *st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   LowParams* const one[1] = {&p};
-  const LowGrid g = low_grid(one, 1, a.adapters, *st);
+  const LowGrid g = low_grid(one, 1, a.adapters, behind, st->sm_count);
   const long ctas = g.ctas[0];
   cudaError_t e = g.deep ? allow_low<kIsBf16, kRankInner, true>(*st) : allow_low<kIsBf16, kRankInner, false>(*st);
   if (e == cudaSuccess)
@@ -497,7 +502,7 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
 // low (from A and down) and d_low (from dC and up) in one launch.
 template <bool kIsBf16>
 int launch_low_pair(const gemm_sm100_lora_args& a, void* low, long ld_low, const void* dC, long ld_dc, void* d_low, long ld_d_low,
-                    cudaStream_t stream, int* cuda_error_out) {
+                    int behind, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
@@ -507,7 +512,7 @@ int launch_low_pair(const gemm_sm100_lora_args& a, void* low, long ld_low, const
     rc = low_params(&q, a, true, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low, ld_d_low, *st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   LowParams* const both[2] = {&p, &q};
-  const LowGrid g = low_grid(both, 2, a.adapters, *st);
+  const LowGrid g = low_grid(both, 2, a.adapters, behind, st->sm_count);
   const int first = static_cast<int>(g.ctas[0]);
   const long ctas = g.ctas[0] + g.ctas[1];
   cudaError_t e = g.deep ? allow_low_pair<kIsBf16, true>(*st) : allow_low_pair<kIsBf16, false>(*st);
@@ -598,6 +603,15 @@ int prepare_type(DeviceState& st, int* cuda_error_out, std::integer_sequence<int
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
 
+// The low-rank rows of A; the caller has checked what all calls share.
+int low_rows(const gemm_sm100_lora_args& a, void* low, long ld_low, int behind, cudaStream_t stream, int* cuda_error_out) {
+  if (!a.plan) return GEMM_SM100_ERR_NULL_POINTER;
+  int rc = check_matrix(a.A, a.K, a.lda);
+  if (rc || (rc = check_down(a)) || (rc = check_matrix(low, a.R, ld_low))) return rc;
+  return (a.dtype == GEMM_SM100_BF16 ? launch_low<true, false> : launch_low<false, false>)(
+      a, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low, ld_low, behind, stream, cuda_error_out);
+}
+
 }  // namespace
 
 namespace gemm_sm100 {
@@ -645,22 +659,25 @@ int gemm_sm100_lora_describe_plan(int M, int N, int K, int R, int adapters, int 
   // (dA is an [M, K] output with N contracted)
   const Plan plan = product_plan(M, gradient ? K : N, gradient ? N : K, gradient != 0, R, adapters, current_sm_count(), &rule);
   const int n = std::snprintf(buf, buf_bytes, "%s: ", rule);
-  if (n > 0 && static_cast<size_t>(n) < buf_bytes) describe(plan, gradient ? K : N, buf + n, buf_bytes - n);
+  if (n <= 0 || static_cast<size_t>(n) >= buf_bytes) return GEMM_SM100_OK;
+  describe(plan, gradient ? K : N, buf + n, buf_bytes - n);
+  LowParams low;
+  std::memset(&low, 0, sizeof(low));
+  low_shape(&low, M, R, gradient ? N : K, gradient != 0);
+  LowParams* const one[1] = {&low};
+  const LowGrid grid = low_grid(one, 1, adapters, plan.ctas, current_sm_count());
+  const size_t used = std::strlen(buf);
+  std::snprintf(buf + used, buf_bytes - used, "; low rows: %ld ctas in clusters of %d, %s ring", grid.ctas[0], grid.cluster,
+                grid.deep ? "deep" : "short");
   return GEMM_SM100_OK;
 }
 
 int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low, void* cuda_stream, int* cuda_error_out) {
   if (cuda_error_out) *cuda_error_out = 0;
   if (!args) return GEMM_SM100_ERR_NULL_POINTER;
-  const gemm_sm100_lora_args& a = *args;
-  int rc = check_common(a);
-  if (rc != GEMM_SM100_OK) return rc;
-  if (a.M == 0) return GEMM_SM100_OK;
-  if (!a.plan) return GEMM_SM100_ERR_NULL_POINTER;
-  if ((rc = check_matrix(a.A, a.K, a.lda)) || (rc = check_down(a)) || (rc = check_matrix(low, a.R, ld_low))) return rc;
-  auto launch = a.dtype == GEMM_SM100_BF16 ? launch_low<true, false> : launch_low<false, false>;
-  return launch(a, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low, ld_low, static_cast<cudaStream_t>(cuda_stream),
-                cuda_error_out);
+  const int rc = check_common(*args);
+  if (rc != GEMM_SM100_OK || args->M == 0) return rc;
+  return low_rows(*args, low, ld_low, /*behind=*/0, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
 }
 
 int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* low, long ld_low, void* cuda_stream,
@@ -672,12 +689,14 @@ int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* l
   if (rc != GEMM_SM100_OK) return rc;
   if (a.M == 0) return GEMM_SM100_OK;
   if ((rc = check_matrix(a.B, a.K, a.ldb)) || (rc = check_up(a)) || (rc = check_matrix(C, a.N, ldc))) return rc;
-  rc = gemm_sm100_lora_low(args, low, ld_low, cuda_stream, cuda_error_out);
+  const char* rule;
+  const Plan plan = product_plan(a.M, a.N, a.K, /*b_is_kn=*/false, a.R, a.adapters, current_sm_count(), &rule);
+  rc = low_rows(a, low, ld_low, plan.ctas, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   const Problem p{a.A, a.B, C, a.M, a.N, a.K, a.lda, a.ldb, ldc, a.dtype};
   const AdapterOperands o{low, ld_low, a.up, a.ld_up, a.stride_up, a.R, a.adapters, a.plan};
   return (a.dtype == GEMM_SM100_BF16 ? launch_product<true> : launch_product<false>)(
-      p, o, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
+      p, o, plan, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
 }
 
 int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, long ld_dc, void* low, long ld_low,
@@ -707,22 +726,27 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
   const bool bf16 = a.dtype == GEMM_SM100_BF16;
   const bool again = recompute_low != 0 && d_up != nullptr;
   if (again && ((rc = check_matrix(a.A, a.K, a.lda)) || (rc = check_down(a)))) return rc;
+  Plan plan;
+  if (dA) {
+    const char* rule;
+    plan = product_plan(a.M, a.K, a.N, /*b_is_kn=*/true, a.R, a.adapters, current_sm_count(), &rule);
+  }
   if (dA || d_down) {
     if ((rc = check_up(a)) || (rc = check_matrix(d_low, a.R, ld_d_low))) return rc;
     if (again)
-      rc = (bf16 ? launch_low_pair<true> : launch_low_pair<false>)(a, low, ld_low, dC, ld_dc, d_low, ld_d_low, stream, cuda_error_out);
+      rc = (bf16 ? launch_low_pair<true> : launch_low_pair<false>)(a, low, ld_low, dC, ld_dc, d_low, ld_d_low, plan.ctas, stream,
+                                                                       cuda_error_out);
     else
       rc = (bf16 ? launch_low<true, true> : launch_low<false, true>)(a, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low,
-                                                                     ld_d_low, stream, cuda_error_out);
+                                                                     ld_d_low, plan.ctas, stream, cuda_error_out);
   } else if (again) {
-    rc = (bf16 ? launch_low<true, false> : launch_low<false, false>)(a, a.A, a.lda, a.down, a.ld_down, a.stride_down, a.K, low,
-                                                                     ld_low, stream, cuda_error_out);
+    rc = low_rows(a, low, ld_low, /*behind=*/0, stream, cuda_error_out);
   }
   if (rc != GEMM_SM100_OK) return rc;
   if (dA) {
     const Problem p{dC, a.B, dA, a.M, a.K, a.N, ld_dc, a.ldb, ld_da, a.dtype, /*b_is_kn=*/true};
     const AdapterOperands o{d_low, ld_d_low, a.down, a.ld_down, a.stride_down, a.R, a.adapters, a.plan};
-    rc = (bf16 ? launch_product<true> : launch_product<false>)(p, o, stream, cuda_error_out);
+    rc = (bf16 ? launch_product<true> : launch_product<false>)(p, o, plan, stream, cuda_error_out);
     if (rc != GEMM_SM100_OK) return rc;
   }
   if (!d_down && !d_up) return GEMM_SM100_OK;

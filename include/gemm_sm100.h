@@ -337,7 +337,7 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
 
 /* Writes what gemm_sm100_lora (gradient = 0) or the product dA of gemm_sm100_lora_backward (gradient = 1) would do for this
  * problem on the current device: "few rows: ", "less than a wave: " or "planner: " for what chose it, then the words of
- * gemm_sm100_describe_plan. */
+ * gemm_sm100_describe_plan, then the launch that computes low (with gradient = 1 d_low, where low was kept). */
 int gemm_sm100_lora_describe_plan(int M, int N, int K, int R, int adapters, int gradient, char* buf, size_t buf_bytes);
 
 /* Static, human-readable name of a return code. */

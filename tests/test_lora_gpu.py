@@ -740,3 +740,21 @@ def test_widest_output_of_less_than_a_wave(gk):
     for name, value in got.items():
         check(name, value, res, tol)
     gk.device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K,R,G,kind,deep", [(16, 8192, 4096, 64, 16, "own", "forward"), (1100, 4096, 2048, 64, 1, "one", "backward"),
+                                                 (500, 8192, 2048, 40, 2, "runs", "both in one launch")])
+def test_low_rows_through_the_deep_ring(gk, M, N, K, R, G, kind, deep, dtype):
+    """The low rows of a forward pass, of a backward pass that kept them, and both kinds in one launch (64 CTAs)."""
+    t = make(M, N, K, R, G, dtype, 900 + M, id_pattern(kind, M, G, 3))
+    if deep in ("forward", "backward"):
+        assert gk.describe_lora_plan(M, N, K, R, G, gradient=deep == "backward").endswith("deep ring")
+    res, tol = want(t)
+    for name, value in run_all(gk, t).items():
+        check(name, value, res, tol)
+    plan = gk.LoraPlan(t["ids"], G)
+    grads = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"])
+    for name, value in zip(("dA", "d_down", "d_up"), grads):
+        check(name, value, res, tol)
+    gk.device_status()

@@ -211,3 +211,17 @@ def test_twelve_narrow_tiles_are_left_to_the_planner(shape):
     import gemm_kernels as gk
 
     assert gk.describe_lora_plan(*shape).startswith("planner: ")
+
+
+@pytest.mark.parametrize("shape,gradient,low", [
+    # the deep ring only where the product behind finds no room beside the short one either
+    ((64, 8192, 14336, 64, 16), False, "64 ctas in clusters of 8, deep"), ((1100, 2048, 8192, 64, 1), False, "72 ctas in clusters of 8, deep"),
+    ((16, 8192, 8192, 64, 8), False, "32 ctas in clusters of 8, short"), ((700, 1024, 8192, 64, 1), False, "48 ctas in clusters of 8, short"),
+    ((512, 4096, 8192, 64, 1), False, "32 ctas in clusters of 8, short"), ((64, 4096, 14336, 64, 32), False, "128 ctas in clusters of 8, short"),
+    ((128, 14336, 4096, 16, 64), False, "64 ctas in clusters of 8, short"), ((1100, 8192, 2048, 64, 1), True, "72 ctas in clusters of 8, deep"),
+    ((64, 14336, 2048, 64, 16), True, "64 ctas in clusters of 8, short"),
+])
+def test_ring_of_the_low_rows(shape, gradient, low):
+    import gemm_kernels as gk
+
+    assert gk.describe_lora_plan(*shape, gradient=gradient).endswith(f"; low rows: {low} ring")
