@@ -204,6 +204,31 @@ bool choice_forced() {
   return g_opt_tile_config >= 0 || g_opt_split_k >= 0 || g_opt_sk_cluster >= 0 || g_opt_tiles_n > 0 || g_opt_max_ctas > 0;
 }
 
+// ---- low-rank rows: how they are cut
+void low_shape(LowParams* p, int M, int R, int L, bool rank_inner) {
+  p->M = M, p->R = R, p->L = L;
+  p->group_slots = 128 / (rank_inner ? static_cast<int>(ceil_div(R, rank_chunk(R))) * rank_chunk(R) : R);
+}
+
+// How a problem is cut.  Two CTAs fit on an SM.  L is cut over as many CTAs of a cluster as leave them all at work at once;
+// what is free beyond that takes groups of adapters of the same tile (how many a tile really has is
+// known on the device only: a CTA without a group has nothing to do).  The cut is the order in which a row is added up,
+// so it depends on the problem alone and not on what shares its launch: a backward pass gives the same bits
+// whether the low rows were kept or not, and whichever gradients are wanted.
+void cut_low(LowParams* p, int adapters, int sm_count) {
+  const int M = p->M;
+  const long tiles = ceil_div(M, 128), k_blocks = ceil_div(p->L, 64), room = 2L * sm_count;
+  p->splits = 8;
+  while (p->splits > 1 && (tiles * p->splits > room || p->splits > k_blocks)) p->splits /= 2;
+  p->workers = p->splits;
+  const long tile_rows = M < kLoraTileRows ? M : kLoraTileRows;
+  const long most_groups = ceil_div(adapters < tile_rows ? adapters : tile_rows, p->group_slots);
+  const long groups = room / (tiles * p->splits);
+  p->groups = static_cast<int>(groups < 1 ? 1 : (groups > most_groups ? most_groups : groups));
+  p->clusters = p->groups;
+}
+
+// ---- product: which tiles
 // Tiles for few rows (at most 128, K a multiple of 64), where the shared planner, which does not know what adapter
 // stages cost on a tile, is up to 40 % off.  From forced runs of every configuration (M 2 to 128, N 128 to 16384, K 256 to 28672,
 // 4 to 16 adapters of rank 16 and 64), planner's choice against this one:
@@ -211,11 +236,14 @@ bool choice_forced() {
 //    30.7 us, 64 x 12288 x 8192 59.8 / 57.0, 4 x 16384 x 2048 19.6 / 17.7; 64-column tiles would need two waves);
 //  * fewer, and K at most twice N or at most 2048: 64-column tiles, whole (1 x 4096 x 4096 18.7 / 14.9, 64 x 4096 x 4096 23.2 /
 //    18.4, 16 x 5120 x 8192 34.2 / 28.8, 2 x 512 x 2048 12.5 / 9.3, 64 x 256 x 256 10.6 / 9.3; for 65 to 128 rows there is no such tile);
-//  * K longer: 128-column tiles cut in four while their clusters fit at once (16 x 2048 x 8192 29.6 / 20.3, 32 x 3584 x 28672 72.7 /
-//    48.4), else 256-column tiles cut in four (8 x 4096 x 14336 41.5 / 35.9, 128 x 5120 x 28672 76.5 / 70.0).  Where the
-//    clusters of the narrow tiles just fit, many adapter ranks (`adapter_ranks`: those that a tile's rows can use, all
-//    adapters together) want their twice as many CTAs: 64 x 4096 x 14336 with 32 adapters of rank 64 51.5 / 45.0.
-bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* out) {
+//  * K longer: tiles cut in four, inside clusters.  The kernel of the low rows (`low_ctas`, two on an SM) still holds SMs when
+//    this one starts, and what has no room beside it waits for it.  So 128-column tiles where they fit into seven eighths of
+//    the SMs together with it (the rest is left over in the GPCs: 29 tiles with 32 CTAs are 9 % faster by themselves, 30 of them
+//    13 to 19 % slower), else 256-column tiles where those do (64 x 3584 x 14336 with 16 adapters of rank 64 45.8 against 38.5 us),
+//    else, when either has to wait, up to 33 128-column tiles again (64 x 4096 x 14336 with 64 adapters 65.9 / 59.0).  Of 756 lines
+//    (M 16 to 128, N 512 to 4224, K 8704 to 28672, 1 to 64 adapters of rank 16 or 64, by themselves and behind a GEMM) the choice is on
+//    average 0.3 % slower than the better of the two.
+bool few_row_plan(int M, int N, int K, long low_ctas, int sm_count, Plan* out) {
   if (M > 128 || K % 64 != 0 || choice_forced()) return false;
   const long t64 = ceil_div(N, 64), t128 = ceil_div(N, 128), t256 = ceil_div(N, 256);
   Plan plan;
@@ -228,8 +256,9 @@ bool few_row_plan(int M, int N, int K, long adapter_ranks, int sm_count, Plan* o
     plan.config = M <= 16 ? 13 : 14;
     plan.ctas = static_cast<int>(t64);
   } else {
-    if (K < 64 * 32 || t256 > 33) return false;            // eight K blocks each at least, all clusters at once
-    plan.config = t128 <= 28 || (t128 <= 33 && adapter_ranks >= 1024) ? 12 : 2;
+    if (t256 > 33) return false;                           // all clusters at once
+    auto beside = [&](long tiles) { return 4 * tiles + low_ctas / 2 <= sm_count * 7 / 8; };
+    plan.config = beside(t128) || (t128 <= 33 && !beside(t256)) ? 12 : 2;
     plan.split_k = plan.cluster = true;
     plan.split_factor = 4;
     plan.ctas = static_cast<int>((plan.config == 12 ? t128 : t256) * 4);
@@ -308,7 +337,12 @@ bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) 
 Plan product_plan(int M, int N, int K, bool b_is_kn, int R, int adapters, int sm_count, const char** rule) {
   Plan plan;
   *rule = "few rows";
-  if (!b_is_kn && few_row_plan(M, N, K, static_cast<long>(adapters < M ? adapters : M) * R, sm_count, &plan)) return plan;
+  if (!b_is_kn) {
+    LowParams low;
+    low_shape(&low, M, R, K, /*rank_inner=*/false);
+    cut_low(&low, adapters, sm_count);
+    if (few_row_plan(M, N, K, ceil_div(M, 128) * low.splits * low.groups, sm_count, &plan)) return plan;
+  }
   *rule = "less than a wave";
   if (half_wave_plan(M, N, K, b_is_kn, sm_count, &plan)) return plan;
   *rule = "planner";
@@ -388,11 +422,6 @@ cudaError_t allow_low_pair(DeviceState& st) {
   return allow_smem(lora_low_pair_kernel<kIsBf16, kDeep>, LowConfig<kDeep>::kSmemBytes, allowed, st.device);
 }
 
-void low_shape(LowParams* p, int M, int R, int L, bool rank_inner) {
-  p->M = M, p->R = R, p->L = L;
-  p->group_slots = 128 / (rank_inner ? static_cast<int>(ceil_div(R, rank_chunk(R))) * rank_chunk(R) : R);
-}
-
 // Parameters of the low-rank rows of P [M, L] through W: down [adapters, R, L], or (rank_inner) up [adapters, L, R].
 int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_inner, const void* P, long ldp, const void* W,
                long ld_w, long stride_w, int L, void* out, long ld_out, const DeviceState& st, int* cuda_error_out) {
@@ -414,24 +443,6 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
   p.status = st.status_ptr;
   p.timeout_ns = static_cast<unsigned long long>(g_opt_timeout_ms.load()) * 1000000ull;
   return GEMM_SM100_OK;
-}
-
-// How a problem is cut.  Two CTAs fit on an SM.  L is cut over as many CTAs of a cluster as leave them all at work at once;
-// what is free beyond that takes groups of adapters of the same tile (how many a tile really has is
-// known on the device only: a CTA without a group has nothing to do).  The cut is the order in which a row is added up,
-// so it depends on the problem alone and not on what shares its launch: a backward pass gives the same bits
-// whether the low rows were kept or not, and whichever gradients are wanted.
-void cut_low(LowParams* p, int adapters, int sm_count) {
-  const int M = p->M;
-  const long tiles = ceil_div(M, 128), k_blocks = ceil_div(p->L, 64), room = 2L * sm_count;
-  p->splits = 8;
-  while (p->splits > 1 && (tiles * p->splits > room || p->splits > k_blocks)) p->splits /= 2;
-  p->workers = p->splits;
-  const long tile_rows = M < kLoraTileRows ? M : kLoraTileRows;
-  const long most_groups = ceil_div(adapters < tile_rows ? adapters : tile_rows, p->group_slots);
-  const long groups = room / (tiles * p->splits);
-  p->groups = static_cast<int>(groups < 1 ? 1 : (groups > most_groups ? most_groups : groups));
-  p->clusters = p->groups;
 }
 
 // CTAs of a launch that `problems` share.  Two that do not fit on the SMs together get half of the CTAs each, with up to two

@@ -225,3 +225,16 @@ def test_ring_of_the_low_rows(shape, gradient, low):
     import gemm_kernels as gk
 
     assert gk.describe_lora_plan(*shape, gradient=gradient).endswith(f"; low rows: {low} ring")
+
+
+@pytest.mark.parametrize("shape,chosen", [
+    # tiles of few rows and a long K, by the SMs that the low rows' CTAs (two to an SM) leave
+    ((64, 4096, 14336, 64, 32), "config=2 "), ((64, 3584, 14336, 64, 16), "config=2 "), ((64, 3200, 8704, 64, 28), "config=2 "),
+    ((16, 3968, 14336, 16, 1), "config=12 "), ((128, 3584, 14336, 16, 8), "config=12 "), ((64, 4096, 14336, 64, 64), "config=12 "),
+    ((64, 512, 8704, 64, 28), "config=12 "), ((128, 4224, 28672, 16, 1), "config=2 "),
+    ((64, 8448, 17408, 64, 64), "config=2 "),
+])
+def test_few_rows_beside_the_low_rows(shape, chosen):
+    import gemm_kernels as gk
+
+    assert gk.describe_lora_plan(*shape).startswith("few rows: " + chosen)
