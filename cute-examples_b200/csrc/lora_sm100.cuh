@@ -166,7 +166,6 @@ struct LowParams {
   int M, R, L;
   int p_rows;            // rows per box of P: 128, or fewer when M is
   int splits;            // partial sums of a row: L is cut over as many CTAs, or over half of them with two sums each
-  int workers;           // CTAs of the cluster that work (splits or splits / 2); those beyond have nothing to do
   int clusters;          // clusters per tile; the tile's groups are dealt to them
   int group_slots;       // adapters per group
   int groups;            // groups that are taken one to a cluster of `splits` sums; with more, fewer sums of each are formed
@@ -206,7 +205,6 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   const int rank = static_cast<int>(cluster_ctarank());
   uint32_t cluster_size;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_size));
-  const bool idle = rank >= p.workers;                 // (a shared launch has the clusters of the problem that is cut further)
   const int unit = block / static_cast<int>(cluster_size);
   const int tile = unit / p.clusters, group0 = unit % p.clusters;
   WaitCtx ctx{abort_flag, smem_u32(const_cast<const uint32_t*>(abort_flag)), p.status, p.timeout_ns};
@@ -243,15 +241,16 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   // each (one exchange instead of one per group: 2048 x (4096 + 4096), 16 adapters of rank 32 in every tile, 38 us one after
   // another).  `sums` follows from the problem alone, for it is the order in which a row is added up; where the CTAs are
   // half as many, each has every second of its K blocks in a second accumulator.
+  // (All of these are powers of two.  The clusters of a shared launch may be larger than `splits`.)
   int sums = p.splits;
-  while (sums > 1 && p.splits / sums * p.groups < groups) sums /= 2;
-  int parts = sums < p.workers ? sums : p.workers;
-  if (parts == sums && sums > 1 && p.workers / parts * p.clusters < groups) parts /= 2;
-  const int at_once = p.workers / parts;
-  const int part = rank % parts, leader = rank - part;
+  for (int taken = p.groups; sums > 1 && taken < groups; taken *= 2) sums >>= 1;
+  int parts_log = __ffs(min(sums, static_cast<int>(cluster_size))) - 1;
+  if (1 << parts_log == sums && sums > 1 && static_cast<int>(cluster_size >> parts_log) * p.clusters < groups) --parts_log;
+  const int parts = 1 << parts_log, at_once = static_cast<int>(cluster_size >> parts_log);
+  const int part = rank & (parts - 1), leader = rank - part;
   const uint32_t second = parts < sums ? 128u : 0u;    // column of the second accumulator
   // The CTAs of a part take the K blocks in turn: what they read of a row of P at any moment is contiguous.
-  const int steps = (k_blocks - part + parts - 1) / parts;
+  const int steps = (k_blocks - part + parts - 1) >> parts_log;
   const int pitch = R + 4;                             // floats per partial row: 16-byte accesses without bank conflicts
   uint32_t step = 0;                                   // ring position, running on over the groups
   uint32_t parity = 0;
@@ -266,9 +265,9 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
   }
 #pragma unroll 1
   for (int first = group0 * at_once; first < groups; first += p.clusters * at_once) {
-    const int group = first + rank / parts;
+    const int group = first + (rank >> parts_log);
     const int slot0 = group * p.group_slots;
-    const int n_slots = idle ? 0 : min(p.group_slots, slots - slot0);   // (none left: the CTA only takes part in the exchange)
+    const int n_slots = min(p.group_slots, slots - slot0);   // (none left: the CTA only takes part in the exchange)
     const bool ok = *abort_flag == 0;
     if (n_slots > 0 && ok) {
       if (warp == 0) {
@@ -337,17 +336,17 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
           for (int j = 0; j < n_slots; ++j) {
             if (!__any_sync(0xffffffffu, mine == j)) continue;
             for (int r = 0; r < R; r += 8) {
-              for (uint32_t acc = 0; acc <= second; acc += 128u) {
-                uint32_t x[8];
-                tmem_ld_32x8(lanes + acc + j * slot_cols + r, x);
-                tmem_ld_wait();
-                if (mine == j) {
-                  const uint32_t to = dst + r * 4u + acc * (static_cast<uint32_t>(pitch) * 4u);   // 128 rows further on
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
-                               : "memory");
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16u), "r"(x[4]), "r"(x[5]), "r"(x[6]),
-                               "r"(x[7])
-                               : "memory");
+              uint32_t x[8], y[8];
+              tmem_ld_32x8(lanes + j * slot_cols + r, x);
+              if (second != 0u) tmem_ld_32x8(lanes + second + j * slot_cols + r, y);
+              tmem_ld_wait();
+              if (mine == j) {
+                const uint32_t to = dst + r * 4u, to2 = to + 128u * 4u * static_cast<uint32_t>(pitch);
+                st_shared_v4(to, x[0], x[1], x[2], x[3]);
+                st_shared_v4(to + 16u, x[4], x[5], x[6], x[7]);
+                if (second != 0u) {
+                  st_shared_v4(to2, y[0], y[1], y[2], y[3]);
+                  st_shared_v4(to2 + 16u, y[4], y[5], y[6], y[7]);
                 }
               }
             }
@@ -363,7 +362,7 @@ __device__ __forceinline__ void lora_low_body(const LowParams& p, const int bloc
     cluster_arrive();
     cluster_wait();
     // This CTA's share of the rows, summed over the parts' sums in their order.
-    const int share = idle ? 0 : 128 / parts, quads = R / 4;
+    const int share = 128 >> parts_log, quads = R / 4;
     for (int i = threadIdx.x; i < share * quads; i += Cfg::kThreads) {
       const int row = part * share + i / quads, r = i % quads * 4;
       const long m = static_cast<long>(tile) * 128 + row;

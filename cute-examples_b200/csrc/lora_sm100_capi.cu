@@ -220,12 +220,10 @@ void cut_low(LowParams* p, int adapters, int sm_count) {
   const long tiles = ceil_div(M, 128), k_blocks = ceil_div(p->L, 64), room = 2L * sm_count;
   p->splits = 8;
   while (p->splits > 1 && (tiles * p->splits > room || p->splits > k_blocks)) p->splits /= 2;
-  p->workers = p->splits;
   const long tile_rows = M < kLoraTileRows ? M : kLoraTileRows;
   const long most_groups = ceil_div(adapters < tile_rows ? adapters : tile_rows, p->group_slots);
   const long groups = room / (tiles * p->splits);
   p->groups = static_cast<int>(groups < 1 ? 1 : (groups > most_groups ? most_groups : groups));
-  p->clusters = p->groups;
 }
 
 // ---- product: which tiles
@@ -470,20 +468,18 @@ LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behin
     wanted += tiles * params[i]->splits * params[i]->groups;
   }
   const bool fold = problems > 1 && wanted > 2L * sm_count && params[0]->R <= LowConfig<false>::kMaxFoldedRank;
-  bool long_runs = false;
   for (int i = 0; i < problems; ++i) {
-    LowParams& p = *params[i];
-    if (fold && p.groups > 1)
-      p.clusters = static_cast<int>(ceil_div(p.groups, 2));
-    else if (fold && p.splits > 1)
-      p.workers = p.splits / 2;
-    if (p.workers > g.cluster) g.cluster = p.workers;
-    if (ceil_div(p.L, 64) >= 8L * p.workers) long_runs = true;
+    const int ctas = fold && params[i]->groups == 1 ? params[i]->splits / 2 : params[i]->splits;
+    if (ctas > g.cluster) g.cluster = ctas;
   }
+  bool long_runs = false;
   long total = 0;
   for (int i = 0; i < problems; ++i) {
-    g.ctas[i] = tiles * params[i]->clusters * g.cluster;
+    LowParams& p = *params[i];
+    p.clusters = static_cast<int>(ceil_div(static_cast<long>(p.groups) * p.splits, (fold ? 2L : 1L) * g.cluster));
+    g.ctas[i] = tiles * p.clusters * g.cluster;
     total += g.ctas[i];
+    if (ceil_div(p.L, 64) >= 8L * g.cluster) long_runs = true;
   }
   g.deep = long_runs && 2 * total <= sm_count && total + 2L * behind > 2L * sm_count;
   return g;

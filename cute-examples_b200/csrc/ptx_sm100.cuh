@@ -114,6 +114,11 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, uint32_t a,
                : "memory");
 }
 
+// 16-byte store to this CTA's shared memory.
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // 16-byte load from the shared memory of a CTA of this cluster (address from map_to_cta).
 __device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
   float4 v;
