@@ -574,8 +574,9 @@ int launch_grad(const gemm_sm100_lora_args& a, const GradSide& down, const GradS
   }
   p.split_rows = static_cast<int>(ceil_div(a.M, splits));
   if (p.split_rows < 128) p.split_rows = 128;
-  const long most = ceil_div(p.tiles, 1) * a.adapters;
-  e = launch_cluster(kernel, (most < clusters ? most : clusters) * kGradCluster, kGradCluster, Cfg::kThreads, Cfg::kSmemBytes,
+  // as many units as there can be (those of adapters without rows write zeros instead)
+  const long units = ceil_div(static_cast<long>(p.tiles) * splits, kGradCluster) * a.adapters;
+  e = launch_cluster(kernel, (units < clusters ? units : clusters) * kGradCluster, kGradCluster, Cfg::kThreads, Cfg::kSmemBytes,
                      stream, p);
   return e == cudaSuccess ? GEMM_SM100_OK : set_cuda_error(cuda_error_out, e);
 }
