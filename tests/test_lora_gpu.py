@@ -758,3 +758,67 @@ def test_low_rows_through_the_deep_ring(gk, M, N, K, R, G, kind, deep, dtype):
     for name, value in zip(("dA", "d_down", "d_up"), grads):
         check(name, value, res, tol)
     gk.device_status()
+
+
+@pytest.mark.parametrize("M,K,R,G,kind", [(1, 64, 8, 3, "own"), (77, 1032, 24, 5, "random"), (300, 520, 128, 9, "runs"), (2500, 1024, 16, 4, "runs"),
+                                          (900, 264, 40, 60, "random"), (64, 14336, 64, 32, "own")])
+def test_low_rows_as_a_call_of_their_own(gk, M, K, R, G, kind):
+    """gemm_sm100_lora_low without B and up: the rows that a forward pass leaves, bit for bit, also with a pitch."""
+    import ctypes
+
+    from conftest import load_capi
+    from test_lora_host import LoraArgs
+
+    t = make(M, 72, K, R, G, torch.bfloat16, 1000 + M, id_pattern(kind, M, G, 3))
+    plan = gk.LoraPlan(t["ids"], G)
+    low = torch.empty(M, R, dtype=torch.bfloat16, device="cuda")
+    gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low)
+    wide = torch.full((M + 1, R + 16), 3.0, dtype=torch.bfloat16, device="cuda")
+    args = LoraArgs(M=M, N=72, K=K, R=R, adapters=G, dtype=0, A=t["A"].data_ptr(), B=None, down=t["down"].data_ptr(), up=None, lda=K, ldb=0,
+                    ld_down=K, stride_down=R * K, ld_up=0, stride_up=0, scales=t["scale"].data_ptr(), scale=1.0, plan=plan.buffer.data_ptr())
+    err = ctypes.c_int(0)
+    call = load_capi().gemm_sm100_lora_low
+    call.argtypes = [ctypes.POINTER(LoraArgs), ctypes.c_void_p, ctypes.c_long, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int)]
+    assert call(ctypes.byref(args), wide.data_ptr(), R + 16, torch.cuda.current_stream().cuda_stream, ctypes.byref(err)) == 0
+    gk.device_status()
+    assert torch.equal(wide[:M, :R], low) and bool((wide[:, R:] == 3).all()) and bool((wide[M:] == 3).all())
+    res, tol = want(t)
+    check("low", low, res, tol)
+
+
+def test_threads_that_share_a_stream(gk):
+    """Four host threads on one stream: any kernel of another thread may stand in front of a product that starts before its
+    predecessor has finished.  Plans are refilled in between, and plain products run among them."""
+    import threading
+
+    shared = torch.cuda.Stream()
+    cases = [[make(90 + 150 * i, 264 + 520 * i, 328 + 64 * i, 16, 3 + i, torch.bfloat16, 1100 + 2 * i + j,
+                   id_pattern("random", 90 + 150 * i, 3 + i, j)) for j in range(2)] for i in range(4)]
+    alone = [[run_all(gk, t) for t in pair] for pair in cases]
+    plain = [[gk.gemm_tn(t["A"], t["B"]) for t in pair] for pair in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(shared):
+            plan = gk.LoraPlan(cases[i][0]["ids"], 3 + i)
+            for step in range(40):
+                j = step % 2
+                t = cases[i][j]
+                plan.update(t["ids"])
+                low = torch.empty(t["A"].shape[0], 16, dtype=torch.bfloat16, device="cuda")
+                C = gk.gemm_lora(t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low)
+                other = gk.gemm_tn(t["A"], t["B"])
+                grads = gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"], low=low if step % 3 else None)
+                got = dict(zip(("C", "low", "dA", "d_down", "d_up"), (C, low) + grads))
+                same = [torch.equal(v, alone[i][j][name]) for name, v in got.items()] + [torch.equal(other, plain[i][j])]
+                if not all(same):
+                    wrong.append((i, step, same))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong, wrong[:3]
+    gk.device_status()
