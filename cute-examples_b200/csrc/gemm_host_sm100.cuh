@@ -84,6 +84,7 @@ inline std::atomic<long> g_opt_debug_flags{0};
 inline std::atomic<long> g_opt_group_m{0};
 inline std::atomic<long> g_opt_k_rotate{-1};   // 0 never, 1 always, -1 (default) when there is a single tile row: 3 % on the few-row shapes, 2 = serpentine
 inline std::atomic<long> g_opt_sk_cluster{-1};  // cluster K-split (partial sums through distributed shared memory): -1 planner, 0 never, 1 always where an even split of 2 or 4 is made
+inline std::atomic<long> g_opt_lora_ring{-1};   // ring of the kernel of the low-rank rows: -1 by the launch, 0 short, 1 deep
 inline std::atomic<long> g_opt_pdl{1};        // 1: launch with programmatic stream serialization (overlap with the previous kernel's tail)
 inline std::atomic<long> g_opt_early_prefetch{1};   // with pdl: L2 prefetch of the first stages before waiting for the previous kernel
 inline std::atomic<long> g_opt_tiles_n{0};    // > 0: force this many tiles per tile row (tests), when the configuration allows the widths

@@ -1166,6 +1166,11 @@ int gemm_sm100_set_option(const char* name, long value) {
     g_opt_sk_cluster = value;
     return GEMM_SM100_OK;
   }
+  if (std::strcmp(name, "lora_ring") == 0) {
+    if (value < -1 || value > 1) return GEMM_SM100_ERR_BAD_OPTION;
+    g_opt_lora_ring = value;
+    return GEMM_SM100_OK;
+  }
   if (std::strcmp(name, "pdl") == 0) {
     if (value < 0 || value > 1) return GEMM_SM100_ERR_BAD_OPTION;
     g_opt_pdl = value;

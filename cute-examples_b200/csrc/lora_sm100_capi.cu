@@ -482,6 +482,8 @@ LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behin
     if (ceil_div(p.L, 64) >= 8L * g.cluster) long_runs = true;
   }
   g.deep = long_runs && 2 * total <= sm_count && total + 2L * behind > 2L * sm_count;
+  const long forced = g_opt_lora_ring.load();
+  if (forced >= 0) g.deep = forced != 0;
   return g;
 }
 

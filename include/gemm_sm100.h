@@ -199,6 +199,9 @@ int gemm_sm100_device_status(unsigned int* status_out, int* cuda_error_out);
  *                  per CTA or pair, partial tiles moved between the CTAs' shared memories by
  *                  asynchronous bulk copies; needs no workspace and no co-residency of the grid);
  *                  0 = always through the workspace; -1 = the planner decides (default).
+ *   "lora_ring"    ring of the kernel that computes the low-rank rows of the adapter calls: 0 = three
+ *                  stages and two CTAs per SM, 1 = six and one, -1 = by the launch and the product
+ *                  behind it (default).  The same bits either way.
  *   "balance"      1 = the planner may give a tile row a number of tiles that fills the SMs evenly,
  *                  with tile widths in steps of 64 columns (default); 0 = uniform tiles only.
  *   "pdl"          1 = launch with the programmatic-stream-serialization attribute (default): when

@@ -822,3 +822,21 @@ def test_threads_that_share_a_stream(gk):
         th.join()
     assert not wrong, wrong[:3]
     gk.device_status()
+
+
+@pytest.mark.parametrize("M,N,K,R,G,kind", [(1, 64, 64, 8, 1, "one"), (130, 72, 4000, 24, 4, "runs"), (64, 1024, 1024, 64, 64, "own"),
+                                            (700, 264, 1024, 16, 60, "random"), (2500, 1024, 1024, 16, 4, "runs"), (300, 200, 264, 128, 9, "random")])
+def test_either_ring_gives_the_same_bits(gk, M, N, K, R, G, kind):
+    t = make(M, N, K, R, G, torch.bfloat16, 1200 + M, id_pattern(kind, M, G, 3))
+    plan = gk.LoraPlan(t["ids"], G)
+    got = []
+    try:
+        for ring in (0, 1):
+            gk.set_option("lora_ring", ring)
+            got.append(list(run_all(gk, t).values()) +
+                       list(gk.gemm_lora_backward(t["dC"], t["A"], t["B"], t["down"], t["up"], plan, scale=t["scale"])))
+    finally:
+        gk.set_option("lora_ring", -1)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    gk.device_status()

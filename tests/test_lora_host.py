@@ -238,3 +238,17 @@ def test_few_rows_beside_the_low_rows(shape, chosen):
     import gemm_kernels as gk
 
     assert gk.describe_lora_plan(*shape).startswith("few rows: " + chosen)
+
+
+def test_ring_option():
+    import gemm_kernels as gk
+
+    try:
+        for value, words in ((1, "deep ring"), (0, "short ring"), (-1, "short ring")):
+            gk.set_option("lora_ring", value)
+            assert gk.describe_lora_plan(1, 4096, 4096, 16, 4).endswith(words)
+        for value in (-2, 2):
+            with pytest.raises(RuntimeError, match="unknown option or value"):
+                gk.set_option("lora_ring", value)
+    finally:
+        gk.set_option("lora_ring", -1)
