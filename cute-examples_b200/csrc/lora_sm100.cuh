@@ -56,8 +56,10 @@ __device__ __forceinline__ int lora_read_id(const void* ids, int ids_are_64, lon
 
 // One launch, 256 threads a block.  Block t < tiles: the slot list of tile t.  Block tiles + g: the rows of
 // adapter g in ascending order; their place in `order` is the number of rows of adapters below g,
-// which the block counts itself, so that no block waits for another (adapters x M ids read from L2:
-// 2 MB for 64 adapters and 8192 rows).
+// which the block counts itself, so that no block waits for another.  Every adapter's block reads all indices from L2, and
+// reads them again if the adapter has rows: for 64 adapters and 8192 rows 4 MB of 32-bit indices, 8 MB of 64-bit ones.
+// Measured: 128 rows of 16 adapters 4.0 us, 1024 of 64 8.7, 8192 of up to 64 8.9 (the chain of 32 blocks of 256 rows is what
+// takes the time), 8192 of 4096 100, 65536 of 64 98.
 __global__ void __launch_bounds__(256) lora_plan_kernel(const void* ids, int ids_are_64, int M, int adapters, void* plan) {
   const LoraPlanView v = lora_plan_view(plan, M);
   const int tiles = static_cast<int>(lora_plan_tiles(M));
@@ -146,14 +148,15 @@ __host__ __device__ constexpr int rank_chunk(int R) { return R <= 16 ? 16 : (R <
 
 // ------------------------------------------------------------------------------ low-rank rows
 // low[m] = s_g P[m] W_g^T over the long axis L: P = A and W = down [R, L], or (kRankInner) P = dC and W = up
-// [L, R].  A tile of 128 rows is one MMA operand; the adapters of the tile's rows lie side by side along
+// [L, R].  A tile of 128 rows is one MMA operand; the adapters of the plan's tile (256 rows: this tile's and its
+// neighbour's, so an adapter that only the neighbour uses is multiplied in vain) lie side by side along
 // the MMA's N, in groups of up to 128 columns, so that P is read once however many adapters a group
 // holds, and every row takes its own adapter's columns out of the accumulator.  The work is a read of
-// P and of the adapters in use: bytes, not products, bound it.  L is cut over the CTAs of a cluster, which
+// P and, per pair of tiles, of its adapters: bytes, not products, bound it.  L is cut over the CTAs of a cluster, which
 // add their partial rows through distributed shared memory in rank order.
-// Measured: 8192 x 4096 with rank 16 18.8 to 20.9 us with a cold L2, 67.7 MB from DRAM (3.2 to 3.6 TB/s; about 5 us of it
-// are launch, first loads and exchange); 8192 x 14336 with rank 64 51 us at 5.0 TB/s; 64 x 14336 with 32 adapters of
-// rank 64 (61 MB, nearly all adapters) 18 us.  Groups of 128 columns because two CTAs with three stages of 32 KB
+// Measured: 8192 x 4096 with rank 16 16.4 to 17.3 us (67.2 MB, 4 TB/s; about 5 us of it are launch, first loads and exchange), with a cold
+// L2 19.5 to 21.7; 8192 x 14336 with rank 64 45 us at 5.4 TB/s; 64 x 14336 with 32 adapters of
+// rank 64 (61 MB, nearly all adapters) 19.7 us.  Groups of 128 columns because two CTAs with three stages of 32 KB
 // then share an SM; the alternative of one product per adapter and row tile reads P once per adapter.
 struct LowParams {
   CUtensorMap tmap_p;    // [M, L]: boxes of 64 x p_rows

@@ -449,11 +449,12 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
 //
 // Deep ring (six stages, one CTA per SM) or short (three, two CTAs): the deep one is faster by itself, but takes twice the SMs,
 // and the product kernel behind (`behind` CTAs of one per SM, 0 for none) starts on those that are left.  So it is taken where the
-// product would have to wait in any case and the launch keeps to half of the SMs: 12 to 148 tiles of M 16 to 1100, N 1024 to 8192,
-// K 4096 to 14336, the 47 such shapes of a sweep behind a GEMM 0 to 9 % faster, by themselves 0 to 11 % (64 x 8192 x 14336, 16 adapters
-// of rank 64 66.7 -> 62.0 us; 1100 x 2048 x 8192 with one 51.7 -> 49.7), none slower than 0.4 %.  Elsewhere it costs up to 30 %: 700 x 1024 x
-// 8192 with one adapter 26.1 -> 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7, 64 x 4096 x 14336 with 32 50.5 -> 56.6.  (Not
-// measured below eight K blocks per CTA.)
+// product would have to wait in any case and the launch keeps to half of the SMs.  Of a sweep (M 16 to 1500, N 1024 to 8192, K 4096
+// to 14336, 1 to 64 adapters) that is 47 forward shapes, with it 0 to 9 % faster behind a GEMM, 0 to 11 % by themselves and none
+// slower than 0.4 % (64 x 8192 x 14336 with 16 adapters of rank 64 66.7 -> 62.0 us, 1100 x 2048 x 8192 with one 51.7 -> 49.7), and of
+// backward passes 24 shapes with kept rows (0 to 4 % faster) and 30 with both problems in one launch (1 % slower to 5 % faster).
+// Elsewhere the deep ring costs up to 30 %: 700 x 1024 x 8192 with one adapter 26.1 -> 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7,
+// 64 x 4096 x 14336 with 32 46.6 -> 53.9.  (Not measured below eight K blocks per CTA.)
 struct LowGrid {
   int cluster;           // CTAs of a cluster
   long ctas[2];          // of each problem
