@@ -265,9 +265,10 @@ bool few_row_plan(int M, int N, int K, long low_ctas, int sm_count, Plan* out) {
   return true;
 }
 
-// Tiles for 129 to 1024 rows whose output still is less than a wave (at most four tile rows, so that every count of tiles below
-// means hundreds of columns; with more and narrower rows the same counts lost up to 13 %: 9000 x 64 x 512 36.4 -> 41.1,
-// 2048 x 1024 x 1024 30.7 -> 32.4).  The planner counts on all SMs, but the kernel
+// Tiles for more than 128 rows whose output still is less than a wave: up to 1024 rows, dA with K up to 8192 up to 1792 (beyond
+// 1024 rows in the mean 7 % faster for one adapter, 6 % for runs of four, 2 % slower for 16 in every tile: 1300 x 1536 x 1024 43.2, 37.9, 44.5 ->
+// 36.8, 34.4, 45.4; longer contractions 1 % slower in the mean, 12 % faster to 11 % slower).  With more and narrower rows the same
+// counts of tiles lost up to 13 %: 9000 x 64 x 512 36.4 -> 41.1, 2048 x 1024 x 1024 30.7 -> 32.4, dA 3000 x 768 x 14336 173 -> 189.  The planner counts on all SMs, but the kernel
 // of the low rows still holds some when this one starts: CTAs beyond about 100 (fewer for clusters, which want neighbouring
 // SMs) wait for it, and the whole product with them.  About half of the SMs, busy from the start, are then the
 // better choice.  Forced runs of every configuration (M 129 to 1024, output columns 512 to 12288, K 512 to 16384), and the choice below
@@ -292,7 +293,7 @@ bool few_row_plan(int M, int N, int K, long low_ctas, int sm_count, Plan* out) {
 // (12 such tiles stay with the planner: 128 x 128 tiles cut in four are up to 17 % faster or 7 % slower without a size that
 // tells which: 256 x 1536 x 14336 42.8, 43.8, 57.9 -> 45.8, 46.5, 48.3; 512 x 768 x 14336 49.4, 48.8, 58.3 -> 44.6, 44.9, 60.8.)
 bool half_wave_plan(int M, int N, int K, bool b_is_kn, int sm_count, Plan* out) {
-  if (M <= 128 || M > 1024 || choice_forced()) return false;
+  if (M <= 128 || M > (b_is_kn && K <= 8192 ? 1792 : 1024) || choice_forced()) return false;
   const long rows = ceil_div(M, 256), wide = rows * ceil_div(N, 256), narrow = rows * ceil_div(N, 128);
   const long half = sm_count / 4;                          // pair tiles on half of the SMs
   int config = -1, factor = 1;

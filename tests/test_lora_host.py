@@ -252,3 +252,12 @@ def test_ring_option():
                 gk.set_option("lora_ring", value)
     finally:
         gk.set_option("lora_ring", -1)
+
+
+@pytest.mark.parametrize("shape,want", [((1166, 8192, 1704, 24, 9), "less than a wave: config=0 "), ((1792, 1024, 1280, 16, 1), "less than a wave: config=0 "),
+                                        ((1045, 344, 1776, 64, 23), "less than a wave: config=0 "), ((1793, 1024, 1024, 16, 1), "planner: "),
+                                        ((1100, 14336, 1792, 16, 1), "planner: "), ((1024, 14336, 2304, 16, 1), "less than a wave: config=0 ")])
+def test_gradients_of_some_more_rows(shape, want):
+    import gemm_kernels as gk
+
+    assert gk.describe_lora_plan(*shape, gradient=True).startswith(want)
