@@ -449,19 +449,26 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
 // (4096 x 4096 x 4096, eight adapters of rank 64) and 94.1 instead of 89.3 (2048 x 4096 x 4096, 16 of rank 32 in every tile).
 //
 // Deep ring (six stages, one CTA per SM) or short (three, two CTAs): the deep one is faster by itself, but takes twice the SMs,
-// and the product kernel behind (`behind` CTAs of one per SM, 0 for none) starts on those that are left.  So it is taken where the
-// product would have to wait in any case and the launch keeps to half of the SMs.  Of a sweep (M 16 to 1500, N 1024 to 8192, K 4096
-// to 14336, 1 to 64 adapters) that is 47 forward shapes, with it 0 to 9 % faster behind a GEMM, 0 to 11 % by themselves and none
-// slower than 0.4 % (64 x 8192 x 14336 with 16 adapters of rank 64 66.7 -> 62.0 us, 1100 x 2048 x 8192 with one 51.7 -> 49.7), and of
-// backward passes 24 shapes with kept rows (0 to 4 % faster) and 30 with both problems in one launch (1 % slower to 5 % faster).
-// Elsewhere the deep ring costs up to 30 %: 700 x 1024 x 8192 with one adapter 26.1 -> 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7,
-// 64 x 4096 x 14336 with 32 46.6 -> 53.9.  (Not measured below eight K blocks per CTA.)
+// and the product kernel `behind` (no CTAs: none) starts on those that are left.  So it is taken where the product would
+// have to wait in any case and the launch keeps to half of the SMs: in a sweep of 1224 pairs of times (M 16 to 2048, N and K 1024 to
+// 14336, 1 to 64 adapters; forward behind a GEMM and alone, backward with low rows kept and in one launch) 218 pairs, 1 % slower to 11 %
+// faster, 2.9 % faster in the mean (64 x 8192 x 14336 with 16 adapters of rank 64 66.7 -> 62.0 us, 1100 x 2048 x 8192 with one 51.7 ->
+// 49.7, 128 x 4096 x 8192 with eight 33.9 -> 31.5).  And where a launch of up to 32 CTAs and the product fit beside one another: 332 pairs,
+// 2.6 % slower to 3.6 % faster, 0.1 % in the mean (a training step of 114 x 17328 x 2912 with ten of rank 24 102 -> 89 us).  Elsewhere the deep ring costs up to 30 %: 700 x 1024 x 8192 with one adapter 26.1 ->
+// 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7, 64 x 4096 x 14336 with 32 46.6 -> 53.9.  (Not measured below eight K blocks per CTA.)
 struct LowGrid {
   int cluster;           // CTAs of a cluster
   long ctas[2];          // of each problem
   bool deep;
 };
-LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behind, int sm_count) {
+// SMs that the product behind wants: its CTAs, one per SM, and an eighth more where clusters of four or more of them have to
+// find room in the GPCs.
+int wanted_sms(const Plan& plan, int sm_count) {
+  const int cluster = plan.split_k ? plan.split_factor * kConfigs[plan.config].cta_group : 1;
+  return plan.ctas + (cluster >= 4 ? sm_count / 8 : 0);
+}
+
+LowGrid low_grid(LowParams* const* params, int problems, int adapters, const Plan& behind, int sm_count) {
   LowGrid g = {1, {0, 0}, false};
   const long tiles = ceil_div(params[0]->M, 128);
   long wanted = 0;
@@ -483,7 +490,9 @@ LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behin
     total += g.ctas[i];
     if (ceil_div(p.L, 64) >= 8L * g.cluster) long_runs = true;
   }
-  g.deep = long_runs && 2 * total <= sm_count && total + 2L * behind > 2L * sm_count;
+  const bool no_room = 2 * total <= sm_count && total + 2L * wanted_sms(behind, sm_count) > 2L * sm_count;
+  const bool room_for_both = total <= 32 && total + wanted_sms(behind, sm_count) <= sm_count;
+  g.deep = long_runs && (no_room || room_for_both);
   const long forced = g_opt_lora_ring.load();
   if (forced >= 0) g.deep = forced != 0;
   return g;
@@ -491,7 +500,7 @@ LowGrid low_grid(LowParams* const* params, int problems, int adapters, int behin
 
 template <bool kIsBf16, bool kRankInner>
 int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const void* W, long ld_w, long stride_w, int L, void* out,
-               long ld_out, int behind, cudaStream_t stream, int* cuda_error_out) {
+               long ld_out, const Plan& behind, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
@@ -513,7 +522,7 @@ int launch_low(const gemm_sm100_lora_args& a, const void* P, long ldp, const voi
 // low (from A and down) and d_low (from dC and up) in one launch.
 template <bool kIsBf16>
 int launch_low_pair(const gemm_sm100_lora_args& a, void* low, long ld_low, const void* dC, long ld_dc, void* d_low, long ld_d_low,
-                    int behind, cudaStream_t stream, int* cuda_error_out) {
+                    const Plan& behind, cudaStream_t stream, int* cuda_error_out) {
   DeviceState* st = nullptr;
   int rc = ready(&st, cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
@@ -616,7 +625,7 @@ int prepare_type(DeviceState& st, int* cuda_error_out, std::integer_sequence<int
 }
 
 // The low-rank rows of A; the caller has checked what all calls share.
-int low_rows(const gemm_sm100_lora_args& a, void* low, long ld_low, int behind, cudaStream_t stream, int* cuda_error_out) {
+int low_rows(const gemm_sm100_lora_args& a, void* low, long ld_low, const Plan& behind, cudaStream_t stream, int* cuda_error_out) {
   if (!a.plan) return GEMM_SM100_ERR_NULL_POINTER;
   int rc = check_matrix(a.A, a.K, a.lda);
   if (rc || (rc = check_down(a)) || (rc = check_matrix(low, a.R, ld_low))) return rc;
@@ -677,7 +686,7 @@ int gemm_sm100_lora_describe_plan(int M, int N, int K, int R, int adapters, int 
   std::memset(&low, 0, sizeof(low));
   low_shape(&low, M, R, gradient ? N : K, gradient != 0);
   LowParams* const one[1] = {&low};
-  const LowGrid grid = low_grid(one, 1, adapters, plan.ctas, current_sm_count());
+  const LowGrid grid = low_grid(one, 1, adapters, plan, current_sm_count());
   const size_t used = std::strlen(buf);
   std::snprintf(buf + used, buf_bytes - used, "; low rows: %ld ctas in clusters of %d, %s ring", grid.ctas[0], grid.cluster,
                 grid.deep ? "deep" : "short");
@@ -689,7 +698,7 @@ int gemm_sm100_lora_low(const gemm_sm100_lora_args* args, void* low, long ld_low
   if (!args) return GEMM_SM100_ERR_NULL_POINTER;
   const int rc = check_common(*args);
   if (rc != GEMM_SM100_OK || args->M == 0) return rc;
-  return low_rows(*args, low, ld_low, /*behind=*/0, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
+  return low_rows(*args, low, ld_low, /*behind=*/Plan{}, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
 }
 
 int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* low, long ld_low, void* cuda_stream,
@@ -703,7 +712,7 @@ int gemm_sm100_lora(const gemm_sm100_lora_args* args, void* C, long ldc, void* l
   if ((rc = check_matrix(a.B, a.K, a.ldb)) || (rc = check_up(a)) || (rc = check_matrix(C, a.N, ldc))) return rc;
   const char* rule;
   const Plan plan = product_plan(a.M, a.N, a.K, /*b_is_kn=*/false, a.R, a.adapters, current_sm_count(), &rule);
-  rc = low_rows(a, low, ld_low, plan.ctas, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
+  rc = low_rows(a, low, ld_low, plan, static_cast<cudaStream_t>(cuda_stream), cuda_error_out);
   if (rc != GEMM_SM100_OK) return rc;
   const Problem p{a.A, a.B, C, a.M, a.N, a.K, a.lda, a.ldb, ldc, a.dtype};
   const AdapterOperands o{low, ld_low, a.up, a.ld_up, a.stride_up, a.R, a.adapters, a.plan};
@@ -746,13 +755,13 @@ int gemm_sm100_lora_backward(const gemm_sm100_lora_args* args, const void* dC, l
   if (dA || d_down) {
     if ((rc = check_up(a)) || (rc = check_matrix(d_low, a.R, ld_d_low))) return rc;
     if (again)
-      rc = (bf16 ? launch_low_pair<true> : launch_low_pair<false>)(a, low, ld_low, dC, ld_dc, d_low, ld_d_low, plan.ctas, stream,
+      rc = (bf16 ? launch_low_pair<true> : launch_low_pair<false>)(a, low, ld_low, dC, ld_dc, d_low, ld_d_low, plan, stream,
                                                                        cuda_error_out);
     else
       rc = (bf16 ? launch_low<true, true> : launch_low<false, true>)(a, dC, ld_dc, a.up, a.ld_up, a.stride_up, a.N, d_low,
-                                                                     ld_d_low, plan.ctas, stream, cuda_error_out);
+                                                                     ld_d_low, plan, stream, cuda_error_out);
   } else if (again) {
-    rc = low_rows(a, low, ld_low, /*behind=*/0, stream, cuda_error_out);
+    rc = low_rows(a, low, ld_low, /*behind=*/plan, stream, cuda_error_out);
   }
   if (rc != GEMM_SM100_OK) return rc;
   if (dA) {

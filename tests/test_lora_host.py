@@ -214,12 +214,15 @@ def test_twelve_narrow_tiles_are_left_to_the_planner(shape):
 
 
 @pytest.mark.parametrize("shape,gradient,low", [
-    # the deep ring only where the product behind finds no room beside the short one either
+    # the deep ring where the product behind finds no room beside the short one either
     ((64, 8192, 14336, 64, 16), False, "64 ctas in clusters of 8, deep"), ((1100, 2048, 8192, 64, 1), False, "72 ctas in clusters of 8, deep"),
     ((16, 8192, 8192, 64, 8), False, "32 ctas in clusters of 8, short"), ((700, 1024, 8192, 64, 1), False, "48 ctas in clusters of 8, short"),
     ((512, 4096, 8192, 64, 1), False, "32 ctas in clusters of 8, short"), ((64, 4096, 14336, 64, 32), False, "128 ctas in clusters of 8, short"),
     ((128, 14336, 4096, 16, 64), False, "64 ctas in clusters of 8, short"), ((1100, 8192, 2048, 64, 1), True, "72 ctas in clusters of 8, deep"),
     ((64, 14336, 2048, 64, 16), True, "64 ctas in clusters of 8, short"),
+    # (the clusters of a product that is cut along K want more of it), or where few CTAs and the product both have their own SMs
+    ((128, 4096, 8192, 64, 8), False, "32 ctas in clusters of 8, deep"), ((128, 8192, 8192, 64, 8), False, "32 ctas in clusters of 8, short"),
+    ((66, 27248, 8160, 88, 2), True, "16 ctas in clusters of 8, deep"), ((300, 4096, 8192, 64, 1), False, "24 ctas in clusters of 8, short"),
 ])
 def test_ring_of_the_low_rows(shape, gradient, low):
     import gemm_kernels as gk
@@ -246,7 +249,7 @@ def test_ring_option():
     try:
         for value, words in ((1, "deep ring"), (0, "short ring"), (-1, "short ring")):
             gk.set_option("lora_ring", value)
-            assert gk.describe_lora_plan(1, 4096, 4096, 16, 4).endswith(words)
+            assert gk.describe_lora_plan(700, 1024, 8192, 64, 1).endswith(words)
         for value in (-2, 2):
             with pytest.raises(RuntimeError, match="unknown option or value"):
                 gk.set_option("lora_ring", value)
