@@ -455,7 +455,9 @@ int low_params(LowParams* out_params, const gemm_sm100_lora_args& a, bool rank_i
 // faster, 2.9 % faster in the mean (64 x 8192 x 14336 with 16 adapters of rank 64 66.7 -> 62.0 us, 1100 x 2048 x 8192 with one 51.7 ->
 // 49.7, 128 x 4096 x 8192 with eight 33.9 -> 31.5).  And where a launch of up to 32 CTAs and the product fit beside one another: 332 pairs,
 // 2.6 % slower to 3.6 % faster, 0.1 % in the mean (a training step of 114 x 17328 x 2912 with ten of rank 24 102 -> 89 us).  Elsewhere the deep ring costs up to 30 %: 700 x 1024 x 8192 with one adapter 26.1 ->
-// 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7, 64 x 4096 x 14336 with 32 46.6 -> 53.9.  (Not measured below eight K blocks per CTA.)
+// 31.8 us, 16 x 8192 x 8192 with eight 33.2 -> 39.7, 64 x 4096 x 14336 with 32 46.6 -> 53.9.  On more than half of
+// the SMs it depends on the rows' order, which the host does not know: backward pass of 1024 x 8192 x 1024 with two adapters of rank 128,
+// rows in order 51.1 -> 49.1 (half of the CTAs have no adapters), mixed 51.5 -> 56.6.  (Not measured below eight K blocks per CTA.)
 struct LowGrid {
   int cluster;           // CTAs of a cluster
   long ctas[2];          // of each problem
